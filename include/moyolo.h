@@ -607,6 +607,19 @@ int moy_msda_prep(const float* offaw, int64_t ld, int col_off, int col_aw, const
 /* x T [M, N] (ld): rows with mask[m] != 0 are zeroed (value.masked_fill_(input_padding_mask[..., None], 0), ms_deform_attn.py:95-96). */
 int moy_mask_rows(void* x, int64_t ld, int M, int N, const uint8_t* mask, int dtype, void* stream);
 
+/* ---- operators a transformer layer is trained with (csrc/layer_norm.hip) ----
+ * Layer norm over the last axis, s = x (+ r):  y = (s - mean(s)) / sqrt(var(s) + eps) * w + b  (var: the biased one).
+ * x, r, y T [rows, C] with row strides ldx / ldr / ldy in elements (any alignment of T; ldx and ldr may be 0); r, w, b optional; w, b [C] fp32 or T
+ * (w_dtype).  mean / rstd fp32 [rows]: both or neither, what moy_layer_norm_bwd takes.  C up to 16384 (16-bit T) or 8192 (fp32), else MOY_ENOSYS. */
+int moy_layer_norm(const void* x, int64_t ldx, const void* r, int64_t ldr, const void* w, const void* b, int w_dtype, int64_t rows, int C,
+                   float eps, void* y, int64_t ldy, float* mean, float* rstd, int dtype, void* stream);
+/* Gradients of moy_layer_norm: dx T [rows, C] (the gradient of x and of r alike), dw / db [C] in w_dtype; each optional, one at least given.  ws
+ * fp32 with ws_len >= moy_layer_norm_bwd_ws(rows, C, dtype) floats where dw or db is given.  dw and db are added in a fixed order. */
+int moy_layer_norm_bwd(const void* dy, int64_t ldd, const void* x, int64_t ldx, const void* r, int64_t ldr, const void* w, int w_dtype,
+                       const float* mean, const float* rstd, int64_t rows, int C, void* dx, int64_t ldo, void* dw, void* db, float* ws,
+                       int64_t ws_len, int dtype, void* stream);
+int64_t moy_layer_norm_bwd_ws(int64_t rows, int C, int dtype);    /* floats, or a negative MOY_E* code */
+
 #ifdef __cplusplus
 }
 #endif

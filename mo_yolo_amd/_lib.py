@@ -140,6 +140,9 @@ SIGNATURES = {
     "moy_query_order": (C.c_int, [vp, C.c_int, C.c_int, C.c_int, C.c_int, vp, vp]),
     "moy_msda_prep": (C.c_int, [vp, i64, C.c_int, C.c_int, vp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, vp, C.c_int, vp, vp, C.c_int, vp]),
     "moy_mask_rows": (C.c_int, [vp, i64, C.c_int, C.c_int, vp, C.c_int, vp]),
+    "moy_layer_norm": (C.c_int, [vp, i64, vp, i64, vp, vp, C.c_int, i64, C.c_int, f32, vp, i64, vp, vp, C.c_int, vp]),
+    "moy_layer_norm_bwd": (C.c_int, [vp, i64, vp, i64, vp, i64, vp, C.c_int, vp, vp, i64, C.c_int, vp, i64, vp, vp, vp, i64, C.c_int, vp]),
+    "moy_layer_norm_bwd_ws": (i64, [i64, C.c_int, C.c_int]),
 }
 
 _lib = None

@@ -305,6 +305,37 @@ class MSDeformAttnFunction(torch.autograd.Function):
         return gv, None, None, gl, ga, None
 
 
+class LayerNormFunction(torch.autograd.Function):
+    """Autograd of ops.layer_norm_forward: gradients for x, weight, bias and the residual (x and the residual share theirs)."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps, residual):
+        y, mean, rstd = ops.layer_norm_forward(x, weight, bias, eps, residual, stats=True)
+        ctx.save_for_backward(x, weight, residual, mean, rstd)
+        ctx.weight_dtype = None if bias is None else bias.dtype
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, weight, residual, mean, rstd = ctx.saved_tensors
+        nx, nw, nb, _, nr = ctx.needs_input_grad
+        dx, dw, db = ops.layer_norm_backward(dy, x, weight, mean, rstd, residual, need=(nx or nr, nw, nb), weight_dtype=ctx.weight_dtype)
+        return dx if nx else None, dw, db, None, dx if nr else None
+
+
+def _wants_grad(*ts):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5, residual=None):
+    """Layer norm of x (+ residual) over the last axis (the post-norms of transformer.py:515-652, `norm(tgt + tgt2)`), differentiable; without a
+    gradient to compute, the forward alone.  weight / bias [C] in x's type or float32."""
+    if _wants_grad(x, weight, bias, residual):
+        return LayerNormFunction.apply(x, weight, bias, eps, residual)
+    return ops.layer_norm_forward(x, weight, bias, eps, residual)
+
+
 class MSDeformAttn(nn.Module):
     """transformer.py:193-287 (d_model 256, 8 heads, 4 points, <= 4 levels, 4-d reference boxes)."""
 

@@ -511,3 +511,117 @@ def sigmoid_f32(x):
     out = torch.empty_like(x)
     L.check(L.lib().moy_sigmoid_f32(x.data_ptr(), x.numel(), out.data_ptr(), _st()), "moy_sigmoid_f32")
     return out
+
+
+# ----------------------------------------------------------------------------- operators of a trained transformer layer
+class _NoGuard:
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return False
+
+
+_NO_GUARD = _NoGuard()
+
+
+def _on(t):
+    """The tensor's device as the current one for a launch (its current stream is what _st() then names)."""
+    return _NO_GUARD if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _one_device(*ts):
+    _need_gpu(*ts)
+    dev = None
+    for t in ts:
+        if t is not None:
+            dev = dev or t.device
+            if t.device != dev:
+                raise ValueError(f"tensors on {dev} and {t.device}")
+
+
+def _as_rows(t, what):
+    """[..., C] -> a 2-D view [rows, C] with unit column stride (a copy where the strides allow none)."""
+    if t.dim() == 0:
+        raise ValueError(f"{what}: at least one axis expected")
+    t = t if t.dim() == 2 else t.reshape(-1, t.shape[-1]) if t.shape[-1] else t.reshape(0, 0)
+    return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
+
+
+def _norm_check(x, weight, bias, residual, *more):
+    _one_device(x, weight, bias, residual, *more)
+    code = _code(x)
+    if x.dim() == 0 or x.shape[-1] == 0:
+        raise ValueError("layer_norm: x must be [..., C] with C > 0")
+    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
+        raise ValueError("layer_norm: residual must have x's shape and type")
+    wdt = None
+    for t in (weight, bias):
+        if t is not None:
+            if t.dim() != 1 or t.shape[0] != x.shape[-1] or t.dtype not in (x.dtype, torch.float32) or (wdt or t.dtype) != t.dtype:
+                raise ValueError("layer_norm: weight and bias must be [C], both in x's type or both float32")
+            wdt = t.dtype
+    return code, L.F32 if wdt in (None, torch.float32) else code
+
+
+def layer_norm_forward(x, weight=None, bias=None, eps=1e-5, residual=None, stats=False):
+    """Layer norm of x (+ residual) over the last axis (moy_layer_norm); weight / bias [C] in x's type or float32.  float32 / bfloat16 /
+    float16, any leading shape and row stride.  -> y, or with stats (y, mean, rstd) as layer_norm_backward takes them (fp32, one per row)."""
+    code, wcode = _norm_check(x, weight, bias, residual)
+    if not eps >= 0:
+        raise ValueError("layer_norm: eps must not be negative")
+    x2 = _as_rows(x, "x")
+    r2 = None if residual is None else _as_rows(residual, "residual")
+    rows, c = x2.shape
+    w, b = (None if t is None else t.contiguous() for t in (weight, bias))
+    with _on(x):
+        y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+        mean = rstd = None
+        if stats:
+            mean, rstd = torch.empty(2, rows, device=x.device, dtype=torch.float32).unbind(0)
+        if rows:
+            L.check(L.lib().moy_layer_norm(x2.data_ptr(), x2.stride(0), _ptr(r2), 0 if r2 is None else r2.stride(0), _ptr(w), _ptr(b), wcode, rows, c,
+                                           eps, y.data_ptr(), c, _ptr(mean), _ptr(rstd), code, _st()), "moy_layer_norm")
+    return (y, mean, rstd) if stats else y
+
+
+def layer_norm_backward(dy, x, weight, mean, rstd, residual=None, need=(True, True, True), weight_dtype=None):
+    """Gradients of layer_norm_forward (moy_layer_norm_bwd): (dx, dweight, dbias); dx is the gradient of x and of the residual alike.  need: which of
+    the three are computed (None in the others' place); weight_dtype: the type of dweight / dbias where weight is None (float32)."""
+    code, wcode = _norm_check(x, weight, None, residual, dy, mean, rstd)
+    if weight is None and weight_dtype is not None:
+        if weight_dtype not in (x.dtype, torch.float32):
+            raise ValueError("layer_norm_backward: weight_dtype is x's type or float32")
+        wcode = L.F32 if weight_dtype == torch.float32 else code
+    if dy.shape != x.shape or dy.dtype != x.dtype:
+        raise ValueError("layer_norm_backward: dy must have x's shape and type")
+    x2, g2 = _as_rows(x, "x"), _as_rows(dy, "dy")
+    rows, c = x2.shape
+    for t in (mean, rstd):
+        if t.dtype != torch.float32 or t.numel() != rows or not t.is_contiguous():
+            raise ValueError("layer_norm_backward: mean and rstd must be contiguous float32, one per row")
+    if not any(need):
+        return None, None, None
+    r2 = None if residual is None else _as_rows(residual, "residual")
+    w = None if weight is None else weight.contiguous()
+    wdt = torch.float32 if wcode == L.F32 else x.dtype
+    with _on(x):
+        dx = torch.empty(x.shape, device=x.device, dtype=x.dtype) if need[0] else None
+        dw, db = (torch.empty(c, device=x.device, dtype=wdt) if n else None for n in need[1:])
+        if rows == 0:
+            for t in (dw, db):
+                if t is not None:
+                    t.zero_()
+            return dx, dw, db
+        n = L.lib().moy_layer_norm_bwd_ws(rows, c, code) if (need[1] or need[2]) else 0
+        if n < 0:
+            L.check(n, "moy_layer_norm_bwd_ws")
+        ws = torch.empty(n, device=x.device, dtype=torch.float32) if n else None
+        L.check(L.lib().moy_layer_norm_bwd(g2.data_ptr(), g2.stride(0), x2.data_ptr(), x2.stride(0), _ptr(r2), 0 if r2 is None else r2.stride(0), _ptr(w),
+                                           wcode, mean.data_ptr(), rstd.data_ptr(), rows, c, _ptr(dx), c, _ptr(dw), _ptr(db), _ptr(ws), n, code,
+                                           _st()), "moy_layer_norm_bwd")
+    return dx, dw, db
