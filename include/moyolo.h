@@ -620,6 +620,38 @@ int moy_layer_norm_bwd(const void* dy, int64_t ldd, const void* x, int64_t ldx, 
                        int64_t ws_len, int dtype, void* stream);
 int64_t moy_layer_norm_bwd_ws(int64_t rows, int C, int dtype);    /* floats, or a negative MOY_E* code */
 
+/* ---- attention with a learned relative position bias by buckets (csrc/attention.hip)
+ *   S[i, j] = scale * q_i . k_j + table[lut[clamp(j - (i + start), -max_distance, max_distance) + max_distance], h]
+ *   o_i = sum_j softmax_j(S)[i, j] v_j  over the keys that count; a query without one: zeros (and no gradient).
+ * q T [B, Lq, H, D], k / v T [B, Lk, Hk, D] (H % Hk == 0: query head h takes key head h / (H / Hk)), D % 8 == 0 up to 128 (else MOY_ENOSYS), any
+ * strides of whole 16-byte steps (sb batch, sl token, sh head, in elements), 16-byte aligned bases.  o T [B, Lq, H, D] dense; lse fp32 [B, H, Lq]
+ * (optional; what the backward takes).
+ * table T [num_buckets <= 64, H] with lut uint8 [2 max_distance + 1] (device; entries past num_buckets count as the last), max_distance <= 1024; both NULL: no
+ * bias.  Key j counts iff j < k_len[b] (int32 [B], device, clamped to [0, Lk]; NULL: Lk), and j <= i + start if causal, and mask (uint8, strides m_sb,
+ * m_sh, m_sq, key stride 1; NULL: none) is 0 there.  start = q_start, or with q_from_end k_len[b] - Lq (the queries are the last tokens of the cache).
+ * Rows of k / v from k_len on are not read, nor those that a mask without query and head strides (m_sq == m_sh == 0) hides; a key that such a rule does not
+ * hide has to be finite wherever any query counts it or not (its weight 0 still multiplies it).
+ * ws: fp32 workspace of moy_attention_ws / moy_attention_bwd_ws floats (0: none needed; negative: a MOY_E* code).
+ * Backward: dout T [B, Lq, H, D] strided (g_*), the forward's o and lse; dq dense like o, dk / dv dense [B, Lk, Hk, D] (zeros from k_len on), dtable T
+ * [num_buckets, H]; each optional, one at least given.  16-bit types: P and dS are rounded to T for the matrix cores, sums are fp32; nothing is
+ * added in an order that depends on the launch. */
+typedef struct moy_attention_args {
+  const void* q; const void* k; const void* v;
+  int64_t q_sb; int64_t q_sl; int64_t q_sh; int64_t k_sb; int64_t k_sl; int64_t k_sh; int64_t v_sb; int64_t v_sl; int64_t v_sh;
+  int32_t B; int32_t H; int32_t Hk; int32_t Lq; int32_t Lk; int32_t D;
+  const void* table; const uint8_t* lut; int32_t num_buckets; int32_t max_distance;
+  const int32_t* k_len; int32_t q_from_end; int32_t q_start; int32_t causal;
+  const uint8_t* mask; int64_t m_sb; int64_t m_sh; int64_t m_sq;
+  float scale; int32_t dtype;
+  void* o; float* lse; float* ws; int64_t ws_len;
+  const void* dout; int64_t g_sb; int64_t g_sl; int64_t g_sh;
+  void* dq; void* dk; void* dv; void* dtable;
+} moy_attention_args;
+int moy_attention(const moy_attention_args* args, void* stream);
+int moy_attention_bwd(const moy_attention_args* args, void* stream);
+int64_t moy_attention_ws(const moy_attention_args* args);
+int64_t moy_attention_bwd_ws(const moy_attention_args* args);
+
 #ifdef __cplusplus
 }
 #endif

@@ -90,6 +90,20 @@ class C2fArgs(C.Structure):
     ]
 
 
+class AttentionArgs(C.Structure):
+    """Mirror of `moy_attention_args` (include/moyolo.h)."""
+    _fields_ = [
+        ("q", vp), ("k", vp), ("v", vp),
+        ("q_sb", i64), ("q_sl", i64), ("q_sh", i64), ("k_sb", i64), ("k_sl", i64), ("k_sh", i64), ("v_sb", i64), ("v_sl", i64), ("v_sh", i64),
+        ("B", i32), ("H", i32), ("Hk", i32), ("Lq", i32), ("Lk", i32), ("D", i32),
+        ("table", vp), ("lut", vp), ("num_buckets", i32), ("max_distance", i32),
+        ("k_len", vp), ("q_from_end", i32), ("q_start", i32), ("causal", i32),
+        ("mask", vp), ("m_sb", i64), ("m_sh", i64), ("m_sq", i64), ("scale", f32), ("dtype", i32),
+        ("o", vp), ("lse", vp), ("ws", vp), ("ws_len", i64),
+        ("dout", vp), ("g_sb", i64), ("g_sl", i64), ("g_sh", i64), ("dq", vp), ("dk", vp), ("dv", vp), ("dtable", vp),
+    ]
+
+
 # name -> (restype, argtypes); every symbol declared in include/moyolo.h
 SIGNATURES = {
     "moy_version": (C.c_int, []),
@@ -143,6 +157,10 @@ SIGNATURES = {
     "moy_layer_norm": (C.c_int, [vp, i64, vp, i64, vp, vp, C.c_int, i64, C.c_int, f32, vp, i64, vp, vp, C.c_int, vp]),
     "moy_layer_norm_bwd": (C.c_int, [vp, i64, vp, i64, vp, i64, vp, C.c_int, vp, vp, i64, C.c_int, vp, i64, vp, vp, vp, i64, C.c_int, vp]),
     "moy_layer_norm_bwd_ws": (i64, [i64, C.c_int, C.c_int]),
+    "moy_attention": (C.c_int, [C.POINTER(AttentionArgs), vp]),
+    "moy_attention_bwd": (C.c_int, [C.POINTER(AttentionArgs), vp]),
+    "moy_attention_ws": (i64, [C.POINTER(AttentionArgs)]),
+    "moy_attention_bwd_ws": (i64, [C.POINTER(AttentionArgs)]),
 }
 
 _lib = None

@@ -1,0 +1,1049 @@
+// Attention with a learned relative position bias by buckets, forward and backward.
+//
+//   S_ij = scale q_i . k_j + table[lut[clamp(j - (i + start), -far, far) + far], h]     (log2 units here: scale and bias carry log2 e)
+//   P = softmax_j S over the keys that count     O = P V          empty rows: O = 0, no gradient
+//   dP = dO V^T    dS = P (dP - delta), delta_i = dO_i . O_i      dq = scale dS K    dK = scale dS^T Q    dV = P^T dO    dtable[b] = sum of dS in bucket b
+//
+// One pass over the keys with a running maximum and sum (fp32).  All products run on the matrix cores (16x16 tiles; 16-bit types: K = 32 at a time, P and
+// dS rounded to the type for the second products; fp32: exact fp32 products, K = 4 at a time in the same register layout), and are laid out so that
+// probabilities never leave registers: S^T = K Q^T puts a query in a lane's column and four consecutive keys in its accumulator, which is (keys permuted
+// alike on both sides) the operand that O^T = V^T P^T takes.  V^T, K^T, Q^T, dO^T operands come out of row-major LDS tiles through the transposing LDS
+// read (16-bit) or by single elements (fp32).  A row's maximum, sum, delta and position are one lane's scalars; only the maximum crosses lanes.
+//
+// Kernels: attn_fwd_kernel (a block takes 64 * NQ queries of one head, tiles of keys double-buffered in LDS); attn_split_kernel (few queries over a long cache:
+// 16 (query, head of a shared group) rows to a block, the keys split over waves and blocks, partial results joined in split order); attn_dq_kernel (dQ,
+// delta, sums of dtable); attn_dkv_kernel (dK, dV: a block owns keys and walks the queries of every head that shares them).  The two backward kernels
+// compute S twice instead of adding dQ atomically: results do not depend on the order in which blocks run.
+#include "common.hpp"
+
+namespace moy {
+
+constexpr float LOG2E = 1.4426950408889634f;
+
+struct AttnParams {
+  const void *q, *k, *v;
+  int64_t q_sb, q_sl, q_sh, k_sb, k_sl, k_sh, v_sb, v_sl, v_sh;
+  int B, H, Hk, Lq, Lk, D;
+  const void* table; const uint8_t* lut; int nb, far;
+  const int32_t* k_len; int q_from_end, q_start, causal;
+  const uint8_t* mask; int64_t m_sb, m_sh, m_sq;
+  float scale, scale2;                     // scale2 = scale log2 e
+  void* o; float* lse;                     // lse fp32 [B, H, Lq], log2 units; -inf: an empty row
+  const void* dout; int64_t g_sb, g_sl, g_sh;
+  void *dq, *dk, *dv;
+  float* delta;                            // backward: fp32 [B, H, Lq]
+  float* part;                             // backward: fp32 [H][B * query tiles][nb] sums of dS; split forward: partial results
+  int tiles, splits, split_keys;           // row tiles of a (batch, head); key splits of the split forward and their length
+};
+
+// ---- matrix operands: 8 elements of one row / column for a lane (l % 16 = row or column, l / 16 = which eight of 32)
+template <typename T>
+struct Frag {
+  u32x4 w;
+};
+template <>
+struct Frag<float> {
+  f32x4 lo, hi;
+};
+__device__ __forceinline__ f32x4 attn_mma(f32x4 acc, const Frag<bf16_t>& a, const Frag<bf16_t>& b) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a.w), __builtin_bit_cast(bf16x8, b.w), acc, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 attn_mma(f32x4 acc, const Frag<f16_t>& a, const Frag<f16_t>& b) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a.w), __builtin_bit_cast(f16x8, b.w), acc, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 attn_mma(f32x4 acc, const Frag<float>& a, const Frag<float>& b) {
+  acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a.lo.x, b.lo.x, acc, 0, 0, 0);
+  acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a.lo.y, b.lo.y, acc, 0, 0, 0);
+  acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a.lo.z, b.lo.z, acc, 0, 0, 0);
+  acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a.lo.w, b.lo.w, acc, 0, 0, 0);
+  acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a.hi.x, b.hi.x, acc, 0, 0, 0);
+  acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a.hi.y, b.hi.y, acc, 0, 0, 0);
+  acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a.hi.z, b.hi.z, acc, 0, 0, 0);
+  acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a.hi.w, b.hi.w, acc, 0, 0, 0);
+  return acc;
+}
+// two accumulators (rows 4 q .. 4 q + 3 of two 16-row tiles) -> the operand whose lane holds those eight
+template <typename T>
+__device__ __forceinline__ Frag<T> frag_of(const f32x4& a, const f32x4& b) {
+  if constexpr (sizeof(T) == 4) return Frag<T>{a, b};
+  else return Frag<T>{u32x4{DT<T>::pack2(a.x, a.y), DT<T>::pack2(a.z, a.w), DT<T>::pack2(b.x, b.y), DT<T>::pack2(b.z, b.w)}};
+}
+// eight consecutive elements of a row, in memory or LDS (16-byte aligned)
+template <typename T>
+__device__ __forceinline__ Frag<T> frag_row(const T* p) {
+  if constexpr (sizeof(T) == 4) return Frag<T>{*reinterpret_cast<const f32x4*>(p), *reinterpret_cast<const f32x4*>(p + 4)};
+  else return Frag<T>{*reinterpret_cast<const u32x4*>(p)};
+}
+template <typename T>
+__device__ __forceinline__ Frag<T> frag_zero() {
+  if constexpr (sizeof(T) == 4) return Frag<T>{f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+  else return Frag<T>{u32x4{0u, 0u, 0u, 0u}};
+}
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
+// the transposed operand of a row-major LDS tile: lane (c = l % 16, g = l / 16) gets column col0 + c of rows row0 + 4 g + 0..3 and row0 + 16 + 4 g + 0..3
+// (the order in which frag_of lays down accumulators)
+template <typename T, int PITCH>
+__device__ __forceinline__ Frag<T> frag_cols(const T* tile, int row0, int col0, int lane) {
+  if constexpr (sizeof(T) == 4) {
+    const float* p = reinterpret_cast<const float*>(tile) + (row0 + 4 * (lane >> 4)) * PITCH + col0 + (lane & 15);
+    return Frag<T>{f32x4{p[0], p[PITCH], p[2 * PITCH], p[3 * PITCH]}, f32x4{p[16 * PITCH], p[17 * PITCH], p[18 * PITCH], p[19 * PITCH]}};
+  } else {
+    const T* p = tile + (row0 + 4 * (lane >> 4) + ((lane >> 2) & 3)) * PITCH + col0 + 4 * (lane & 3);
+    const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(const_cast<T*>(p)));
+    const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(const_cast<T*>(p + 16 * PITCH)));
+    const u32x2 x = __builtin_bit_cast(u32x2, a), y = __builtin_bit_cast(u32x2, b);
+    return Frag<T>{u32x4{x.x, x.y, y.x, y.y}};
+  }
+}
+// across the four lanes (l, l ^ 16, l ^ 32, l ^ 48) that share a column
+__device__ __forceinline__ float cols_max(float v) {
+  typedef uint32_t pair __attribute__((ext_vector_type(2)));
+  uint32_t u = __builtin_bit_cast(uint32_t, v);
+  pair r = __builtin_bit_cast(pair, __builtin_amdgcn_permlane16_swap(u, u, false, false));
+  uint32_t x = r.x, y = r.y;
+  v = fmaxf(__builtin_bit_cast(float, x), __builtin_bit_cast(float, y));
+  u = __builtin_bit_cast(uint32_t, v);
+  r = __builtin_bit_cast(pair, __builtin_amdgcn_permlane32_swap(u, u, false, false));
+  x = r.x;
+  y = r.y;
+  return fmaxf(__builtin_bit_cast(float, x), __builtin_bit_cast(float, y));
+}
+__device__ __forceinline__ float cols_sum(float v) {
+  v += __shfl_xor(v, 16);
+  return v + __shfl_xor(v, 32);
+}
+
+// ---- a [ROWS][DP] tile of a strided tensor: 256 threads take 16-byte chunks, columns past D and rows that do not count are zeros
+template <typename T, int DP, int ROWS, int THREADS>
+struct Tile {
+  static constexpr int VEC = DT<T>::KPB, CH = DP / VEC, N = ROWS * CH / THREADS, PITCH = DP + VEC;   // 16 bytes of padding spread the rows over the banks
+  static_assert(N * THREADS == ROWS * CH, "whole chunks");
+  static constexpr int BYTES = ROWS * PITCH * (int)sizeof(T);
+  u32x4 r[N];
+  __device__ __forceinline__ void load(const T* base, int64_t ld, int row0, int rows, int D, const uint8_t* hide, int tid) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int c = tid + n * THREADS, row = row0 + c / CH, col = c % CH * VEC;
+      const bool in = row < rows && col < D && !(hide && hide[row]);
+      r[n] = in ? *reinterpret_cast<const u32x4*>(base + (int64_t)row * ld + col) : u32x4{0u, 0u, 0u, 0u};
+    }
+  }
+  __device__ __forceinline__ void store(T* lds, int tid) const {
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int c = tid + n * THREADS;
+      *reinterpret_cast<u32x4*>(lds + (c / CH) * PITCH + c % CH * VEC) = r[n];
+    }
+  }
+};
+
+// XCD-aware order: the blocks of one XCD take consecutive tiles, so that the tiles of a head share its keys in one L2
+__device__ __forceinline__ int xcd_order(int bid, int nb) {
+  const int qd = nb >> 3, rm = nb & 7, x = bid & 7;
+  return (x < rm ? x * (qd + 1) : rm * (qd + 1) + (x - rm) * qd) + (bid >> 3);
+}
+
+// What a (batch, head) attends over.
+struct Span {
+  int klen, start;                         // keys that count; position of query 0
+  const uint8_t* mask; int64_t m_sq;       // mask + query * m_sq + key: not 0 = hidden
+  const uint8_t* hide;                     // the same row for every query: hidden keys' rows are not read at all
+};
+__device__ __forceinline__ Span span_of(const AttnParams& p, int b, int h) {
+  Span s;
+  s.klen = p.Lk;
+  if (p.k_len) s.klen = min(max(p.k_len[b], 0), p.Lk);
+  s.start = p.q_from_end ? s.klen - p.Lq : p.q_start;
+  s.mask = p.mask ? p.mask + b * p.m_sb + h * p.m_sh : nullptr;
+  s.m_sq = p.m_sq;
+  s.hide = p.mask && p.m_sq == 0 ? s.mask : nullptr;
+  return s;
+}
+
+// The bias of one head by clamped distance, four constant entries beyond each end (so that four neighbours are one read wherever they lie):
+// entry e stands for distance e - 4 - far.
+template <typename T>
+__device__ __forceinline__ void load_bias(const AttnParams& p, int h, float* bias, int threads) {
+  for (int e = threadIdx.x; e < 2 * p.far + 9; e += threads) {
+    const int at = min(max(e - 4, 0), 2 * p.far);
+    bias[e] = DT<T>::load1(static_cast<const T*>(p.table) + (int64_t)min((int)p.lut[at], p.nb - 1) * p.H + h) * LOG2E;
+  }
+}
+// entry of the first of four neighbours at distances d .. d + 3
+__device__ __forceinline__ int bias_at(int d, int far) { return min(max(d, -far - 4), far + 1) + far + 4; }
+
+// does the tile of keys [j0, j0 + nk) against positions [p0, p1] lie wholly beyond one end (its bias is one number)?  -1 / 1: before / after, 0: no
+__device__ __forceinline__ int beyond(int j0, int nk, int p0, int p1, int far) { return j0 + nk - 1 - p0 <= -far ? -1 : j0 - p1 >= far ? 1 : 0; }
+
+// four mask bytes of keys j .. j + 3 (bytes past the last key: hidden)
+__device__ __forceinline__ uint32_t mask4(const uint8_t* m, int j, int lk) {
+  uint32_t w = 0x01010101u;
+  if (j + 4 <= lk) {
+    __builtin_memcpy(&w, m + j, 4);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (j + e < lk) w = (w & ~(0xffu << (8 * e))) | ((uint32_t)m[j + e] << (8 * e));
+  }
+  return w;
+}
+
+template <typename T, int DP>
+struct AttnGeom {
+  static constexpr int KP = DP / 32, DT16 = DP / 16;
+  static constexpr int NQ = sizeof(T) == 2 && DP <= 64 ? 2 : 1;       // 16-query tiles of a wave
+  static constexpr int BK = sizeof(T) * DP <= 128 ? 64 : 32;          // keys of an LDS tile
+};
+
+// ------------------------------------------------------------------------------------------------------------------------------ forward
+template <typename T, int DP, int NQ, int BK>
+__global__ __launch_bounds__(256, 2) void attn_fwd_kernel(const AttnParams p) {
+  constexpr int KP = DP / 32, DT16 = DP / 16, NKT = BK / 16, BQ = 64 * NQ;
+  using TL = Tile<T, DP, BK, 256>;
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  T* kt_ = reinterpret_cast<T*>(smem);
+  T* vt_ = reinterpret_cast<T*>(smem + 2 * TL::BYTES);
+  float* bias = reinterpret_cast<float*>(smem + 4 * TL::BYTES);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
+  const int id = xcd_order(blockIdx.x, gridDim.x);
+  const int bh = id / p.tiles, qt = p.tiles - 1 - (id - bh * p.tiles);          // late query tiles first: under a causal mask they are the long ones
+  const int b = bh / p.H, h = bh - b * p.H, hk = h / (p.H / p.Hk);
+  const Span sp = span_of(p, b, h);
+  const T* kb = static_cast<const T*>(p.k) + b * p.k_sb + hk * p.k_sh;
+  const T* vb = static_cast<const T*>(p.v) + b * p.v_sb + hk * p.v_sh;
+  const int q0 = qt * BQ + wave * 16 * NQ;                                      // the wave's first query
+  const int last = min(qt * BQ + BQ, p.Lq) - 1 + sp.start;                      // position of the block's last query
+  const int kend = p.causal ? min(sp.klen, last + 1) : sp.klen;
+  const int nt = kend > 0 ? (kend + BK - 1) / BK : 0;
+
+  Frag<T> qf[NQ][KP];
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
+    const int i = q0 + n * 16 + c;
+    const T* qp = static_cast<const T*>(p.q) + b * p.q_sb + (int64_t)i * p.q_sl + h * p.q_sh + g * 8;
+#pragma unroll
+    for (int kp = 0; kp < KP; ++kp) qf[n][kp] = i < p.Lq && kp * 32 + g * 8 < p.D ? frag_row(qp + kp * 32) : frag_zero<T>();
+  }
+  f32x4 o[DT16][NQ];
+  float m[NQ], l[NQ];
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
+    m[n] = -INFINITY;
+    l[n] = 0.f;
+#pragma unroll
+    for (int d = 0; d < DT16; ++d) o[d][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  TL kr, vr;
+  if (nt > 0) {
+    kr.load(kb, p.k_sl, 0, sp.klen, p.D, sp.hide, tid);
+    vr.load(vb, p.v_sl, 0, sp.klen, p.D, sp.hide, tid);
+    if (p.table) load_bias<T>(p, h, bias, 256);
+    kr.store(kt_, tid);
+    vr.store(vt_, tid);
+  }
+  __syncthreads();
+  for (int t = 0; t < nt; ++t) {
+    const T* ks = kt_ + (t & 1) * (TL::BYTES / (int)sizeof(T));
+    const T* vs = vt_ + (t & 1) * (TL::BYTES / (int)sizeof(T));
+    const int j0 = t * BK;
+    if (t + 1 < nt) {
+      kr.load(kb, p.k_sl, j0 + BK, sp.klen, p.D, sp.hide, tid);
+      vr.load(vb, p.v_sl, j0 + BK, sp.klen, p.D, sp.hide, tid);
+    }
+    f32x4 s[NKT][NQ];
+#pragma unroll
+    for (int kt = 0; kt < NKT; ++kt) {
+#pragma unroll
+      for (int n = 0; n < NQ; ++n) s[kt][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int kp = 0; kp < KP; ++kp) {
+        const Frag<T> a = frag_row(ks + (kt * 16 + c) * TL::PITCH + kp * 32 + g * 8);
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) s[kt][n] = attn_mma(s[kt][n], a, qf[n][kp]);
+      }
+    }
+    const int p0 = q0 + sp.start, p1 = p0 + 16 * NQ - 1;                        // positions of the wave's queries
+    const int far = p.table ? beyond(j0, BK, p0, p1, p.far) : -1;
+    const bool cut = sp.mask || j0 + BK > sp.klen || (p.causal && j0 + BK - 1 > p0);
+    Frag<T> pf[BK / 32][NQ];
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+      const int i = q0 + n * 16 + c, pos = i + sp.start;
+      if (far) {
+        const float fixed = p.table ? bias[far < 0 ? 0 : 2 * p.far + 8] : 0.f;
+#pragma unroll
+        for (int kt = 0; kt < NKT; ++kt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[kt][n][e] = s[kt][n][e] * p.scale2 + fixed;
+      } else {
+#pragma unroll
+        for (int kt = 0; kt < NKT; ++kt) {
+          const float* w = bias + bias_at(j0 + kt * 16 + 4 * g - pos, p.far);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[kt][n][e] = s[kt][n][e] * p.scale2 + w[e];
+        }
+      }
+      if (cut) {
+        const int end = p.causal ? min(sp.klen, pos + 1) : sp.klen;
+#pragma unroll
+        for (int kt = 0; kt < NKT; ++kt) {
+          const int j = j0 + kt * 16 + 4 * g;
+          const uint32_t w = sp.mask && i < p.Lq ? mask4(sp.mask + (int64_t)i * sp.m_sq, j, p.Lk) : 0u;
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (j + e >= end || ((w >> (8 * e)) & 0xffu)) s[kt][n][e] = -INFINITY;
+        }
+      }
+      float top = m[n];
+#pragma unroll
+      for (int kt = 0; kt < NKT; ++kt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) top = fmaxf(top, s[kt][n][e]);
+      top = cols_max(top);
+      if (__any(top != m[n])) {
+        const float f = top == m[n] ? 1.f : __builtin_amdgcn_exp2f(m[n] - top);   // m = -inf at first: the sums are zeros
+        l[n] *= f;
+#pragma unroll
+        for (int d = 0; d < DT16; ++d) o[d][n] *= f;
+        m[n] = top;
+      }
+      const float ref = top == -INFINITY ? 0.f : top;                           // nothing counted yet: exp2(-inf) below, not NaN
+      float sum = 0.f;
+#pragma unroll
+      for (int kt = 0; kt < NKT; ++kt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          s[kt][n][e] = __builtin_amdgcn_exp2f(s[kt][n][e] - ref);
+          sum += s[kt][n][e];
+        }
+      l[n] += sum;
+#pragma unroll
+      for (int kc = 0; kc < BK / 32; ++kc) pf[kc][n] = frag_of<T>(s[2 * kc][n], s[2 * kc + 1][n]);
+    }
+#pragma unroll
+    for (int d = 0; d < DT16; ++d)
+#pragma unroll
+      for (int kc = 0; kc < BK / 32; ++kc) {
+        const Frag<T> a = frag_cols<T, TL::PITCH>(vs, kc * 32, d * 16, lane);
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) o[d][n] = attn_mma(o[d][n], a, pf[kc][n]);
+      }
+    if (t + 1 < nt) {
+      kr.store(kt_ + ((t + 1) & 1) * (TL::BYTES / (int)sizeof(T)), tid);
+      vr.store(vt_ + ((t + 1) & 1) * (TL::BYTES / (int)sizeof(T)), tid);
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
+    const int i = q0 + n * 16 + c;
+    const float sum = cols_sum(l[n]);
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    if (i >= p.Lq) continue;
+    if (p.lse && g == 0) p.lse[((int64_t)b * p.H + h) * p.Lq + i] = sum == 0.f ? -INFINITY : m[n] + __builtin_amdgcn_logf(sum);
+    T* op = static_cast<T*>(p.o) + (((int64_t)b * p.Lq + i) * p.H + h) * p.D + g * 4;
+#pragma unroll
+    for (int d = 0; d < DT16; ++d)
+      if (d * 16 + g * 4 < p.D) DT<T>::store4(op + d * 16, o[d][n] * inv);
+  }
+}
+
+// -------------------------------------------------------------------------------------------------------- few queries over many keys
+// Rows are (query, head of the group that shares a key head): 16 to a block, so that the keys are read once for all of them.  A block takes one split of the
+// keys, its four waves every fourth 32-key tile of it, each with a running maximum of its own: K comes from memory in operand order, V by way of
+// the wave's own LDS tile; the waves are joined in LDS, the splits by attn_join_kernel.
+template <typename T, int DP>
+__global__ __launch_bounds__(256, 2) void attn_split_kernel(const AttnParams p) {
+  constexpr int KP = DP / 32, DT16 = DP / 16;
+  using TL = Tile<T, DP, 32, 64>;
+  constexpr int VBYTES = 4 * TL::BYTES, OBYTES = 4 * 16 * (DP + 1) * 4;
+  constexpr int BYTES = VBYTES > OBYTES ? VBYTES : OBYTES;
+  __shared__ __attribute__((aligned(16))) unsigned char smem[BYTES];
+  __shared__ float ml[4][16][2];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
+  T* vs = reinterpret_cast<T*>(smem + wave * TL::BYTES);
+  int id = blockIdx.x;
+  const int split = id % p.splits;
+  id /= p.splits;
+  const int rt = id % p.tiles, bh = id / p.tiles, b = bh / p.Hk, hk = bh - b * p.Hk;
+  const int share = p.H / p.Hk, rows = p.Lq * share, row = rt * 16 + c, i = row / share, h = hk * share + row - i * share;
+  const bool live = row < rows;
+  const Span sp = span_of(p, b, live ? h : hk * share);
+  const int pos = i + sp.start;
+  const T* kb = static_cast<const T*>(p.k) + b * p.k_sb + hk * p.k_sh;
+  const T* vb = static_cast<const T*>(p.v) + b * p.v_sb + hk * p.v_sh;
+  const int first = rt * 16 / share + sp.start, last = min((rt * 16 + 15) / share, p.Lq - 1) + sp.start;    // positions of the block's rows
+  const int k0 = split * p.split_keys, kall = p.causal ? min(sp.klen, last + 1) : sp.klen, k1 = min(kall, k0 + p.split_keys);
+  const int end = p.causal ? min(sp.klen, pos + 1) : sp.klen;
+  const uint8_t* hide = sp.hide && p.m_sh == 0 ? sp.hide : nullptr;            // (a mask that differs by head hides rows of no key for all of them)
+  float edge[2] = {0.f, 0.f};                                                  // the bias beyond either end
+  if (p.table && live) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+      edge[s] = DT<T>::load1(static_cast<const T*>(p.table) + (int64_t)min((int)p.lut[s * 2 * p.far], p.nb - 1) * p.H + h) * LOG2E;
+  }
+  Frag<T> qf[KP];
+  const T* qp = static_cast<const T*>(p.q) + b * p.q_sb + (int64_t)i * p.q_sl + h * p.q_sh + g * 8;
+#pragma unroll
+  for (int kp = 0; kp < KP; ++kp) qf[kp] = live && kp * 32 + g * 8 < p.D ? frag_row(qp + kp * 32) : frag_zero<T>();
+  f32x4 o[DT16];
+#pragma unroll
+  for (int d = 0; d < DT16; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY, l = 0.f;
+  Frag<T> kf[2][KP];
+  TL vr;
+  auto load = [&](int j0) {
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) {
+      const int j = j0 + kt * 16 + c;
+      const bool in = j < sp.klen && !(hide && hide[j]);
+      const T* kp_ = kb + (int64_t)j * p.k_sl + g * 8;
+#pragma unroll
+      for (int kp = 0; kp < KP; ++kp) kf[kt][kp] = in && kp * 32 + g * 8 < p.D ? frag_row(kp_ + kp * 32) : frag_zero<T>();
+    }
+    vr.load(vb, p.v_sl, j0, sp.klen, p.D, hide, lane);
+  };
+  int j0 = k0 + wave * 32;
+  if (j0 < k1) load(j0);
+  for (; j0 < k1; j0 += 128) {
+    f32x4 s[2];
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) {
+      s[kt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int kp = 0; kp < KP; ++kp) s[kt] = attn_mma(s[kt], kf[kt][kp], qf[kp]);
+    }
+    vr.store(vs, lane);
+    if (j0 + 128 < k1) load(j0 + 128);
+    const int far = p.table ? beyond(j0, 32, first, last, p.far) : -1;
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) {
+      const int j = j0 + kt * 16 + 4 * g;
+      const uint32_t w = sp.mask && live ? mask4(sp.mask + (int64_t)i * sp.m_sq, j, p.Lk) : 0u;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float add = far < 0 ? edge[0] : edge[1];
+        if (!far && live) {
+          const int at = min(max(j + e - pos, -p.far), p.far) + p.far;
+          add = DT<T>::load1(static_cast<const T*>(p.table) + (int64_t)min((int)p.lut[at], p.nb - 1) * p.H + h) * LOG2E;
+        }
+        const float x = s[kt][e] * p.scale2 + add;
+        s[kt][e] = j + e >= end || ((w >> (8 * e)) & 0xffu) ? -INFINITY : x;
+      }
+    }
+    float top = m;
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) top = fmaxf(top, s[kt][e]);
+    top = cols_max(top);
+    if (__any(top != m)) {
+      const float f = top == m ? 1.f : __builtin_amdgcn_exp2f(m - top);
+      l *= f;
+#pragma unroll
+      for (int d = 0; d < DT16; ++d) o[d] *= f;
+      m = top;
+    }
+    const float ref = top == -INFINITY ? 0.f : top;
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        s[kt][e] = __builtin_amdgcn_exp2f(s[kt][e] - ref);
+        l += s[kt][e];
+      }
+    const Frag<T> pf = frag_of<T>(s[0], s[1]);
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int d = 0; d < DT16; ++d) o[d] = attn_mma(o[d], frag_cols<T, TL::PITCH>(vs, 0, d * 16, lane), pf);
+    __builtin_amdgcn_wave_barrier();
+  }
+  // join the waves (in wave order)
+  l = cols_sum(l);
+  if (g == 0) {
+    ml[wave][c][0] = m;
+    ml[wave][c][1] = l;
+  }
+  __syncthreads();
+  float* os = reinterpret_cast<float*>(smem);
+#pragma unroll
+  for (int d = 0; d < DT16; ++d)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) os[(wave * 16 + c) * (DP + 1) + d * 16 + g * 4 + e] = o[d][e];
+  __syncthreads();
+  for (int x = tid; x < 16 * DP; x += 256) {
+    const int r = x / DP, d = x % DP, rr = rt * 16 + r;
+    if (rr >= rows) continue;
+    float top = -INFINITY, sum = 0.f, val = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) top = fmaxf(top, ml[w][r][0]);
+    bool nan = false;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float f = ml[w][r][0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[w][r][0] - top);
+      nan |= ml[w][r][1] != ml[w][r][1];
+      sum += ml[w][r][1] * f;
+      val += os[(w * 16 + r) * (DP + 1) + d] * f;
+    }
+    if (nan) sum = val = NAN;
+    const int qi = rr / share, hh = hk * share + rr - qi * share;
+    const int64_t at = ((int64_t)b * p.H + hh) * p.Lq + qi;
+    if (p.splits == 1) {
+      if (d < p.D) DT<T>::store1(static_cast<T*>(p.o) + (((int64_t)b * p.Lq + qi) * p.H + hh) * p.D + d, sum == 0.f ? 0.f : val / sum);
+      if (d == 0 && p.lse) p.lse[at] = sum == 0.f ? -INFINITY : top + __builtin_amdgcn_logf(sum);
+    } else {
+      const int64_t n = (int64_t)p.B * p.H * p.Lq, slot = split * n + at;
+      if (d < p.D) p.part[2 * p.splits * n + slot * p.D + d] = val;
+      if (d == 0) {
+        p.part[2 * slot] = top;
+        p.part[2 * slot + 1] = sum;
+      }
+    }
+  }
+}
+
+// a row's splits, joined in split order: 64 threads to a row, up to two columns each
+template <typename T>
+__global__ __launch_bounds__(256) void attn_join_kernel(const AttnParams p) {
+  const int64_t n = (int64_t)p.B * p.H * p.Lq, at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (at >= n) return;
+  const int lane = threadIdx.x & 63;
+  float top = -INFINITY;
+  for (int s = 0; s < p.splits; ++s) top = fmaxf(top, p.part[2 * (s * n + at)]);
+  float sum = 0.f, val[2] = {0.f, 0.f};
+  for (int s = 0; s < p.splits; ++s) {
+    const int64_t slot = s * n + at;
+    const float m = p.part[2 * slot], f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top), l = p.part[2 * slot + 1];
+    if (m == -INFINITY && l == l) continue;
+    sum += l == l ? l * f : l;
+    const float* part = p.part + 2 * p.splits * n + slot * p.D;
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+      if (lane + 64 * k < p.D) val[k] += part[lane + 64 * k] * f;
+  }
+  const int i = at % p.Lq, h = at / p.Lq % p.H, b = at / p.Lq / p.H;
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+    if (lane + 64 * k < p.D)
+      DT<T>::store1(static_cast<T*>(p.o) + (((int64_t)b * p.Lq + i) * p.H + h) * p.D + lane + 64 * k, sum == 0.f ? 0.f : sum == sum ? val[k] / sum : NAN);
+  if (lane == 0 && p.lse) p.lse[at] = sum == 0.f ? -INFINITY : top + __builtin_amdgcn_logf(sum);
+}
+
+// ----------------------------------------------------------------------------------------------------------------------------- backward
+// dQ, delta and the sums of dS by bucket.  As the forward: a lane owns a query's column, K and V tiles stream through LDS; dQ^T += K^T dS^T.
+// The sums by bucket: each lane adds into its own column of a [bucket][lane] table of its wave in LDS (no two lanes share an address, so the order of additions
+// is the program's), tiles wholly beyond `far` add into two registers instead.
+template <typename T, int DP, int NQ, int BK>
+__global__ __launch_bounds__(256, 2) void attn_dq_kernel(const AttnParams p) {
+  constexpr int KP = DP / 32, DT16 = DP / 16, BQ = 64 * NQ;
+  using TL = Tile<T, DP, BK, 256>;
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  T* kt_ = reinterpret_cast<T*>(smem);
+  T* vt_ = reinterpret_cast<T*>(smem + 2 * TL::BYTES);
+  float* bias = reinterpret_cast<float*>(smem + 4 * TL::BYTES);
+  const int entries = p.table ? 2 * p.far + 9 : 0;
+  uint32_t* place = reinterpret_cast<uint32_t*>(bias + entries);               // bucket * 64 by distance
+  float* hist = reinterpret_cast<float*>(place + (p.part ? entries : 0));      // [wave][bucket][lane]
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
+  const int id = xcd_order(blockIdx.x, gridDim.x);
+  const int bh = id / p.tiles, qt = p.tiles - 1 - (id - bh * p.tiles);
+  const int b = bh / p.H, h = bh - b * p.H, hk = h / (p.H / p.Hk);
+  const Span sp = span_of(p, b, h);
+  const T* kb = static_cast<const T*>(p.k) + b * p.k_sb + hk * p.k_sh;
+  const T* vb = static_cast<const T*>(p.v) + b * p.v_sb + hk * p.v_sh;
+  const int q0 = qt * BQ + wave * 16 * NQ;
+  const int last = min(qt * BQ + BQ, p.Lq) - 1 + sp.start;
+  const int kend = p.causal ? min(sp.klen, last + 1) : sp.klen;
+  const int nt = kend > 0 ? (kend + BK - 1) / BK : 0;
+  TL kr, vr;
+  if (nt > 0) {
+    kr.load(kb, p.k_sl, 0, sp.klen, p.D, sp.hide, tid);
+    vr.load(vb, p.v_sl, 0, sp.klen, p.D, sp.hide, tid);
+  }
+  Frag<T> qf[NQ][KP], gf[NQ][KP];
+  float lse[NQ], delta[NQ];
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
+    const int i = q0 + n * 16 + c;
+    const bool in = i < p.Lq;
+    const T* qp = static_cast<const T*>(p.q) + b * p.q_sb + (int64_t)i * p.q_sl + h * p.q_sh + g * 8;
+    const T* gp = static_cast<const T*>(p.dout) + b * p.g_sb + (int64_t)i * p.g_sl + h * p.g_sh + g * 8;
+    const T* op = static_cast<const T*>(p.o) + (((int64_t)b * p.Lq + i) * p.H + h) * p.D + g * 8;
+    // delta = the diagonal of O dO^T by the same products as dP = V dO^T: where one key holds all the weight, O is its value and dS exactly zero
+    f32x4 od = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int kp = 0; kp < KP; ++kp) {
+      const bool on = in && kp * 32 + g * 8 < p.D;
+      qf[n][kp] = on ? frag_row(qp + kp * 32) : frag_zero<T>();
+      gf[n][kp] = on ? frag_row(gp + kp * 32) : frag_zero<T>();
+      od = attn_mma(od, on ? frag_row(op + kp * 32) : frag_zero<T>(), gf[n][kp]);
+    }
+    const float mine = (c & 2) ? ((c & 1) ? od.w : od.z) : ((c & 1) ? od.y : od.x);
+    delta[n] = __shfl(mine, (c >> 2) * 16 + c);
+    const int64_t at = ((int64_t)b * p.H + h) * p.Lq + i;
+    lse[n] = in ? p.lse[at] : INFINITY;
+    if (lse[n] == -INFINITY) lse[n] = INFINITY;                                // an empty row: every probability 0
+    if (in && g == 0) p.delta[at] = delta[n];
+  }
+  f32x4 dq[DT16][NQ];
+#pragma unroll
+  for (int n = 0; n < NQ; ++n)
+#pragma unroll
+    for (int d = 0; d < DT16; ++d) dq[d][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float* mine = hist + wave * p.nb * 64 + lane;
+  float before = 0.f, after = 0.f;
+  if (p.table) load_bias<T>(p, h, bias, 256);
+  if (p.part) {
+    for (int e = tid; e < entries; e += 256) place[e] = (uint32_t)min((int)p.lut[min(max(e - 4, 0), 2 * p.far)], p.nb - 1) * 64;
+    for (int k = 0; k < p.nb; ++k) mine[k * 64] = 0.f;
+  }
+  if (nt > 0) {
+    kr.store(kt_, tid);
+    vr.store(vt_, tid);
+  }
+  __syncthreads();
+  for (int t = 0; t < nt; ++t) {
+    const T* ks = kt_ + (t & 1) * (TL::BYTES / (int)sizeof(T));
+    const T* vs = vt_ + (t & 1) * (TL::BYTES / (int)sizeof(T));
+    const int j0 = t * BK;
+    if (t + 1 < nt) {
+      kr.load(kb, p.k_sl, j0 + BK, sp.klen, p.D, sp.hide, tid);
+      vr.load(vb, p.v_sl, j0 + BK, sp.klen, p.D, sp.hide, tid);
+    }
+    const int p0 = q0 + sp.start, p1 = p0 + 16 * NQ - 1;
+    const int far = p.table ? beyond(j0, BK, p0, p1, p.far) : -1;
+    const bool cut = sp.mask || j0 + BK > sp.klen || (p.causal && j0 + BK - 1 > p0);
+    const float fixed = p.table && far ? bias[far < 0 ? 0 : 2 * p.far + 8] : 0.f;
+#pragma unroll
+    for (int kc = 0; kc < BK / 32; ++kc) {                                     // 32 keys at a time: two score tiles make one operand
+      f32x4 s[2][NQ], w[2][NQ];
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt) {
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) s[kt][n] = w[kt][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int kp = 0; kp < KP; ++kp) {
+          const int off = (kc * 32 + kt * 16 + c) * TL::PITCH + kp * 32 + g * 8;
+          const Frag<T> a = frag_row(ks + off), v = frag_row(vs + off);
+#pragma unroll
+          for (int n = 0; n < NQ; ++n) {
+            s[kt][n] = attn_mma(s[kt][n], a, qf[n][kp]);
+            w[kt][n] = attn_mma(w[kt][n], v, gf[n][kp]);
+          }
+        }
+      }
+      Frag<T> df[NQ];
+#pragma unroll
+      for (int n = 0; n < NQ; ++n) {
+        const int i = q0 + n * 16 + c, pos = i + sp.start;
+        const int end = p.causal ? min(sp.klen, pos + 1) : sp.klen;
+        float sum = 0.f;
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) {
+          const int j = j0 + kc * 32 + kt * 16 + 4 * g;
+          const int at = far ? 0 : bias_at(j - pos, p.far);
+          uint32_t hid = 0u;
+          if (cut && sp.mask && i < p.Lq) hid = mask4(sp.mask + (int64_t)i * sp.m_sq, j, p.Lk);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float x = s[kt][n][e] * p.scale2 + (far ? fixed : bias[at + e]);
+            float d = __builtin_amdgcn_exp2f(x - lse[n]) * (w[kt][n][e] - delta[n]);
+            if (cut && (j + e >= end || ((hid >> (8 * e)) & 0xffu))) d = 0.f;
+            s[kt][n][e] = d;
+            sum += d;
+          }
+          if (p.part && !far)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) __hip_atomic_fetch_add(mine + place[at + e], s[kt][n][e], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
+        }
+        if (far < 0) before += sum;
+        if (far > 0) after += sum;
+        df[n] = frag_of<T>(s[0][n], s[1][n]);
+      }
+#pragma unroll
+      for (int d = 0; d < DT16; ++d) {
+        const Frag<T> a = frag_cols<T, TL::PITCH>(ks, kc * 32, d * 16, lane);
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) dq[d][n] = attn_mma(dq[d][n], a, df[n]);
+      }
+    }
+    if (t + 1 < nt) {
+      kr.store(kt_ + ((t + 1) & 1) * (TL::BYTES / (int)sizeof(T)), tid);
+      vr.store(vt_ + ((t + 1) & 1) * (TL::BYTES / (int)sizeof(T)), tid);
+    }
+    __syncthreads();
+  }
+  if (p.dq) {
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+      const int i = q0 + n * 16 + c;
+      if (i >= p.Lq) continue;
+      T* op = static_cast<T*>(p.dq) + (((int64_t)b * p.Lq + i) * p.H + h) * p.D + g * 4;
+#pragma unroll
+      for (int d = 0; d < DT16; ++d)
+        if (d * 16 + g * 4 < p.D) DT<T>::store4(op + d * 16, dq[d][n] * p.scale);
+    }
+  }
+  if (p.part) {
+    mine[place[0]] += before;
+    mine[place[entries - 1]] += after;
+    __syncthreads();
+    float* out = p.part + ((int64_t)h * p.B * p.tiles + (int64_t)b * p.tiles + qt) * p.nb;
+    for (int k = wave; k < p.nb; k += 4) {                                     // a wave adds a bucket's 4 x 64 lanes
+      float v = 0.f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) v += hist[(w * p.nb + k) * 64 + lane];
+      v = wave_sum(v);
+      if (lane == 0) out[k] = v;
+    }
+  }
+}
+
+// dtable[k][h] = the blocks' sums added in block order: a wave to a (bucket, head)
+template <typename T>
+__global__ __launch_bounds__(256) void attn_dtable_kernel(const float* __restrict__ part, int nb, int H, int blocks, T* __restrict__ dtable) {
+  const int x = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (x >= nb * H) return;
+  const int h = x / nb, k = x - h * nb;
+  float v = 0.f;
+  for (int s = lane; s < blocks; s += 64) v += part[((int64_t)h * blocks + s) * nb + k];
+  v = wave_sum(v);
+  if (lane == 0) DT<T>::store1(dtable + (int64_t)k * H + h, v);
+}
+
+// dK and dV.  A lane owns a key's column (K and V of it in registers as operands), Q and dO tiles stream through LDS with their rows' lse and delta:
+// S = Q K^T, dP = dO V^T, then dV^T += dO^T P and dK^T += Q^T dS.  The heads that share the keys follow one another, so their sum needs no atomics.
+template <typename T, int DP, int NK, int BQ>
+__global__ __launch_bounds__(256, 2) void attn_dkv_kernel(const AttnParams p) {
+  constexpr int KP = DP / 32, DT16 = DP / 16, BKB = 64 * NK;
+  using TL = Tile<T, DP, BQ, 256>;
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  T* qt_ = reinterpret_cast<T*>(smem);
+  T* gt_ = reinterpret_cast<T*>(smem + 2 * TL::BYTES);
+  float* stat = reinterpret_cast<float*>(smem + 4 * TL::BYTES);                // [2][lse BQ | delta BQ]
+  float* bias = stat + 4 * BQ;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
+  const int id = xcd_order(blockIdx.x, gridDim.x);
+  const int bh = id / p.tiles, jt = id - bh * p.tiles;
+  const int b = bh / p.Hk, hk = bh - b * p.Hk, share = p.H / p.Hk;
+  const int jb = jt * BKB, jw = jb + wave * 16 * NK;                           // the block's and the wave's first key
+  Span sp = span_of(p, b, hk * share);
+  const T* kb = static_cast<const T*>(p.k) + b * p.k_sb + hk * p.k_sh;
+  const T* vb = static_cast<const T*>(p.v) + b * p.v_sb + hk * p.v_sh;
+  Frag<T> kf[NK][KP], vf[NK][KP];
+#pragma unroll
+  for (int n = 0; n < NK; ++n) {
+    const int j = jw + n * 16 + c;
+    const bool in = j < sp.klen && !(sp.hide && p.m_sh == 0 && sp.hide[j]);
+#pragma unroll
+    for (int kp = 0; kp < KP; ++kp) {
+      const bool on = in && kp * 32 + g * 8 < p.D;
+      kf[n][kp] = on ? frag_row(kb + (int64_t)j * p.k_sl + kp * 32 + g * 8) : frag_zero<T>();
+      vf[n][kp] = on ? frag_row(vb + (int64_t)j * p.v_sl + kp * 32 + g * 8) : frag_zero<T>();
+    }
+  }
+  f32x4 dk[DT16][NK], dv[DT16][NK];
+#pragma unroll
+  for (int n = 0; n < NK; ++n)
+#pragma unroll
+    for (int d = 0; d < DT16; ++d) dk[d][n] = dv[d][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+  // queries that see a key of this block: from the one at its first key's position on
+  const int i0 = p.causal ? max(0, jb - sp.start) / BQ * BQ : 0;
+  const int nt = jb < sp.klen && i0 < p.Lq ? (p.Lq - i0 + BQ - 1) / BQ : 0, all = nt * share;
+  TL qr, gr;
+  float st = 0.f;
+  auto load = [&](int t) {                                                     // tile t: head t / nt of the group, queries i0 + (t % nt) BQ ..
+    const int h = hk * share + t / nt, i = i0 + (t % nt) * BQ;
+    qr.load(static_cast<const T*>(p.q) + b * p.q_sb + h * p.q_sh, p.q_sl, i, p.Lq, p.D, nullptr, tid);
+    gr.load(static_cast<const T*>(p.dout) + b * p.g_sb + h * p.g_sh, p.g_sl, i, p.Lq, p.D, nullptr, tid);
+    if (tid < 2 * BQ) {
+      const int ii = i + tid % BQ;
+      const float* src = tid < BQ ? p.lse : p.delta;
+      st = ii < p.Lq ? src[((int64_t)b * p.H + h) * p.Lq + ii] : 0.f;
+      if (tid < BQ && (ii >= p.Lq || st == -INFINITY)) st = INFINITY;          // no such row, or an empty one: every probability 0
+    }
+  };
+  auto keep = [&](int t) {
+    qr.store(qt_ + (t & 1) * (TL::BYTES / (int)sizeof(T)), tid);
+    gr.store(gt_ + (t & 1) * (TL::BYTES / (int)sizeof(T)), tid);
+    if (tid < 2 * BQ) stat[(t & 1) * 2 * BQ + tid] = st;
+  };
+  if (all > 0) {
+    load(0);
+    if (p.table) load_bias<T>(p, hk * share, bias, 256);
+    keep(0);
+  }
+  __syncthreads();
+  for (int t = 0; t < all; ++t) {
+    const int h = hk * share + t / nt, iq = i0 + (t % nt) * BQ;
+    if (t && t % nt == 0) {                                                    // the next head of the group: its bias, its mask
+      if (p.table) {
+        load_bias<T>(p, h, bias, 256);
+        __syncthreads();
+      }
+      if (sp.mask) sp.mask += p.m_sh;
+    }
+    const T* qs = qt_ + (t & 1) * (TL::BYTES / (int)sizeof(T));
+    const T* gs = gt_ + (t & 1) * (TL::BYTES / (int)sizeof(T));
+    const float* ls = stat + (t & 1) * 2 * BQ;
+    if (t + 1 < all) load(t + 1);
+    const int p0 = iq + sp.start, p1 = p0 + BQ - 1;
+    const int far = p.table ? beyond(jw, 16 * NK, p0, p1, p.far) : -1;
+    const bool cut = sp.mask || jw + 16 * NK > sp.klen || (p.causal && jw + 16 * NK - 1 > p0);
+    const float fixed = p.table && far ? bias[far < 0 ? 0 : 2 * p.far + 8] : 0.f;
+#pragma unroll
+    for (int qc = 0; qc < BQ / 32; ++qc) {
+      f32x4 s[2][NK], w[2][NK];
+#pragma unroll
+      for (int qq = 0; qq < 2; ++qq) {
+#pragma unroll
+        for (int n = 0; n < NK; ++n) s[qq][n] = w[qq][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int kp = 0; kp < KP; ++kp) {
+          const int off = (qc * 32 + qq * 16 + c) * TL::PITCH + kp * 32 + g * 8;
+          const Frag<T> a = frag_row(qs + off), x = frag_row(gs + off);
+#pragma unroll
+          for (int n = 0; n < NK; ++n) {
+            s[qq][n] = attn_mma(s[qq][n], a, kf[n][kp]);
+            w[qq][n] = attn_mma(w[qq][n], x, vf[n][kp]);
+          }
+        }
+      }
+      Frag<T> pf[NK], df[NK];
+#pragma unroll
+      for (int qq = 0; qq < 2; ++qq) {
+        const int i = qc * 32 + qq * 16 + 4 * g;                               // the lane's first of four queries in the tile
+        const f32x4 ll = *reinterpret_cast<const f32x4*>(ls + i), dd = *reinterpret_cast<const f32x4*>(ls + BQ + i);
+#pragma unroll
+        for (int n = 0; n < NK; ++n) {
+          const int j = jw + n * 16 + c, pos = p0 + i;
+          const int at = far ? 0 : bias_at(j - pos - 3, p.far);                // four neighbours, the last query's first
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float x = s[qq][n][e] * p.scale2 + (far ? fixed : bias[at + 3 - e]);
+            float pr = __builtin_amdgcn_exp2f(x - ll[e]);
+            if (cut) {
+              bool off = j >= sp.klen || (p.causal && j > pos + e);
+              if (sp.mask && j < p.Lk && iq + i + e < p.Lq) off |= sp.mask[(int64_t)(iq + i + e) * sp.m_sq + j] != 0;
+              if (off) pr = 0.f;
+            }
+            const float d = w[qq][n][e] - dd[e];
+            s[qq][n][e] = pr;
+            w[qq][n][e] = cut && pr == 0.f ? 0.f : pr * d;
+          }
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < NK; ++n) {
+        pf[n] = frag_of<T>(s[0][n], s[1][n]);
+        df[n] = frag_of<T>(w[0][n], w[1][n]);
+      }
+#pragma unroll
+      for (int d = 0; d < DT16; ++d) {
+        const Frag<T> a = frag_cols<T, TL::PITCH>(gs, qc * 32, d * 16, lane), x = frag_cols<T, TL::PITCH>(qs, qc * 32, d * 16, lane);
+#pragma unroll
+        for (int n = 0; n < NK; ++n) {
+          dv[d][n] = attn_mma(dv[d][n], a, pf[n]);
+          dk[d][n] = attn_mma(dk[d][n], x, df[n]);
+        }
+      }
+    }
+    if (t + 1 < all) keep(t + 1);
+    __syncthreads();
+  }
+#pragma unroll
+  for (int n = 0; n < NK; ++n) {
+    const int j = jw + n * 16 + c;
+    if (j >= p.Lk) continue;
+    const int64_t at = (((int64_t)b * p.Lk + j) * p.Hk + hk) * p.D + g * 4;
+#pragma unroll
+    for (int d = 0; d < DT16; ++d)
+      if (d * 16 + g * 4 < p.D) {
+        if (p.dk) DT<T>::store4(static_cast<T*>(p.dk) + at + d * 16, dk[d][n] * p.scale);
+        if (p.dv) DT<T>::store4(static_cast<T*>(p.dv) + at + d * 16, dv[d][n]);
+      }
+  }
+}
+
+// -------------------------------------------------------------------------------------------------------------------------------- host
+static bool attn_stride_ok(int64_t s, int es) { return s >= 0 && s * es % 16 == 0; }
+
+static int attn_check(const moy_attention_args* a, bool bwd) {
+  if (!a || a->dtype < MOY_F32 || a->dtype > MOY_F16) return MOY_EINVAL;
+  const int es = a->dtype == MOY_F32 ? 4 : 2;
+  if (!a->q || !a->k || !a->v || !a->o || a->B <= 0 || a->H <= 0 || a->Hk <= 0 || a->Lq <= 0 || a->Lk <= 0 || a->D <= 0) return MOY_EINVAL;
+  if (a->H % a->Hk || a->D % 8) return MOY_EINVAL;
+  if (a->D > 128) return MOY_ENOSYS;
+  if (a->Lq > (1 << 30) || a->Lk > (1 << 30) || a->q_start > (1 << 30) || a->q_start < -(1 << 30)) return MOY_EINVAL;
+  if (!aligned16(a->q) || !aligned16(a->k) || !aligned16(a->v) || !aligned16(a->o)) return MOY_EINVAL;
+  const int64_t st[] = {a->q_sb, a->q_sl, a->q_sh, a->k_sb, a->k_sl, a->k_sh, a->v_sb, a->v_sl, a->v_sh};
+  for (int64_t s : st)
+    if (!attn_stride_ok(s, es)) return MOY_EINVAL;
+  if ((a->table == nullptr) != (a->lut == nullptr)) return MOY_EINVAL;
+  if (a->table && (a->num_buckets < 1 || a->num_buckets > 64 || a->max_distance < 1 || a->max_distance > 1024)) return MOY_EINVAL;
+  if (reinterpret_cast<uintptr_t>(a->table) % es || reinterpret_cast<uintptr_t>(a->k_len) % 4) return MOY_EINVAL;
+  if (a->mask && (a->m_sb < 0 || a->m_sh < 0 || a->m_sq < 0)) return MOY_EINVAL;
+  if (!(a->scale - a->scale == 0.f)) return MOY_EINVAL;
+  if ((int64_t)a->B * a->H > (1 << 24) || (int64_t)a->B * a->H * ((a->Lq > a->Lk ? a->Lq : a->Lk) / 64 + 1) > 0x7fffffffLL / 8) return MOY_EINVAL;
+  if (bwd) {
+    const int64_t gs[] = {a->g_sb, a->g_sl, a->g_sh};
+    for (int64_t s : gs)
+      if (!attn_stride_ok(s, es)) return MOY_EINVAL;
+    if (!a->lse || !a->dout || !aligned16(a->dout) || !aligned16(a->dq) || !aligned16(a->dk) || !aligned16(a->dv)) return MOY_EINVAL;
+    if (!a->dq && !a->dk && !a->dv && !a->dtable) return MOY_EINVAL;
+    if (a->dtable && (!a->table || reinterpret_cast<uintptr_t>(a->dtable) % es)) return MOY_EINVAL;
+  }
+  return MOY_OK;
+}
+
+static AttnParams attn_params(const moy_attention_args* a) {
+  AttnParams p{};
+  p.q = a->q; p.k = a->k; p.v = a->v;
+  p.q_sb = a->q_sb; p.q_sl = a->q_sl; p.q_sh = a->q_sh; p.k_sb = a->k_sb; p.k_sl = a->k_sl; p.k_sh = a->k_sh;
+  p.v_sb = a->v_sb; p.v_sl = a->v_sl; p.v_sh = a->v_sh;
+  p.B = a->B; p.H = a->H; p.Hk = a->Hk; p.Lq = a->Lq; p.Lk = a->Lk; p.D = a->D;
+  p.table = a->table; p.lut = a->lut; p.nb = a->num_buckets; p.far = a->max_distance;
+  p.k_len = a->k_len; p.q_from_end = a->q_from_end; p.q_start = a->q_start; p.causal = a->causal;
+  p.mask = a->mask; p.m_sb = a->m_sb; p.m_sh = a->m_sh; p.m_sq = a->m_sq;
+  p.scale = a->scale; p.scale2 = a->scale * LOG2E;
+  p.o = a->o; p.lse = a->lse;
+  p.dout = a->dout; p.g_sb = a->g_sb; p.g_sl = a->g_sl; p.g_sh = a->g_sh;
+  p.dq = a->dq; p.dk = a->dk; p.dv = a->dv;
+  return p;
+}
+
+// Few rows, or too few blocks of 64 queries to fill the chip: the keys are split.
+static bool attn_uses_split(const moy_attention_args* a) {
+  const int share = a->H / a->Hk;
+  if ((int64_t)a->Lq * share <= 16) return true;
+  return (int64_t)a->B * a->H * ((a->Lq + 63) / 64) < 128 && a->Lk >= 1024;
+}
+
+// Splits of at least 256 keys (two 32-key tiles to a wave), as many as give four blocks to a compute unit, 64 at most.
+static void attn_splits(const moy_attention_args* a, int* tiles, int* splits, int* keys) {
+  const int rows = a->Lq * (a->H / a->Hk);
+  *tiles = (rows + 15) / 16;
+  const int64_t blocks = (int64_t)a->B * a->Hk * *tiles;
+  int64_t s = (1024 + blocks - 1) / blocks;
+  const int64_t most = (a->Lk + 255) / 256;
+  if (s > most) s = most;
+  if (s > 64) s = 64;
+  *keys = (int)(((a->Lk + s - 1) / s + 127) / 128 * 128);
+  *splits = (a->Lk + *keys - 1) / *keys;
+}
+
+static int attn_lds_opt_in(const void* kern) {
+  return hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024) == hipSuccess ? MOY_OK : MOY_ELAUNCH;
+}
+
+static size_t attn_bias_bytes(const moy_attention_args* a) { return a->table ? (2 * (size_t)a->max_distance + 9) * 4 : 0; }
+
+template <typename T, int DP>
+static int attn_fwd(const moy_attention_args* a, AttnParams p, hipStream_t st) {
+  using G = AttnGeom<T, DP>;
+  if (attn_uses_split(a)) {
+    attn_splits(a, &p.tiles, &p.splits, &p.split_keys);
+    p.part = a->ws;
+    hipLaunchKernelGGL((attn_split_kernel<T, DP>), dim3((unsigned)((int64_t)a->B * a->Hk * p.tiles * p.splits)), dim3(256), 0, st, p);
+    const int rc = launch_status();
+    if (rc != MOY_OK || p.splits == 1) return rc;
+    hipLaunchKernelGGL((attn_join_kernel<T>), dim3((unsigned)(((int64_t)a->B * a->H * a->Lq + 3) / 4)), dim3(256), 0, st, p);
+    return launch_status();
+  }
+  constexpr int NQ = G::NQ, BK = G::BK;
+  auto kern = attn_fwd_kernel<T, DP, NQ, BK>;
+  static const int ready = attn_lds_opt_in(reinterpret_cast<const void*>(kern));
+  if (ready != MOY_OK) return ready;
+  p.tiles = (a->Lq + 64 * NQ - 1) / (64 * NQ);
+  const size_t lds = 4 * Tile<T, DP, BK, 256>::BYTES + attn_bias_bytes(a);
+  hipLaunchKernelGGL(kern, dim3((unsigned)(a->B * a->H * p.tiles)), dim3(256), lds, st, p);
+  return launch_status();
+}
+
+template <typename T, int DP>
+struct AttnBwdGeom {
+  static constexpr int NQ = AttnGeom<T, DP>::NQ, BK = AttnGeom<T, DP>::BK;
+  static constexpr int NK = sizeof(T) == 2 && DP <= 64 ? 2 : 1, BQ = sizeof(T) * DP <= 128 ? 64 : 32;
+};
+
+static int attn_dq_tiles(const moy_attention_args* a) {
+  const int rows = a->dtype != MOY_F32 && a->D <= 64 ? 128 : 64;
+  return (a->Lq + rows - 1) / rows;
+}
+
+template <typename T, int DP>
+static int attn_bwd(const moy_attention_args* a, AttnParams p, hipStream_t st) {
+  using G = AttnBwdGeom<T, DP>;
+  const size_t bias = attn_bias_bytes(a);
+  {
+    auto kern = attn_dq_kernel<T, DP, G::NQ, G::BK>;
+    static const int ready = attn_lds_opt_in(reinterpret_cast<const void*>(kern));
+    if (ready != MOY_OK) return ready;
+    p.tiles = attn_dq_tiles(a);
+    const size_t lds = 4 * Tile<T, DP, G::BK, 256>::BYTES + bias + (p.part ? bias + 4 * 64 * 4 * (size_t)a->num_buckets : 0);
+    hipLaunchKernelGGL(kern, dim3((unsigned)(a->B * a->H * p.tiles)), dim3(256), lds, st, p);
+    const int rc = launch_status();
+    if (rc != MOY_OK) return rc;
+  }
+  if (a->dtable) {
+    hipLaunchKernelGGL((attn_dtable_kernel<T>), dim3((a->num_buckets * a->H + 3) / 4), dim3(256), 0, st, p.part, a->num_buckets, a->H, a->B * p.tiles,
+                       static_cast<T*>(a->dtable));
+    const int rc = launch_status();
+    if (rc != MOY_OK) return rc;
+  }
+  if (!a->dk && !a->dv) return MOY_OK;
+  auto kern = attn_dkv_kernel<T, DP, G::NK, G::BQ>;
+  static const int ready = attn_lds_opt_in(reinterpret_cast<const void*>(kern));
+  if (ready != MOY_OK) return ready;
+  p.tiles = (a->Lk + 64 * G::NK - 1) / (64 * G::NK);
+  const size_t lds = 4 * Tile<T, DP, G::BQ, 256>::BYTES + 16 * G::BQ + bias;
+  hipLaunchKernelGGL(kern, dim3((unsigned)(a->B * a->Hk * p.tiles)), dim3(256), lds, st, p);
+  return launch_status();
+}
+
+#define MOY_ATTN_DISPATCH(FN, ...)                                                                                            \
+  switch (a->dtype) {                                                                                                         \
+    case MOY_F32: return a->D <= 32 ? FN<float, 32>(__VA_ARGS__) : a->D <= 64 ? FN<float, 64>(__VA_ARGS__) : FN<float, 128>(__VA_ARGS__);       \
+    case MOY_BF16: return a->D <= 32 ? FN<bf16_t, 32>(__VA_ARGS__) : a->D <= 64 ? FN<bf16_t, 64>(__VA_ARGS__) : FN<bf16_t, 128>(__VA_ARGS__);   \
+    default: return a->D <= 32 ? FN<f16_t, 32>(__VA_ARGS__) : a->D <= 64 ? FN<f16_t, 64>(__VA_ARGS__) : FN<f16_t, 128>(__VA_ARGS__);            \
+  }
+
+}  // namespace moy
+
+using namespace moy;
+
+extern "C" int64_t moy_attention_ws(const moy_attention_args* a) {
+  const int rc = attn_check(a, false);
+  if (rc != MOY_OK) return rc;
+  if (!attn_uses_split(a)) return 0;
+  int tiles, splits, keys;
+  attn_splits(a, &tiles, &splits, &keys);
+  return splits == 1 ? 0 : (int64_t)splits * a->B * a->H * a->Lq * (2 + a->D);
+}
+
+extern "C" int moy_attention(const moy_attention_args* a, void* stream) {
+  const int64_t need = moy_attention_ws(a);
+  if (need < 0) return (int)need;
+  if (need > 0 && (!a->ws || a->ws_len < need)) return MOY_EINVAL;
+  const AttnParams p = attn_params(a);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  MOY_ATTN_DISPATCH(attn_fwd, a, p, st)
+}
+
+extern "C" int64_t moy_attention_bwd_ws(const moy_attention_args* a) {
+  const int rc = attn_check(a, true);
+  if (rc != MOY_OK) return rc;
+  return (int64_t)a->B * a->H * a->Lq + (a->dtable ? (int64_t)a->H * a->B * attn_dq_tiles(a) * a->num_buckets : 0);
+}
+
+extern "C" int moy_attention_bwd(const moy_attention_args* a, void* stream) {
+  const int64_t need = moy_attention_bwd_ws(a);
+  if (need < 0) return (int)need;
+  if (!a->ws || a->ws_len < need) return MOY_EINVAL;
+  AttnParams p = attn_params(a);
+  p.delta = a->ws;
+  p.part = a->dtable ? a->ws + (int64_t)a->B * a->H * a->Lq : nullptr;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  MOY_ATTN_DISPATCH(attn_bwd, a, p, st)
+}

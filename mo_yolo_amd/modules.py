@@ -336,6 +336,32 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, residual=None):
     return ops.layer_norm_forward(x, weight, bias, eps, residual)
 
 
+class BiasedAttentionFunction(torch.autograd.Function):
+    """Autograd of ops.attention_forward: gradients for q, k, v and the bias table."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, table, lut, causal, q_start, k_len, attn_mask, scale):
+        o, lse = ops.attention_forward(q, k, v, table, lut, causal=causal, q_start=q_start, k_len=k_len, attn_mask=attn_mask, scale=scale, need_lse=True)
+        ctx.save_for_backward(q, k, v, o, lse, table, lut, k_len, attn_mask)
+        ctx.how = dict(causal=causal, q_start=q_start, scale=scale)
+        return o
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        q, k, v, o, lse, table, lut, k_len, attn_mask = ctx.saved_tensors
+        grads = ops.attention_backward(dout, q, k, v, o, lse, table, lut, k_len=k_len, attn_mask=attn_mask, need=ctx.needs_input_grad[:4], **ctx.how)
+        return (*grads, None, None, None, None, None, None)
+
+
+def biased_attention(q, k, v, table=None, lut=None, *, causal=False, q_start=None, k_len=None, attn_mask=None, scale=None):
+    """Attention with a learned relative position bias by buckets, differentiable in q, k, v and table; arguments as ops.attention_forward.  Without a
+    gradient to compute, the forward alone (a single new token over a long cache among it: the keys are split over the chip)."""
+    if _wants_grad(q, k, v, table):
+        return BiasedAttentionFunction.apply(q, k, v, table, lut, causal, q_start, k_len, attn_mask, scale)
+    return ops.attention_forward(q, k, v, table, lut, causal=causal, q_start=q_start, k_len=k_len, attn_mask=attn_mask, scale=scale)
+
+
 class MSDeformAttn(nn.Module):
     """transformer.py:193-287 (d_model 256, 8 heads, 4 points, <= 4 levels, 4-d reference boxes)."""
 

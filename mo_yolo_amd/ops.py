@@ -625,3 +625,140 @@ def layer_norm_backward(dy, x, weight, mean, rstd, residual=None, need=(True, Tr
                                            wcode, mean.data_ptr(), rstd.data_ptr(), rows, c, _ptr(dx), c, _ptr(dw), _ptr(db), _ptr(ws), n, code,
                                            _st()), "moy_layer_norm_bwd")
     return dx, dw, db
+
+
+def relative_buckets(num_buckets, max_distance, bidirectional=True, device="cuda"):
+    """The bucket of every clamped distance key - query in [-max_distance, max_distance] as uint8 [2 * max_distance + 1], for attention_forward's
+    `lut`: a bucket for each of the nearest distances (half of the buckets), then ranges that grow by a constant factor up to max_distance.
+    bidirectional: the upper half of the buckets is for keys after the query; otherwise those share bucket 0 with the query itself.  Borders are
+    decided in whole numbers (n^m near^t >= max_distance^t near^m), so they are the same on every machine."""
+    half = num_buckets // 2 if bidirectional else num_buckets
+    near = half // 2
+    if not 2 <= num_buckets <= 64 or near < 1 or (bidirectional and num_buckets % 2) or not near < max_distance <= 1024:
+        raise ValueError("relative_buckets: 2..64 buckets (an even number of at least 4 if bidirectional), max_distance above the exact ones and at most 1024")
+    steps, side, t = half - near, [], 0
+    for n in range(max_distance + 1):
+        if n >= near:
+            while t < steps - 1 and n ** steps * near ** (t + 1) >= max_distance ** (t + 1) * near ** steps:
+                t += 1
+        side.append(n if n < near else near + t)
+    after = [half + b for b in side[1:]] if bidirectional else [0] * max_distance
+    return torch.tensor(side[:0:-1] + [0] + after, dtype=torch.uint8).to(device)
+
+
+def _strided(t):
+    """A view that the attention kernels address: unit stride within a head, 16-byte steps and base (a copy where the strides allow none)."""
+    es = t.element_size()
+    if t.stride(3) != 1 or t.data_ptr() % 16 or any(t.shape[i] > 1 and t.stride(i) * es % 16 for i in range(3)):
+        t = t.contiguous()
+        if t.data_ptr() % 16:
+            t = t.clone()
+    return t, [0 if t.shape[i] == 1 else t.stride(i) for i in range(3)]
+
+
+def _attention_args(q, k, v, table, lut, causal, q_start, k_len, attn_mask, scale):
+    """Checks the arguments and lays them out: (moy_attention_args, tensors to keep until the launch)."""
+    _one_device(q, k, v, table, lut, k_len, attn_mask)
+    code = _code(q)
+    if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape or q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:
+        raise ValueError("attention: q [B, Lq, H, D], k and v [B, Lk, Hk, D]")
+    B, Lq, H, D = q.shape
+    Lk, Hk = k.shape[1:3]
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise TypeError("attention: q, k and v must have one type")
+    if Hk == 0 or H == 0 or H % Hk or D == 0 or D % 8 or D > 128:
+        raise ValueError("attention: H must be a multiple of Hk and D a multiple of 8 up to 128")
+    a = L.AttentionArgs()
+    (q, (a.q_sb, a.q_sl, a.q_sh)), (k, (a.k_sb, a.k_sl, a.k_sh)), (v, (a.v_sb, a.v_sl, a.v_sh)) = _strided(q), _strided(k), _strided(v)
+    a.q, a.k, a.v, a.B, a.H, a.Hk, a.Lq, a.Lk, a.D, a.dtype = q.data_ptr(), k.data_ptr(), v.data_ptr(), B, H, Hk, Lq, Lk, D, code
+    a.scale = D ** -0.5 if scale is None else scale
+    a.causal, a.q_from_end, a.q_start = int(bool(causal)), int(q_start is None), 0 if q_start is None else int(q_start)
+    if abs(a.q_start) > 1 << 30 or (q_start is not None and a.q_start != q_start):
+        raise ValueError("attention: q_start out of range")
+    keep = [q, k, v]
+    if (table is None) != (lut is None):
+        raise ValueError("attention: table and lut come together")
+    if table is not None:
+        if table.dim() != 2 or table.shape[1] != H or not 1 <= table.shape[0] <= 64 or table.dtype != q.dtype:
+            raise ValueError("attention: table must be [num_buckets <= 64, H] in q's type")
+        if lut.dim() != 1 or lut.dtype != torch.uint8 or lut.shape[0] % 2 == 0 or not 3 <= lut.shape[0] <= 2049:
+            raise ValueError("attention: lut must be uint8 [2 * max_distance + 1], max_distance in 1..1024")
+        table, lut = table.contiguous(), lut.contiguous()
+        a.table, a.lut, a.num_buckets, a.max_distance = table.data_ptr(), lut.data_ptr(), table.shape[0], lut.shape[0] // 2
+        keep += [table, lut]
+    if k_len is not None:
+        if k_len.dtype != torch.int32 or tuple(k_len.shape) != (B,):
+            raise ValueError("attention: k_len must be int32 [B]")
+        k_len = k_len.contiguous()
+        a.k_len = k_len.data_ptr()
+        keep.append(k_len)
+    if attn_mask is not None:
+        m = attn_mask
+        if m.dtype not in (torch.bool, torch.uint8) or m.dim() not in (2, 4) or m.shape[-1] != Lk:
+            raise ValueError("attention: attn_mask must be bool (True: hidden) [Lq or 1, Lk] or [B or 1, H or 1, Lq or 1, Lk]")
+        m = m[None, None] if m.dim() == 2 else m
+        if any(n not in (1, w) for n, w in zip(m.shape, (B, H, Lq))):
+            raise ValueError("attention: attn_mask does not broadcast to [B, H, Lq, Lk]")
+        m = (m if m.stride(3) == 1 or Lk == 1 else m.contiguous()).view(torch.uint8)
+        a.mask, a.m_sb, a.m_sh, a.m_sq = m.data_ptr(), *(0 if n == 1 else m.stride(i) for i, n in enumerate(m.shape[:3]))
+        keep.append(m)
+    return a, keep
+
+
+def attention_forward(q, k, v, table=None, lut=None, *, causal=False, q_start=None, k_len=None, attn_mask=None, scale=None, need_lse=False):
+    """softmax(scale q k^T + bias) v with a learned relative position bias by buckets (moy_attention): q [B, Lq, H, D], k / v [B, Lk, Hk, D] (any
+    strides; H a multiple of Hk: shared key heads), D a multiple of 8 up to 128; float32 / bfloat16 / float16.
+    table [num_buckets, H] in q's type with lut = relative_buckets(...), or any uint8 map of clamped distances to buckets; none: no bias.
+    q_start: position of the first query (keys count from 0); None: the queries are the last of the k_len[b] (or Lk) keys, as with a cache.
+    causal: a query sees keys up to its own position.  k_len int32 [B]: keys that count (rows behind them are not read).  attn_mask bool, True = hidden,
+    [Lq, Lk] or [B, H, Lq, Lk] with axes of 1 where it does not differ; hidden rows of k / v must still be finite, unless the mask differs
+    neither by query nor by head.  scale: D ** -0.5.  A query that sees no key gets zeros.
+    -> o [B, Lq, H, D], or with need_lse (o, lse) as attention_backward takes them."""
+    a, keep = _attention_args(q, k, v, table, lut, causal, q_start, k_len, attn_mask, scale)
+    with _on(q):
+        o = torch.empty(a.B, a.Lq, a.H, a.D, device=q.device, dtype=q.dtype)
+        lse = torch.empty(a.B, a.H, a.Lq, device=q.device, dtype=torch.float32) if need_lse else None
+        if o.numel() and a.Lk == 0:
+            o.zero_()
+            if need_lse:
+                lse.fill_(float("-inf"))
+        elif o.numel():
+            a.o, a.lse = o.data_ptr(), _ptr(lse)
+            n = L.lib().moy_attention_ws(C.byref(a))
+            if n < 0:
+                L.check(n, "moy_attention_ws")
+            if n:
+                ws = torch.empty(n, device=q.device, dtype=torch.float32)
+                a.ws, a.ws_len = ws.data_ptr(), n
+            L.check(L.lib().moy_attention(C.byref(a), _st()), "moy_attention")
+    return (o, lse) if need_lse else o
+
+
+def attention_backward(dout, q, k, v, o, lse, table=None, lut=None, *, causal=False, q_start=None, k_len=None, attn_mask=None, scale=None,
+                       need=(True, True, True, True)):
+    """Gradients of attention_forward (moy_attention_bwd): (dq, dk, dv, dtable), None where `need` says so.  float16: P and dS are rounded to
+    float16 for the matrix cores, so dout wants the usual loss scaling."""
+    a, keep = _attention_args(q, k, v, table, lut, causal, q_start, k_len, attn_mask, scale)
+    _one_device(q, dout, o, lse)
+    if dout.shape != q.shape or dout.dtype != q.dtype or o.shape != q.shape or o.dtype != q.dtype or not o.is_contiguous():
+        raise ValueError("attention_backward: dout and o must have q's shape and type, o contiguous")
+    if lse.dtype != torch.float32 or tuple(lse.shape) != (a.B, a.H, a.Lq) or not lse.is_contiguous():
+        raise ValueError("attention_backward: lse must be the forward's")
+    need = (*need[:3], need[3] and table is not None)
+    with _on(q):
+        new = lambda t, n: torch.empty(t.shape, device=t.device, dtype=t.dtype) if n else None  # noqa: E731
+        out = [new(t, n) for t, n in zip((q, k, v, table), need)]
+        if not any(need):
+            return tuple(out)
+        if q.numel() == 0 or k.numel() == 0:
+            return tuple(t if t is None else t.zero_() for t in out)
+        g, (a.g_sb, a.g_sl, a.g_sh) = _strided(dout)
+        a.dout, a.o, a.lse = g.data_ptr(), o.data_ptr(), lse.data_ptr()
+        a.dq, a.dk, a.dv, a.dtable = (_ptr(t) for t in out)
+        n = L.lib().moy_attention_bwd_ws(C.byref(a))
+        if n < 0:
+            L.check(n, "moy_attention_bwd_ws")
+        ws = torch.empty(n, device=q.device, dtype=torch.float32)
+        a.ws, a.ws_len = ws.data_ptr(), n
+        L.check(L.lib().moy_attention_bwd(C.byref(a), _st()), "moy_attention_bwd")
+    return tuple(out)

@@ -190,3 +190,270 @@ def test_layer_norm_other_stream_and_graph():
         g.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(u, v) for u, v in zip(out, want)), k
+
+
+# ------------------------------------------------------------------------------------------------------------------- attention
+def attention_reference(q, k, v, table=None, lut=None, causal=False, q_start=None, k_len=None, attn_mask=None, scale=None, dout=None):
+    """({y, dq, dk, dv, dtable} in 64 bits, their tolerances)."""
+    dt = q.dtype
+    B, Lq, H, D = q.shape
+    Lk, Hk = k.shape[1:3]
+    share, sc = H // Hk, D ** -0.5 if scale is None else scale
+    hs16 = half_step(dt) if dt != torch.float32 else 0.0                       # P and dS as matrix operands
+    under = tiny(dt) if dt == torch.float16 else 0.0
+    z = lambda *s: torch.zeros(*s, dtype=torch.float64, device=q.device)  # noqa: E731
+    out = dict(y=z(B, Lq, H, D), dq=z(B, Lq, H, D), dk=z(B, Lk, Hk, D), dv=z(B, Lk, Hk, D))
+    tol = {n: torch.zeros_like(t) for n, t in out.items()}
+    mag = {n: torch.zeros_like(t) for n, t in out.items()}
+    if table is not None:
+        out["dtable"], tol["dtable"], mag["dtable"] = (z(*table.shape) for _ in range(3))
+    for b in range(B):
+        n = Lk if k_len is None else min(max(int(k_len[b]), 0), Lk)
+        start = (n - Lq) if q_start is None else q_start
+        if n == 0:
+            continue
+        i, j = torch.arange(Lq, device=q.device)[:, None] + start, torch.arange(n, device=q.device)[None]
+        for h in range(H):
+            hk = h // share
+            qd, kd, vd = q[b, :, h].double(), k[b, :n, hk].double(), v[b, :n, hk].double()
+            hidden = (j > i) if causal else torch.zeros(Lq, n, dtype=torch.bool, device=q.device)
+            if attn_mask is not None:
+                m = attn_mask if attn_mask.dim() == 2 else attn_mask.expand(B, H, Lq, Lk)[b, h]
+                hidden = hidden | (m != 0)[:, :n]
+                if m.shape[0] == 1 or (m.dim() == 2 and m.stride(0) == 0):
+                    kd, vd = kd.masked_fill((m[:1, :n] != 0).t(), 0), vd.masked_fill((m[:1, :n] != 0).t(), 0)
+            s, sm = qd @ kd.t() * sc, qd.abs() @ kd.abs().t() * abs(sc)
+            if table is not None:
+                far = lut.shape[0] // 2
+                at = lut.long()[(j - i).clamp(-far, far) + far].clamp(max=table.shape[0] - 1)
+                s, sm = s + table.double()[at, h], sm + table.double()[at, h].abs()
+            s = s.masked_fill(hidden, float("-inf"))
+            none = hidden.all(-1, keepdim=True)
+            p = torch.softmax(s.masked_fill(none, 0.0), -1).masked_fill(hidden | none, 0.0)
+            # relative error of a probability: its score's (D products, scale, bias in 32 bits), the largest one's of the row through maximum and sum, the exponentials
+            rel = U32 * (2 * (D + 8) * sm.masked_fill(hidden, 0).amax(-1, keepdim=True) + 2 * s.masked_fill(hidden, 0).abs().amax(-1, keepdim=True) + n + 16)
+            y, ya, va = p @ vd, p @ vd.abs(), (~hidden).double() @ vd.abs()
+            out["y"][b, :, h] = y
+            ty = half_step(dt) * y.abs() + tiny(dt) + (hs16 + rel + n * U32) * ya + under * va
+            tol["y"][b, :, h] = ty
+            if dout is None:
+                continue
+            do = dout[b, :, h].double()
+            dp, dpa = do @ vd.t(), do.abs() @ vd.abs().t()
+            delta = (do * y).sum(-1, keepdim=True)
+            ds = p * (dp - delta)
+            off = (do.abs() * ty).sum(-1, keepdim=True) + U32 * (D + 8) * (do.abs() * y.abs()).sum(-1, keepdim=True)
+            te = p * (rel * (dp - delta).abs() + U32 * (D + 8) * dpa + off + 2 * U32 * (dp.abs() + delta.abs()))     # of dS in 32 bits
+            th = te + hs16 * ds.abs() + under                                                                          # ... rounded for the products
+            out["dq"][b, :, h] = sc * ds @ kd
+            tol["dq"][b, :, h] = abs(sc) * ((th + n * U32 * ds.abs()) @ kd.abs())
+            out["dk"][b, :n, hk] += sc * ds.t() @ qd
+            tol["dk"][b, :n, hk] += abs(sc) * ((th + Lq * share * U32 * ds.abs()).t() @ qd.abs())
+            out["dv"][b, :n, hk] += p.t() @ do
+            tol["dv"][b, :n, hk] += (p * (rel + hs16 + Lq * share * U32) + under).t() @ do.abs()
+            if table is not None:
+                out["dtable"][:, h].index_add_(0, at.reshape(-1), ds.reshape(-1))
+                tol["dtable"][:, h].index_add_(0, at.reshape(-1), te.reshape(-1) + (Lk + 64 + B * Lq) * U32 * ds.abs().reshape(-1))
+    for n in out:
+        if n != "y":
+            tol[n] = tol[n] * (1 + half_step(dt)) + half_step(dt) * out[n].abs() + tiny(dt)
+    return out, tol
+
+
+def attention_inputs(seed, B, Lq, Lk, H, Hk, D, dtype, buckets=None, far=None, both=True, grad=True):
+    dt, gen = DT[dtype], gen_of(seed)
+    q, k, v, dout = rand(gen, B, Lq, H, D, dtype=dt), rand(gen, B, Lk, Hk, D, dtype=dt), rand(gen, B, Lk, Hk, D, dtype=dt), rand(gen, B, Lq, H, D, dtype=dt)
+    table = lut = None
+    if buckets:
+        table, lut = rand(gen, buckets, H, dtype=dt), ops.relative_buckets(buckets, far, both)
+    for t in (q, k, v, table):
+        if t is not None and grad:
+            t.requires_grad_(True)
+    return q, k, v, table, lut, dout
+
+
+def check_attention(q, k, v, table, lut, dout, **how):
+    """Forward (alone and with gradients) and backward against the reference."""
+    leaves = [t for t in (q, k, v, table) if t is not None]
+    y = modules.biased_attention(q, k, v, table, lut, **how)
+    grads = torch.autograd.grad(y, leaves, dout)
+    with torch.no_grad():
+        assert torch.equal(modules.biased_attention(q, k, v, table, lut, **how).nan_to_num(7.0), y.nan_to_num(7.0))
+    d = lambda t: None if t is None else t.detach()  # noqa: E731
+    out, tol = attention_reference(d(q), d(k), d(v), d(table), lut, dout=dout, **how)
+    for name, got in zip(("y", "dq", "dk", "dv", "dtable"), (y, *grads)):
+        close(got, out[name], tol[name], name)
+
+
+KLEN = {"none": None, "ragged": [0, 3, 1 << 20, -4]}
+ATTENTION = [
+    # B, Lq, Lk, H, Hk, D, buckets, far, both, causal, q_start, k_len, mask
+    (1, 1, 1, 1, 1, 8, 8, 8, True, False, None, None, None),
+    (2, 5, 7, 2, 1, 40, 8, 6, True, False, 0, None, None),
+    (1, 64, 64, 2, 2, 32, 32, 128, True, False, 0, None, None),
+    (2, 77, 130, 4, 2, 64, 16, 40, True, False, 0, [130, 41], None),
+    (1, 300, 300, 2, 2, 32, 32, 128, True, False, 0, None, "square"),
+    (1, 129, 257, 3, 3, 128, 64, 200, False, True, None, None, None),
+    (4, 33, 65, 1, 1, 72, 4, 2, True, True, 0, [0, 3, 1 << 20, -4], None),
+    (3, 2, 300, 8, 2, 64, 32, 20, False, True, None, [300, 1, 0], None),
+    (2, 1, 5000, 4, 1, 128, 32, 128, False, False, None, [5000, 4097], None),
+    (1, 3, 2111, 6, 6, 16, None, None, True, True, None, None, None),
+    (1, 40, 2050, 3, 1, 32, 32, 900, True, False, 100, None, "rows"),
+    (2, 70, 90, 2, 2, 24, 16, 1024, True, True, -20, None, "full"),
+    (2, 130, 200, 4, 4, 64, None, None, True, False, 0, None, "keys"),
+    (2, 9, 90, 4, 2, 96, 16, 30, True, False, 50, [80, 90], "keys"),
+    (1, 500, 190, 2, 1, 64, 32, 64, True, True, -150, None, None),
+]
+
+
+def attention_mask(kind, seed, B, H, Lq, Lk):
+    if kind is None:
+        return None
+    gen = gen_of(seed + 1)
+    shape = {"square": (Lq, Lk), "rows": (1, H, Lq, Lk), "full": (B, H, Lq, Lk), "keys": (B, 1, 1, Lk)}[kind]
+    m = torch.rand(*shape, device="cuda", generator=gen) < 0.4
+    if kind != "keys":
+        m[..., Lq // 2, :] = True                                             # a query that sees nothing
+        m[..., 0, :] = False
+    return m
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("shape", ATTENTION, ids=lambda s: "-".join(map(str, s)))
+def test_attention(shape, dtype):
+    B, Lq, Lk, H, Hk, D, buckets, far, both, causal, q_start, k_len, mask = shape
+    seed = Lq * 1000 + Lk
+    q, k, v, table, lut, dout = attention_inputs(seed, B, Lq, Lk, H, Hk, D, dtype, buckets, far, both)
+    kl = None if k_len is None else torch.tensor(k_len, dtype=torch.int32, device="cuda")
+    check_attention(q, k, v, table, lut, dout, causal=causal, q_start=q_start, k_len=kl, attn_mask=attention_mask(mask, seed, B, H, Lq, Lk))
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+def test_attention_of_one_key_has_no_gradient_in_q_k_table(dtype):
+    """All the weight on one key: dS is exactly zero, so are dq, dk and dtable; y is the value and dv the sum of dout."""
+    q, k, v, table, lut, dout = attention_inputs(1, 3, 37, 9, 4, 2, 64, dtype, 8, 8)
+    how = dict(q_start=0, k_len=torch.ones(3, dtype=torch.int32, device="cuda"))
+    y = modules.biased_attention(q, k, v, table, lut, **how)
+    dq, dk, dv, dt = torch.autograd.grad(y, (q, k, v, table), dout)
+    assert not dq.any() and not dk.any() and not dt.any()
+    assert torch.equal(y, v[:, :1].repeat_interleave(2, 2).expand(-1, 37, -1, -1))
+    out, tol = attention_reference(q.detach(), k.detach(), v.detach(), table.detach(), lut, dout=dout, **how)
+    close(dv, out["dv"], tol["dv"], "dv")
+
+
+def test_attention_ignores_what_stands_behind_the_keys():
+    """NaN and infinities in rows past k_len, and in rows that a key mask hides, change nothing; their gradients are zeros."""
+    for lq, lk, d, dtype in ((70, 200, 64, "bf16"), (2, 2000, 32, "f32"), (1, 2500, 128, "f16")):
+        q, k, v, table, lut, dout = attention_inputs(5, 2, lq, lk, 4, 2, d, dtype, 32, 100)
+        n = [lk - 77, lk - 130]
+        mask = torch.zeros(2, 1, 1, lk, dtype=torch.bool, device="cuda")
+        mask[0, ..., 5:40] = True
+        how = dict(q_start=0, k_len=torch.tensor(n, dtype=torch.int32, device="cuda"), attn_mask=mask)
+        want = modules.biased_attention(q, k, v, table, lut, **how)
+        gw = torch.autograd.grad(want, (q, k, v, table), dout)
+        with torch.no_grad():
+            for t in (k, v):
+                t[0, n[0]:], t[1, n[1]:], t[0, 5:20], t[0, 20:40] = float("nan"), float("inf"), float("nan"), float("-inf")
+        got = modules.biased_attention(q, k, v, table, lut, **how)
+        gg = torch.autograd.grad(got, (q, k, v, table), dout)
+        assert torch.isfinite(want).all() and torch.equal(got, want)
+        for a, b in zip(gg, gw):
+            assert torch.isfinite(a).all() and torch.equal(a, b)
+        assert not gg[1][0, n[0]:].any() and not gg[2][1, n[1]:].any() and not gg[2][0, 5:40].any()
+
+
+def test_attention_lowest_scores_and_nan():
+    """Scores at the type's ends: a table entry of the lowest value leaves its keys out; NaN in a key that counts shows in every query."""
+    q, k, v, table, lut, dout = attention_inputs(6, 1, 50, 50, 2, 2, 32, "bf16", 8, 8, False, grad=False)
+    table[7] = torch.finfo(torch.bfloat16).min                                # the bucket of every distance of 7 and more
+    how = dict(causal=True, q_start=0)
+    far = torch.arange(50, device="cuda")[None] - torch.arange(50, device="cuda")[:, None] <= -8
+    got, want = ops.attention_forward(q, k, v, table, lut, **how), ops.attention_forward(q, k, v, table, lut, attn_mask=far, **how)
+    assert torch.equal(got, want)
+    k[0, 3, 0, 0] = float("nan")
+    y = ops.attention_forward(q, k, v, q_start=0)
+    assert torch.isnan(y[0, :, 0]).all() and torch.isfinite(y[0, :, 1]).all()
+
+
+def test_attention_strides_and_layouts():
+    gen = gen_of(8)
+    B, L, H, D = 2, 150, 4, 64
+    qkv = rand(gen, B, L, 3, H, D, dtype=torch.bfloat16)
+    q, k, v = qkv.unbind(2)                                                   # one packed buffer
+    want = ops.attention_forward(q.contiguous(), k.contiguous(), v.contiguous(), causal=True)
+    assert torch.equal(ops.attention_forward(q, k, v, causal=True), want)
+    heads_first = [t.transpose(1, 2).contiguous().transpose(1, 2) for t in (q, k, v)]
+    assert torch.equal(ops.attention_forward(*heads_first, causal=True), want)
+    odd = torch.empty(B, L, H, D + 3, device="cuda", dtype=torch.bfloat16)    # rows off the 16-byte steps: copied
+    odd[..., 3:] = q
+    assert torch.equal(ops.attention_forward(odd[..., 3:], k, v, causal=True), want)
+    one = k[:, :, :1].expand(B, L, H, D)                                      # one key head, expanded (stride 0)
+    assert torch.equal(ops.attention_forward(q, one, v), ops.attention_forward(q, one.contiguous(), v))
+    m = torch.rand(L, L, device="cuda", generator=gen) < 0.3
+    assert torch.equal(ops.attention_forward(q, k, v, attn_mask=m.t()), ops.attention_forward(q, k, v, attn_mask=m.t().contiguous()))
+    assert torch.equal(ops.attention_forward(q, k, v, attn_mask=m), ops.attention_forward(q, k, v, attn_mask=m[None, None].expand(B, H, L, L).contiguous()))
+    x = q.contiguous().requires_grad_(True)
+    y = modules.biased_attention(x, k, v)
+    a = torch.autograd.grad(y, x, torch.ones(1, 1, 1, 1, device="cuda", dtype=torch.bfloat16).expand_as(y), retain_graph=True)[0]
+    assert torch.equal(a, torch.autograd.grad(y, x, torch.ones_like(y))[0])
+    e = ops.attention_forward(q[:, :0], k, v)
+    assert e.shape == (B, 0, H, D)
+    assert not ops.attention_forward(q, k[:, :0], v[:, :0]).any()
+    x, kk = q.contiguous().requires_grad_(True), k[:, :0].contiguous().requires_grad_(True)
+    gx, gk = torch.autograd.grad(modules.biased_attention(x, kk, v[:, :0]), (x, kk), torch.ones_like(x))
+    assert not gx.any() and gk.shape == kk.shape
+
+
+def test_attention_offsets_past_32_bits():
+    """A cache whose rows stand 40000 elements apart: the last ones lie past 2^31 elements."""
+    n, pitch = 70000, 40000
+    big = torch.empty(n, pitch, device="cuda", dtype=torch.bfloat16)
+    gen = gen_of(9)
+    big[:, :128] = rand(gen, n, 128, dtype=torch.bfloat16)
+    k, v = big[None, :, None, :64], big[None, :, None, 64:128]
+    q = rand(gen, 1, 1, 1, 64, dtype=torch.bfloat16)
+    assert torch.equal(ops.attention_forward(q, k, v), ops.attention_forward(q, k.contiguous(), v.contiguous()))
+    q = rand(gen, 1, 128 * 64, 1, 64, dtype=torch.bfloat16)                   # ... and through the kernel for many queries
+    assert torch.equal(ops.attention_forward(q, k, v), ops.attention_forward(q, k.contiguous(), v.contiguous()))
+
+
+def test_attention_gradient_against_differences():
+    q, k, v, table, lut, dout = attention_inputs(10, 2, 20, 33, 4, 2, 16, "f32", 16, 20)
+    how = dict(q_start=4, attn_mask=attention_mask("square", 3, 2, 4, 20, 33))
+    leaves = (q, k, v, table)
+    grads = torch.autograd.grad(modules.biased_attention(*leaves, lut, **how), leaves, dout)
+    gen, h = gen_of(11), 2.0 ** -6
+    with torch.no_grad():
+        for n, (t, g) in enumerate(zip(leaves, grads)):
+            d = rand(gen, *t.shape)
+            f = [float((modules.biased_attention(*[u + s * h * d if u is t else u for u in leaves], lut, **how).double() * dout.double()).sum()) for s in (1, -1)]
+            want = float((g.double() * d.double()).sum())
+            size = float((g.double().abs() * d.double().abs()).sum())
+            assert abs((f[0] - f[1]) / (2 * h) - want) < 1e-2 * size, n       # h^2 / 6 = 4e-5 of the third derivative along d
+
+
+def test_attention_repeats_on_any_stream_and_in_graphs():
+    q, k, v, table, lut, dout = attention_inputs(12, 2, 200, 333, 4, 2, 64, "bf16", 32, 64)
+    k_len = torch.tensor([333, 100], dtype=torch.int32, device="cuda")
+    step = lambda: (lambda y: (y.detach(), *torch.autograd.grad(y, (q, k, v, table), dout)))(modules.biased_attention(q, k, v, table, lut, q_start=0, k_len=k_len))  # noqa: E731
+    want = step()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = step()
+    side.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    with torch.no_grad():
+        one = lambda: ops.attention_forward(q[:, :1], k, v, table, lut, k_len=k_len)  # noqa: E731
+        g1, o1 = captured(one)
+    g2, o2 = captured(step)
+    gen = gen_of(13)
+    for n in ((333, 100), (5, 0), (1, 333), (200, 201)):                      # the graphs read the lengths anew
+        with torch.no_grad():
+            k_len.copy_(torch.tensor(n, dtype=torch.int32))
+            q.copy_(rand(gen, *q.shape, dtype=torch.bfloat16))
+        want, w1 = step(), one().detach()
+        g2.replay()
+        g1.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(o2, want)) and torch.equal(o1, w1), n

@@ -49,3 +49,72 @@ def test_layer_ops_refuse_cpu_tensors():
         ops.layer_norm_forward(x)
     with pytest.raises(RuntimeError, match="Not implemented on the CPU"):
         modules.layer_norm(x.requires_grad_(True), torch.ones(8), torch.zeros(8))
+
+
+# ------------------------------------------------------------------------------------------------------------------- attention
+def _attn(bwd=False, **kw):
+    a = _lib.AttentionArgs()
+    for n in ("q", "k", "v", "o"):
+        setattr(a, n, FAKE)
+    a.B, a.H, a.Hk, a.Lq, a.Lk, a.D, a.scale, a.dtype = 2, 4, 2, 5, 7, 64, 0.125, _lib.BF16
+    a.q_sb, a.q_sl, a.q_sh, a.k_sb, a.k_sl, a.k_sh, a.v_sb, a.v_sl, a.v_sh = 5 * 256, 256, 64, 7 * 128, 128, 64, 7 * 128, 128, 64
+    if bwd:
+        a.dout = a.lse = a.dq = a.ws = FAKE
+        a.g_sb, a.g_sl, a.g_sh, a.ws_len = 5 * 256, 256, 64, 1 << 20
+    for n, x in kw.items():
+        setattr(a, n, x)
+    f = _lib.lib().moy_attention_bwd if bwd else _lib.lib().moy_attention
+    return f(C.byref(a), None), (_lib.lib().moy_attention_bwd_ws if bwd else _lib.lib().moy_attention_ws)(C.byref(a))
+
+
+BAD_ATTENTION = [dict(q=None), dict(k=None), dict(v=None), dict(o=None), dict(B=0), dict(Lq=0), dict(Lk=-1), dict(H=3), dict(Hk=0), dict(D=12), dict(D=0),
+                 dict(dtype=9), dict(q=FAKE + 8), dict(q_sl=257), dict(k_sb=-128), dict(table=FAKE), dict(lut=FAKE),
+                 dict(table=FAKE, lut=FAKE, num_buckets=65, max_distance=128), dict(table=FAKE, lut=FAKE, num_buckets=32, max_distance=0),
+                 dict(table=FAKE, lut=FAKE, num_buckets=32, max_distance=1025), dict(scale=float("inf")), dict(scale=float("nan")), dict(q_start=(1 << 30) + 1),
+                 dict(mask=FAKE, m_sq=-1), dict(k_len=FAKE + 2), dict(B=1 << 20, H=1 << 10, Hk=1)]
+
+
+@pytest.mark.parametrize("kw", BAD_ATTENTION)
+def test_attention_refuses(kw):
+    assert _attn(**kw) == (_lib.EINVAL, _lib.EINVAL)
+    assert _attn(True, **kw) == (_lib.EINVAL, _lib.EINVAL)
+
+
+def test_attention_refuses_on_the_way_back():
+    for kw in (dict(dout=None), dict(lse=None), dict(dq=None), dict(dtable=FAKE), dict(dk=FAKE + 4), dict(g_sl=3)):
+        assert _attn(True, **kw)[0] == _lib.EINVAL, kw
+    assert _attn(True, ws=None)[0] == _lib.EINVAL and _attn(True, ws_len=39)[0] == _lib.EINVAL
+    assert _attn(D=136) == (_lib.ENOSYS, _lib.ENOSYS)
+    assert _lib.lib().moy_attention(None, None) == _lib.EINVAL and _lib.lib().moy_attention_bwd_ws(None) == _lib.EINVAL
+    # a long cache is split: partial results need a workspace
+    assert _attn(Lq=1, Lk=8192, ws_len=10, ws=FAKE)[0] == _lib.EINVAL
+    assert _attn(Lq=1, Lk=8192)[1] == 32 * 2 * 4 * 1 * (2 + 64)
+
+
+def test_attention_args_layout_matches_header():
+    import os
+    import re
+    txt = open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include", "moyolo.h")).read()
+    body = txt[txt.index("typedef struct moy_attention_args {"):txt.index("} moy_attention_args;")].split("{", 1)[1]
+    assert [re.split(r"[ *]+", d.strip())[-1] for d in body.split(";") if d.strip()] == [f[0] for f in _lib.AttentionArgs._fields_]
+
+
+def test_relative_buckets():
+    b = ops.relative_buckets(32, 128, True, "cpu")
+    at = lambda d: int(b[d + 128])  # noqa: E731
+    assert b.dtype == torch.uint8 and b.shape == (257,)
+    assert [at(-d) for d in (0, 1, 7, 8, 11, 12, 15, 16, 127, 128)] == [0, 1, 7, 8, 8, 9, 9, 10, 15, 15]      # 8 * (128 / 8)^(t / 8): 8, 11.3, 16, 22.6, ...
+    assert [at(d) for d in (1, 8, 128)] == [17, 24, 31]
+    one = ops.relative_buckets(8, 16, False, "cpu").tolist()                  # exact borders: 4 * 4^(t / 4) = 4, 5.66, 8, 11.3
+    assert one == [7] * 5 + [6] * 4 + [5] * 2 + [4] * 2 + [3, 2, 1, 0] + [0] * 16
+    for bad in ((3, 8, True), (65, 128, False), (1, 8, False), (32, 8, True), (32, 1025, True)):
+        with pytest.raises(ValueError):
+            ops.relative_buckets(*bad, device="cpu")
+
+
+def test_attention_refuses_cpu_tensors():
+    q = torch.zeros(1, 2, 1, 8)
+    with pytest.raises(RuntimeError, match="Not implemented on the CPU"):
+        ops.attention_forward(q, q, q)
+    with pytest.raises(RuntimeError, match="Not implemented on the CPU"):
+        modules.biased_attention(q.requires_grad_(True), q, q)
