@@ -625,7 +625,8 @@ int64_t moy_layer_norm_bwd_ws(int64_t rows, int C, int dtype);    /* floats, or 
  *   o_i = sum_j softmax_j(S)[i, j] v_j  over the keys that count; a query without one: zeros (and no gradient).
  * q T [B, Lq, H, D], k / v T [B, Lk, Hk, D] (H % Hk == 0: query head h takes key head h / (H / Hk)), D % 8 == 0 up to 128 (else MOY_ENOSYS), any
  * strides of whole 16-byte steps (sb batch, sl token, sh head, in elements), 16-byte aligned bases.  o T [B, Lq, H, D] dense; lse fp32 [B, H, Lq]
- * (optional; what the backward takes).
+ * and, for 16-bit T, o_rest T like o (what the rounding of o left out): optional, what the backward takes (without o_rest its row sums are
+ * taken over the rounded o).  scale >= 0.
  * table T [num_buckets <= 64, H] with lut uint8 [2 max_distance + 1] (device; entries past num_buckets count as the last), max_distance <= 1024; both NULL: no
  * bias.  Key j counts iff j < k_len[b] (int32 [B], device, clamped to [0, Lk]; NULL: Lk), and j <= i + start if causal, and mask (uint8, strides m_sb,
  * m_sh, m_sq, key stride 1; NULL: none) is 0 there.  start = q_start, or with q_from_end k_len[b] - Lq (the queries are the last tokens of the cache).
@@ -643,7 +644,7 @@ typedef struct moy_attention_args {
   const int32_t* k_len; int32_t q_from_end; int32_t q_start; int32_t causal;
   const uint8_t* mask; int64_t m_sb; int64_t m_sh; int64_t m_sq;
   float scale; int32_t dtype;
-  void* o; float* lse; float* ws; int64_t ws_len;
+  void* o; void* o_rest; float* lse; float* ws; int64_t ws_len;
   const void* dout; int64_t g_sb; int64_t g_sl; int64_t g_sh;
   void* dq; void* dk; void* dv; void* dtable;
 } moy_attention_args;

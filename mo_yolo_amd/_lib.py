@@ -99,7 +99,7 @@ class AttentionArgs(C.Structure):
         ("table", vp), ("lut", vp), ("num_buckets", i32), ("max_distance", i32),
         ("k_len", vp), ("q_from_end", i32), ("q_start", i32), ("causal", i32),
         ("mask", vp), ("m_sb", i64), ("m_sh", i64), ("m_sq", i64), ("scale", f32), ("dtype", i32),
-        ("o", vp), ("lse", vp), ("ws", vp), ("ws_len", i64),
+        ("o", vp), ("o_rest", vp), ("lse", vp), ("ws", vp), ("ws_len", i64),
         ("dout", vp), ("g_sb", i64), ("g_sl", i64), ("g_sh", i64), ("dq", vp), ("dk", vp), ("dv", vp), ("dtable", vp),
     ]
 

@@ -29,6 +29,7 @@ struct AttnParams {
   const uint8_t* mask; int64_t m_sb, m_sh, m_sq;
   float scale, scale2;                     // scale2 = scale log2 e
   void* o; float* lse;                     // lse fp32 [B, H, Lq], log2 units; -inf: an empty row
+  void* rest;                              // 16-bit types: what the rounding of o left out (o + rest: 16 bits or more of mantissa), for delta
   const void* dout; int64_t g_sb, g_sl, g_sh;
   void *dq, *dk, *dv;
   float* delta;                            // backward: fp32 [B, H, Lq]
@@ -62,11 +63,18 @@ __device__ __forceinline__ f32x4 attn_mma(f32x4 acc, const Frag<float>& a, const
   acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a.hi.w, b.hi.w, acc, 0, 0, 0);
   return acc;
 }
+// (DT<f16_t>::pack2 pins its operands in registers, which costs this file's loops a wave of occupancy)
+template <typename T>
+__device__ __forceinline__ uint32_t pack_as(float lo, float hi) {
+  typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+  if constexpr (DT<T>::code == MOY_F16) return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2_{lo, hi}, h2));
+  else return pack_bf2(lo, hi);
+}
 // two accumulators (rows 4 q .. 4 q + 3 of two 16-row tiles) -> the operand whose lane holds those eight
 template <typename T>
 __device__ __forceinline__ Frag<T> frag_of(const f32x4& a, const f32x4& b) {
   if constexpr (sizeof(T) == 4) return Frag<T>{a, b};
-  else return Frag<T>{u32x4{DT<T>::pack2(a.x, a.y), DT<T>::pack2(a.z, a.w), DT<T>::pack2(b.x, b.y), DT<T>::pack2(b.z, b.w)}};
+  else return Frag<T>{u32x4{pack_as<T>(a.x, a.y), pack_as<T>(a.z, a.w), pack_as<T>(b.x, b.y), pack_as<T>(b.z, b.w)}};
 }
 // eight consecutive elements of a row, in memory or LDS (16-byte aligned)
 template <typename T>
@@ -114,14 +122,41 @@ __device__ __forceinline__ float cols_sum(float v) {
   return v + __shfl_xor(v, 32);
 }
 
+// o = v rounded, and what the rounding left out
+template <typename T>
+__device__ __forceinline__ void store_o(T* o, T* rest, int64_t at, f32x4 v) {
+  DT<T>::store4(o + at, v);
+  if constexpr (sizeof(T) == 2) {
+    if (rest) {
+      const uint32_t a = DT<T>::pack2(v.x, v.y), b = DT<T>::pack2(v.z, v.w);
+      DT<T>::store4(rest + at, f32x4{v.x - DT<T>::lo(a), v.y - DT<T>::hi(a), v.z - DT<T>::lo(b), v.w - DT<T>::hi(b)});
+    }
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store_o1(T* o, T* rest, int64_t at, float v) {
+  DT<T>::store1(o + at, v);
+  if constexpr (sizeof(T) == 2) {
+    if (rest) DT<T>::store1(rest + at, v - DT<T>::lo(DT<T>::pack2(v, v)));
+  }
+}
+
 // ---- a [ROWS][DP] tile of a strided tensor: 256 threads take 16-byte chunks, columns past D and rows that do not count are zeros
 template <typename T, int DP, int ROWS, int THREADS>
 struct Tile {
-  static constexpr int VEC = DT<T>::KPB, CH = DP / VEC, N = ROWS * CH / THREADS, PITCH = DP + VEC;   // 16 bytes of padding spread the rows over the banks
+  static constexpr int VEC = DT<T>::KPB, CH = DP / VEC, N = ROWS * CH / THREADS, PITCH = DP + 32 / (int)sizeof(T);   // 32 bytes of padding: row and transposed reads without bank conflicts (16 bytes: 38 % of the LDS cycles were conflicts)
   static_assert(N * THREADS == ROWS * CH, "whole chunks");
   static constexpr int BYTES = ROWS * PITCH * (int)sizeof(T);
   u32x4 r[N];
   __device__ __forceinline__ void load(const T* base, int64_t ld, int row0, int rows, int D, const uint8_t* hide, int tid) {
+    if (row0 + ROWS <= rows && D == DP && !hide) {
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        const int c = tid + n * THREADS;
+        r[n] = *reinterpret_cast<const u32x4*>(base + (int64_t)(row0 + c / CH) * ld + c % CH * VEC);
+      }
+      return;
+    }
 #pragma unroll
     for (int n = 0; n < N; ++n) {
       const int c = tid + n * THREADS, row = row0 + c / CH, col = c % CH * VEC;
@@ -142,6 +177,19 @@ struct Tile {
 __device__ __forceinline__ int xcd_order(int bid, int nb) {
   const int qd = nb >> 3, rm = nb & 7, x = bid & 7;
   return (x < rm ? x * (qd + 1) : rm * (qd + 1) + (x - rm) * qd) + (bid >> 3);
+}
+
+// Which (batch, head) and tile a block takes.  Without a causal mask a head's tiles follow one another.  With one the tiles differ in length: the long
+// ones (tile p.tiles - 1 first) of the heads of an XCD come first, the short ones fill in behind them.
+__device__ __forceinline__ void tile_order(const AttnParams& p, int id, int heads, int* head, int* tile) {
+  if (p.causal && heads % 8 == 0) {
+    const int per = heads / 8, x = id / (per * p.tiles), y = id - x * per * p.tiles;
+    *tile = p.tiles - 1 - y / per;
+    *head = x * per + y % per;
+  } else {
+    *head = id / p.tiles;
+    *tile = p.tiles - 1 - (id - *head * p.tiles);
+  }
 }
 
 // What a (batch, head) attends over.
@@ -172,6 +220,8 @@ __device__ __forceinline__ void load_bias(const AttnParams& p, int h, float* bia
 }
 // entry of the first of four neighbours at distances d .. d + 3
 __device__ __forceinline__ int bias_at(int d, int far) { return min(max(d, -far - 4), far + 1) + far + 4; }
+
+__device__ __forceinline__ f32x4 bias4(const float* p) { return f32x4{p[0], p[1], p[2], p[3]}; }
 
 // does the tile of keys [j0, j0 + nk) against positions [p0, p1] lie wholly beyond one end (its bias is one number)?  -1 / 1: before / after, 0: no
 __device__ __forceinline__ int beyond(int j0, int nk, int p0, int p1, int far) { return j0 + nk - 1 - p0 <= -far ? -1 : j0 - p1 >= far ? 1 : 0; }
@@ -207,7 +257,8 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(const AttnParams p) {
   float* bias = reinterpret_cast<float*>(smem + 4 * TL::BYTES);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
   const int id = xcd_order(blockIdx.x, gridDim.x);
-  const int bh = id / p.tiles, qt = p.tiles - 1 - (id - bh * p.tiles);          // late query tiles first: under a causal mask they are the long ones
+  int bh, qt;
+  tile_order(p, id, p.B * p.H, &bh, &qt);
   const int b = bh / p.H, h = bh - b * p.H, hk = h / (p.H / p.Hk);
   const Span sp = span_of(p, b, h);
   const T* kb = static_cast<const T*>(p.k) + b * p.k_sb + hk * p.k_sh;
@@ -270,51 +321,54 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(const AttnParams p) {
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
       const int i = q0 + n * 16 + c, pos = i + sp.start;
-      if (far) {
-        const float fixed = p.table ? bias[far < 0 ? 0 : 2 * p.far + 8] : 0.f;
+      const float fixed = p.table && far ? bias[far < 0 ? 0 : 2 * p.far + 8] : 0.f;
+      const bool plain = far && !cut;                                           // one bias for the tile, every key counts: scale and bias wait for the exponential
+      float top = -INFINITY;
+      if (!plain) {
+        if (far) {
 #pragma unroll
-        for (int kt = 0; kt < NKT; ++kt)
+          for (int kt = 0; kt < NKT; ++kt) s[kt][n] = s[kt][n] * p.scale2 + fixed;
+        } else {
+          f32x4 w[NKT];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[kt][n][e] = s[kt][n][e] * p.scale2 + fixed;
-      } else {
+          for (int kt = 0; kt < NKT; ++kt) w[kt] = bias4(bias + bias_at(j0 + kt * 16 + 4 * g - pos, p.far));
 #pragma unroll
-        for (int kt = 0; kt < NKT; ++kt) {
-          const float* w = bias + bias_at(j0 + kt * 16 + 4 * g - pos, p.far);
+          for (int kt = 0; kt < NKT; ++kt) s[kt][n] = s[kt][n] * p.scale2 + w[kt];
+        }
+        if (cut) {
+          const int end = p.causal ? min(sp.klen, pos + 1) : sp.klen;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[kt][n][e] = s[kt][n][e] * p.scale2 + w[e];
+          for (int kt = 0; kt < NKT; ++kt) {
+            const int j = j0 + kt * 16 + 4 * g;
+            const uint32_t w = sp.mask && i < p.Lq ? mask4(sp.mask + (int64_t)i * sp.m_sq, j, p.Lk) : 0u;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (j + e >= end || ((w >> (8 * e)) & 0xffu)) s[kt][n][e] = -INFINITY;
+          }
         }
       }
-      if (cut) {
-        const int end = p.causal ? min(sp.klen, pos + 1) : sp.klen;
-#pragma unroll
-        for (int kt = 0; kt < NKT; ++kt) {
-          const int j = j0 + kt * 16 + 4 * g;
-          const uint32_t w = sp.mask && i < p.Lq ? mask4(sp.mask + (int64_t)i * sp.m_sq, j, p.Lk) : 0u;
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (j + e >= end || ((w >> (8 * e)) & 0xffu)) s[kt][n][e] = -INFINITY;
-        }
-      }
-      float top = m[n];
 #pragma unroll
       for (int kt = 0; kt < NKT; ++kt)
 #pragma unroll
         for (int e = 0; e < 4; ++e) top = fmaxf(top, s[kt][n][e]);
-      top = cols_max(top);
-      if (__any(top != m[n])) {
-        const float f = top == m[n] ? 1.f : __builtin_amdgcn_exp2f(m[n] - top);   // m = -inf at first: the sums are zeros
+      const float mul = plain ? p.scale2 : 1.f;                                 // (scale >= 0: the largest product is the largest score)
+      top = cols_max(plain ? top * mul + fixed : top);
+      // The reference of the exponentials follows the maximum only where that has grown by more than 2^8: weights stay below 256, which costs nothing of
+      // their precision, and the sums are seldom scaled.  (m = -inf at first: then the reference is the maximum, and a lone key weighs exactly 1.)
+      if (__any(top > m[n] + 8.f)) {
+        const float next = top > m[n] + 8.f ? top : m[n], f = next == m[n] ? 1.f : __builtin_amdgcn_exp2f(m[n] - next);
         l[n] *= f;
 #pragma unroll
         for (int d = 0; d < DT16; ++d) o[d][n] *= f;
-        m[n] = top;
+        m[n] = next;
       }
-      const float ref = top == -INFINITY ? 0.f : top;                           // nothing counted yet: exp2(-inf) below, not NaN
+      const float ref = (plain ? fixed : 0.f) - (m[n] == -INFINITY ? 0.f : m[n]);   // nothing counted yet: exp2(-inf) below, not NaN
       float sum = 0.f;
 #pragma unroll
       for (int kt = 0; kt < NKT; ++kt)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          s[kt][n][e] = __builtin_amdgcn_exp2f(s[kt][n][e] - ref);
+          s[kt][n][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][n][e], mul, ref));
           sum += s[kt][n][e];
         }
       l[n] += sum;
@@ -342,10 +396,10 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(const AttnParams p) {
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     if (i >= p.Lq) continue;
     if (p.lse && g == 0) p.lse[((int64_t)b * p.H + h) * p.Lq + i] = sum == 0.f ? -INFINITY : m[n] + __builtin_amdgcn_logf(sum);
-    T* op = static_cast<T*>(p.o) + (((int64_t)b * p.Lq + i) * p.H + h) * p.D + g * 4;
+    const int64_t at = (((int64_t)b * p.Lq + i) * p.H + h) * p.D + g * 4;
 #pragma unroll
     for (int d = 0; d < DT16; ++d)
-      if (d * 16 + g * 4 < p.D) DT<T>::store4(op + d * 16, o[d][n] * inv);
+      if (d * 16 + g * 4 < p.D) store_o(static_cast<T*>(p.o), static_cast<T*>(p.rest), at + d * 16, o[d][n] * inv);
   }
 }
 
@@ -490,7 +544,8 @@ __global__ __launch_bounds__(256, 2) void attn_split_kernel(const AttnParams p) 
     const int qi = rr / share, hh = hk * share + rr - qi * share;
     const int64_t at = ((int64_t)b * p.H + hh) * p.Lq + qi;
     if (p.splits == 1) {
-      if (d < p.D) DT<T>::store1(static_cast<T*>(p.o) + (((int64_t)b * p.Lq + qi) * p.H + hh) * p.D + d, sum == 0.f ? 0.f : val / sum);
+      if (d < p.D)
+        store_o1(static_cast<T*>(p.o), static_cast<T*>(p.rest), (((int64_t)b * p.Lq + qi) * p.H + hh) * p.D + d, sum == 0.f ? 0.f : val / sum);
       if (d == 0 && p.lse) p.lse[at] = sum == 0.f ? -INFINITY : top + __builtin_amdgcn_logf(sum);
     } else {
       const int64_t n = (int64_t)p.B * p.H * p.Lq, slot = split * n + at;
@@ -526,11 +581,15 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnParams p) {
 #pragma unroll
   for (int k = 0; k < 2; ++k)
     if (lane + 64 * k < p.D)
-      DT<T>::store1(static_cast<T*>(p.o) + (((int64_t)b * p.Lq + i) * p.H + h) * p.D + lane + 64 * k, sum == 0.f ? 0.f : sum == sum ? val[k] / sum : NAN);
+      store_o1(static_cast<T*>(p.o), static_cast<T*>(p.rest), (((int64_t)b * p.Lq + i) * p.H + h) * p.D + lane + 64 * k,
+               sum == 0.f ? 0.f : sum == sum ? val[k] / sum : NAN);
   if (lane == 0 && p.lse) p.lse[at] = sum == 0.f ? -INFINITY : top + __builtin_amdgcn_logf(sum);
 }
 
 // ----------------------------------------------------------------------------------------------------------------------------- backward
+// an LDS address that only this lane touches: the order of its additions is the program's
+__device__ __forceinline__ void lane_add(float* p, float v) { __hip_atomic_fetch_add(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT); }
+
 // dQ, delta and the sums of dS by bucket.  As the forward: a lane owns a query's column, K and V tiles stream through LDS; dQ^T += K^T dS^T.
 // The sums by bucket: each lane adds into its own column of a [bucket][lane] table of its wave in LDS (no two lanes share an address, so the order of additions
 // is the program's), tiles wholly beyond `far` add into two registers instead.
@@ -543,11 +602,12 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(const AttnParams p) {
   T* vt_ = reinterpret_cast<T*>(smem + 2 * TL::BYTES);
   float* bias = reinterpret_cast<float*>(smem + 4 * TL::BYTES);
   const int entries = p.table ? 2 * p.far + 9 : 0;
-  uint32_t* place = reinterpret_cast<uint32_t*>(bias + entries);               // bucket * 64 by distance
+  uint32_t* place = reinterpret_cast<uint32_t*>(bias + entries);               // bucket * 64 by distance; RUN: the next three distances share it
   float* hist = reinterpret_cast<float*>(place + (p.part ? entries : 0));      // [wave][bucket][lane]
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
   const int id = xcd_order(blockIdx.x, gridDim.x);
-  const int bh = id / p.tiles, qt = p.tiles - 1 - (id - bh * p.tiles);
+  int bh, qt;
+  tile_order(p, id, p.B * p.H, &bh, &qt);
   const int b = bh / p.H, h = bh - b * p.H, hk = h / (p.H / p.Hk);
   const Span sp = span_of(p, b, h);
   const T* kb = static_cast<const T*>(p.k) + b * p.k_sb + hk * p.k_sh;
@@ -569,7 +629,8 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(const AttnParams p) {
     const bool in = i < p.Lq;
     const T* qp = static_cast<const T*>(p.q) + b * p.q_sb + (int64_t)i * p.q_sl + h * p.q_sh + g * 8;
     const T* gp = static_cast<const T*>(p.dout) + b * p.g_sb + (int64_t)i * p.g_sl + h * p.g_sh + g * 8;
-    const T* op = static_cast<const T*>(p.o) + (((int64_t)b * p.Lq + i) * p.H + h) * p.D + g * 8;
+    const int64_t oat = (((int64_t)b * p.Lq + i) * p.H + h) * p.D + g * 8;
+    const T *op = static_cast<const T*>(p.o) + oat, *rp = static_cast<const T*>(p.rest) + oat;
     // delta = the diagonal of O dO^T by the same products as dP = V dO^T: where one key holds all the weight, O is its value and dS exactly zero
     f32x4 od = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -578,6 +639,10 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(const AttnParams p) {
       qf[n][kp] = on ? frag_row(qp + kp * 32) : frag_zero<T>();
       gf[n][kp] = on ? frag_row(gp + kp * 32) : frag_zero<T>();
       od = attn_mma(od, on ? frag_row(op + kp * 32) : frag_zero<T>(), gf[n][kp]);
+    }
+    if (p.rest) {
+#pragma unroll
+      for (int kp = 0; kp < KP; ++kp) od = attn_mma(od, in && kp * 32 + g * 8 < p.D ? frag_row(rp + kp * 32) : frag_zero<T>(), gf[n][kp]);
     }
     const float mine = (c & 2) ? ((c & 1) ? od.w : od.z) : ((c & 1) ? od.y : od.x);
     delta[n] = __shfl(mine, (c >> 2) * 16 + c);
@@ -592,11 +657,23 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(const AttnParams p) {
 #pragma unroll
     for (int d = 0; d < DT16; ++d) dq[d][n] = f32x4{0.f, 0.f, 0.f, 0.f};
   float* mine = hist + wave * p.nb * 64 + lane;
-  float before = 0.f, after = 0.f;
+  constexpr uint32_t RUN = 0x80000000u;
+  float before = 0.f, after = 0.f, run[NQ];                                    // run: the sum of the lane's current bucket at[]
+  uint32_t at_[NQ];
   if (p.table) load_bias<T>(p, h, bias, 256);
   if (p.part) {
-    for (int e = tid; e < entries; e += 256) place[e] = (uint32_t)min((int)p.lut[min(max(e - 4, 0), 2 * p.far)], p.nb - 1) * 64;
+    for (int e = tid; e < entries; e += 256) {
+      uint32_t k[4];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) k[x] = (uint32_t)min((int)p.lut[min(max(e + x - 4, 0), 2 * p.far)], p.nb - 1) * 64;
+      place[e] = k[0] | (k[0] == k[1] && k[0] == k[2] && k[0] == k[3] ? RUN : 0u);
+    }
     for (int k = 0; k < p.nb; ++k) mine[k * 64] = 0.f;
+  }
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
+    run[n] = 0.f;
+    at_[n] = RUN;                                                              // (bucket 0)
   }
   if (nt > 0) {
     kr.store(kt_, tid);
@@ -643,19 +720,37 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(const AttnParams p) {
         for (int kt = 0; kt < 2; ++kt) {
           const int j = j0 + kc * 32 + kt * 16 + 4 * g;
           const int at = far ? 0 : bias_at(j - pos, p.far);
+          f32x4 add = f32x4{fixed, fixed, fixed, fixed} - lse[n];
+          if (!far) add = bias4(bias + at) - lse[n];
           uint32_t hid = 0u;
           if (cut && sp.mask && i < p.Lq) hid = mask4(sp.mask + (int64_t)i * sp.m_sq, j, p.Lk);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float x = s[kt][n][e] * p.scale2 + (far ? fixed : bias[at + e]);
-            float d = __builtin_amdgcn_exp2f(x - lse[n]) * (w[kt][n][e] - delta[n]);
+            // scale, bias and the row's statistic in one multiply-add
+            float d = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][n][e], p.scale2, add[e])) * (w[kt][n][e] - delta[n]);
             if (cut && (j + e >= end || ((hid >> (8 * e)) & 0xffu))) d = 0.f;
             s[kt][n][e] = d;
-            sum += d;
           }
-          if (p.part && !far)
+          if (p.part) {
+            const float four = (s[kt][n].x + s[kt][n].y) + (s[kt][n].z + s[kt][n].w);
+            sum += four;
+            if (!far) {
+              // a lane's keys follow one another, so its buckets come in runs: a register holds the current one's sum, and LDS is touched where it changes
+              const uint32_t k = place[at];
+              if (!__any(k != at_[n])) {
+                run[n] += four;
+              } else if (k == at_[n]) {
+                run[n] += four;
+              } else if (k & RUN) {
+                lane_add(mine + (at_[n] & ~RUN), run[n]);
+                at_[n] = k;
+                run[n] = four;
+              } else {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) __hip_atomic_fetch_add(mine + place[at + e], s[kt][n][e], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
+                for (int e = 0; e < 4; ++e) lane_add(mine + (place[at + e] & ~RUN), s[kt][n][e]);
+              }
+            }
+          }
         }
         if (far < 0) before += sum;
         if (far > 0) after += sum;
@@ -686,8 +781,10 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(const AttnParams p) {
     }
   }
   if (p.part) {
-    mine[place[0]] += before;
-    mine[place[entries - 1]] += after;
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) lane_add(mine + (at_[n] & ~RUN), run[n]);
+    lane_add(mine + (place[0] & ~RUN), before);
+    lane_add(mine + (place[entries - 1] & ~RUN), after);
     __syncthreads();
     float* out = p.part + ((int64_t)h * p.B * p.tiles + (int64_t)b * p.tiles + qt) * p.nb;
     for (int k = wave; k < p.nb; k += 4) {                                     // a wave adds a bucket's 4 x 64 lanes
@@ -725,7 +822,9 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(const AttnParams p) {
   float* bias = stat + 4 * BQ;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
   const int id = xcd_order(blockIdx.x, gridDim.x);
-  const int bh = id / p.tiles, jt = id - bh * p.tiles;
+  int bh, jt;
+  tile_order(p, id, p.B * p.Hk, &bh, &jt);
+  jt = p.tiles - 1 - jt;                                                       // (the first keys are seen by the most queries)
   const int b = bh / p.Hk, hk = bh - b * p.Hk, share = p.H / p.Hk;
   const int jb = jt * BKB, jw = jb + wave * 16 * NK;                           // the block's and the wave's first key
   Span sp = span_of(p, b, hk * share);
@@ -818,11 +917,14 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(const AttnParams p) {
 #pragma unroll
         for (int n = 0; n < NK; ++n) {
           const int j = jw + n * 16 + c, pos = p0 + i;
-          const int at = far ? 0 : bias_at(j - pos - 3, p.far);                // four neighbours, the last query's first
+          f32x4 add = f32x4{fixed, fixed, fixed, fixed} - ll;
+          if (!far) {
+            const f32x4 w4 = bias4(bias + bias_at(j - pos - 3, p.far));          // four neighbours, the last query's first
+            add = f32x4{w4.w, w4.z, w4.y, w4.x} - ll;
+          }
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float x = s[qq][n][e] * p.scale2 + (far ? fixed : bias[at + 3 - e]);
-            float pr = __builtin_amdgcn_exp2f(x - ll[e]);
+            float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(s[qq][n][e], p.scale2, add[e]));
             if (cut) {
               bool off = j >= sp.klen || (p.causal && j > pos + e);
               if (sp.mask && j < p.Lk && iq + i + e < p.Lq) off |= sp.mask[(int64_t)(iq + i + e) * sp.m_sq + j] != 0;
@@ -884,7 +986,7 @@ static int attn_check(const moy_attention_args* a, bool bwd) {
   if (a->table && (a->num_buckets < 1 || a->num_buckets > 64 || a->max_distance < 1 || a->max_distance > 1024)) return MOY_EINVAL;
   if (reinterpret_cast<uintptr_t>(a->table) % es || reinterpret_cast<uintptr_t>(a->k_len) % 4) return MOY_EINVAL;
   if (a->mask && (a->m_sb < 0 || a->m_sh < 0 || a->m_sq < 0)) return MOY_EINVAL;
-  if (!(a->scale - a->scale == 0.f)) return MOY_EINVAL;
+  if (!(a->scale >= 0.f) || !(a->scale - a->scale == 0.f) || (a->o_rest && !aligned16(a->o_rest))) return MOY_EINVAL;
   if ((int64_t)a->B * a->H > (1 << 24) || (int64_t)a->B * a->H * ((a->Lq > a->Lk ? a->Lq : a->Lk) / 64 + 1) > 0x7fffffffLL / 8) return MOY_EINVAL;
   if (bwd) {
     const int64_t gs[] = {a->g_sb, a->g_sl, a->g_sh};
@@ -908,6 +1010,7 @@ static AttnParams attn_params(const moy_attention_args* a) {
   p.mask = a->mask; p.m_sb = a->m_sb; p.m_sh = a->m_sh; p.m_sq = a->m_sq;
   p.scale = a->scale; p.scale2 = a->scale * LOG2E;
   p.o = a->o; p.lse = a->lse;
+  p.rest = a->dtype == MOY_F32 ? nullptr : a->o_rest;
   p.dout = a->dout; p.g_sb = a->g_sb; p.g_sl = a->g_sl; p.g_sh = a->g_sh;
   p.dq = a->dq; p.dk = a->dk; p.dv = a->dv;
   return p;

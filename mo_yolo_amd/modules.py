@@ -341,16 +341,16 @@ class BiasedAttentionFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, table, lut, causal, q_start, k_len, attn_mask, scale):
-        o, lse = ops.attention_forward(q, k, v, table, lut, causal=causal, q_start=q_start, k_len=k_len, attn_mask=attn_mask, scale=scale, need_lse=True)
-        ctx.save_for_backward(q, k, v, o, lse, table, lut, k_len, attn_mask)
+        o, lse, rest = ops.attention_forward(q, k, v, table, lut, causal=causal, q_start=q_start, k_len=k_len, attn_mask=attn_mask, scale=scale, stats=True)
+        ctx.save_for_backward(q, k, v, o, lse, rest, table, lut, k_len, attn_mask)
         ctx.how = dict(causal=causal, q_start=q_start, scale=scale)
         return o
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        q, k, v, o, lse, table, lut, k_len, attn_mask = ctx.saved_tensors
-        grads = ops.attention_backward(dout, q, k, v, o, lse, table, lut, k_len=k_len, attn_mask=attn_mask, need=ctx.needs_input_grad[:4], **ctx.how)
+        q, k, v, o, lse, rest, table, lut, k_len, attn_mask = ctx.saved_tensors
+        grads = ops.attention_backward(dout, q, k, v, o, lse, rest, table, lut, k_len=k_len, attn_mask=attn_mask, need=ctx.needs_input_grad[:4], **ctx.how)
         return (*grads, None, None, None, None, None, None)
 
 

@@ -672,6 +672,8 @@ def _attention_args(q, k, v, table, lut, causal, q_start, k_len, attn_mask, scal
     (q, (a.q_sb, a.q_sl, a.q_sh)), (k, (a.k_sb, a.k_sl, a.k_sh)), (v, (a.v_sb, a.v_sl, a.v_sh)) = _strided(q), _strided(k), _strided(v)
     a.q, a.k, a.v, a.B, a.H, a.Hk, a.Lq, a.Lk, a.D, a.dtype = q.data_ptr(), k.data_ptr(), v.data_ptr(), B, H, Hk, Lq, Lk, D, code
     a.scale = D ** -0.5 if scale is None else scale
+    if not 0 <= a.scale < float("inf"):
+        raise ValueError("attention: scale must be finite and not negative")
     a.causal, a.q_from_end, a.q_start = int(bool(causal)), int(q_start is None), 0 if q_start is None else int(q_start)
     if abs(a.q_start) > 1 << 30 or (q_start is not None and a.q_start != q_start):
         raise ValueError("attention: q_start out of range")
@@ -705,25 +707,26 @@ def _attention_args(q, k, v, table, lut, causal, q_start, k_len, attn_mask, scal
     return a, keep
 
 
-def attention_forward(q, k, v, table=None, lut=None, *, causal=False, q_start=None, k_len=None, attn_mask=None, scale=None, need_lse=False):
+def attention_forward(q, k, v, table=None, lut=None, *, causal=False, q_start=None, k_len=None, attn_mask=None, scale=None, stats=False):
     """softmax(scale q k^T + bias) v with a learned relative position bias by buckets (moy_attention): q [B, Lq, H, D], k / v [B, Lk, Hk, D] (any
     strides; H a multiple of Hk: shared key heads), D a multiple of 8 up to 128; float32 / bfloat16 / float16.
     table [num_buckets, H] in q's type with lut = relative_buckets(...), or any uint8 map of clamped distances to buckets; none: no bias.
     q_start: position of the first query (keys count from 0); None: the queries are the last of the k_len[b] (or Lk) keys, as with a cache.
     causal: a query sees keys up to its own position.  k_len int32 [B]: keys that count (rows behind them are not read).  attn_mask bool, True = hidden,
     [Lq, Lk] or [B, H, Lq, Lk] with axes of 1 where it does not differ; hidden rows of k / v must still be finite, unless the mask differs
-    neither by query nor by head.  scale: D ** -0.5.  A query that sees no key gets zeros.
-    -> o [B, Lq, H, D], or with need_lse (o, lse) as attention_backward takes them."""
+    neither by query nor by head.  scale: >= 0, D ** -0.5.  A query that sees no key gets zeros.
+    -> o [B, Lq, H, D], or with stats (o, lse, rest) as attention_backward takes them (rest: what the rounding of a 16-bit o left out, else None)."""
     a, keep = _attention_args(q, k, v, table, lut, causal, q_start, k_len, attn_mask, scale)
     with _on(q):
         o = torch.empty(a.B, a.Lq, a.H, a.D, device=q.device, dtype=q.dtype)
-        lse = torch.empty(a.B, a.H, a.Lq, device=q.device, dtype=torch.float32) if need_lse else None
+        lse = torch.empty(a.B, a.H, a.Lq, device=q.device, dtype=torch.float32) if stats else None
+        rest = torch.empty_like(o) if stats and o.dtype != torch.float32 else None
         if o.numel() and a.Lk == 0:
             o.zero_()
-            if need_lse:
+            if stats:
                 lse.fill_(float("-inf"))
         elif o.numel():
-            a.o, a.lse = o.data_ptr(), _ptr(lse)
+            a.o, a.o_rest, a.lse = o.data_ptr(), _ptr(rest), _ptr(lse)
             n = L.lib().moy_attention_ws(C.byref(a))
             if n < 0:
                 L.check(n, "moy_attention_ws")
@@ -731,17 +734,19 @@ def attention_forward(q, k, v, table=None, lut=None, *, causal=False, q_start=No
                 ws = torch.empty(n, device=q.device, dtype=torch.float32)
                 a.ws, a.ws_len = ws.data_ptr(), n
             L.check(L.lib().moy_attention(C.byref(a), _st()), "moy_attention")
-    return (o, lse) if need_lse else o
+    return (o, lse, rest) if stats else o
 
 
-def attention_backward(dout, q, k, v, o, lse, table=None, lut=None, *, causal=False, q_start=None, k_len=None, attn_mask=None, scale=None,
+def attention_backward(dout, q, k, v, o, lse, rest=None, table=None, lut=None, *, causal=False, q_start=None, k_len=None, attn_mask=None, scale=None,
                        need=(True, True, True, True)):
     """Gradients of attention_forward (moy_attention_bwd): (dq, dk, dv, dtable), None where `need` says so.  float16: P and dS are rounded to
     float16 for the matrix cores, so dout wants the usual loss scaling."""
     a, keep = _attention_args(q, k, v, table, lut, causal, q_start, k_len, attn_mask, scale)
-    _one_device(q, dout, o, lse)
+    _one_device(q, dout, o, lse, rest)
     if dout.shape != q.shape or dout.dtype != q.dtype or o.shape != q.shape or o.dtype != q.dtype or not o.is_contiguous():
         raise ValueError("attention_backward: dout and o must have q's shape and type, o contiguous")
+    if rest is not None and (rest.shape != q.shape or rest.dtype != q.dtype or not rest.is_contiguous()):
+        raise ValueError("attention_backward: rest must be the forward's")
     if lse.dtype != torch.float32 or tuple(lse.shape) != (a.B, a.H, a.Lq) or not lse.is_contiguous():
         raise ValueError("attention_backward: lse must be the forward's")
     need = (*need[:3], need[3] and table is not None)
@@ -753,7 +758,7 @@ def attention_backward(dout, q, k, v, o, lse, table=None, lut=None, *, causal=Fa
         if q.numel() == 0 or k.numel() == 0:
             return tuple(t if t is None else t.zero_() for t in out)
         g, (a.g_sb, a.g_sl, a.g_sh) = _strided(dout)
-        a.dout, a.o, a.lse = g.data_ptr(), o.data_ptr(), lse.data_ptr()
+        a.dout, a.o, a.o_rest, a.lse = g.data_ptr(), o.data_ptr(), _ptr(rest), lse.data_ptr()
         a.dq, a.dk, a.dv, a.dtable = (_ptr(t) for t in out)
         n = L.lib().moy_attention_bwd_ws(C.byref(a))
         if n < 0:

@@ -70,7 +70,7 @@ def _attn(bwd=False, **kw):
 BAD_ATTENTION = [dict(q=None), dict(k=None), dict(v=None), dict(o=None), dict(B=0), dict(Lq=0), dict(Lk=-1), dict(H=3), dict(Hk=0), dict(D=12), dict(D=0),
                  dict(dtype=9), dict(q=FAKE + 8), dict(q_sl=257), dict(k_sb=-128), dict(table=FAKE), dict(lut=FAKE),
                  dict(table=FAKE, lut=FAKE, num_buckets=65, max_distance=128), dict(table=FAKE, lut=FAKE, num_buckets=32, max_distance=0),
-                 dict(table=FAKE, lut=FAKE, num_buckets=32, max_distance=1025), dict(scale=float("inf")), dict(scale=float("nan")), dict(q_start=(1 << 30) + 1),
+                 dict(table=FAKE, lut=FAKE, num_buckets=32, max_distance=1025), dict(scale=float("inf")), dict(scale=-0.5), dict(o_rest=FAKE + 8), dict(scale=float("nan")), dict(q_start=(1 << 30) + 1),
                  dict(mask=FAKE, m_sq=-1), dict(k_len=FAKE + 2), dict(B=1 << 20, H=1 << 10, Hk=1)]
 
 
