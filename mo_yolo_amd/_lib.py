@@ -104,6 +104,15 @@ class AttentionArgs(C.Structure):
     ]
 
 
+class LinearArgs(C.Structure):
+    """Mirror of `moy_linear_args` (include/moyolo.h)."""
+    _fields_ = [
+        ("x", vp), ("ldx", i64), ("w", vp), ("ldw", i64), ("b", vp), ("b_dtype", i32), ("act", i32), ("r", vp), ("ldr", i64),
+        ("M", i32), ("N", i32), ("K", i32), ("dtype", i32), ("y", vp), ("ldy", i64), ("z", vp),
+        ("dy", vp), ("ldd", i64), ("dx", vp), ("dw", vp), ("db", vp), ("ws", vp), ("ws_len", i64),
+    ]
+
+
 # name -> (restype, argtypes); every symbol declared in include/moyolo.h
 SIGNATURES = {
     "moy_version": (C.c_int, []),
@@ -157,6 +166,10 @@ SIGNATURES = {
     "moy_layer_norm": (C.c_int, [vp, i64, vp, i64, vp, vp, C.c_int, i64, C.c_int, f32, vp, i64, vp, vp, C.c_int, vp]),
     "moy_layer_norm_bwd": (C.c_int, [vp, i64, vp, i64, vp, i64, vp, C.c_int, vp, vp, i64, C.c_int, vp, i64, vp, vp, vp, i64, C.c_int, vp]),
     "moy_layer_norm_bwd_ws": (i64, [i64, C.c_int, C.c_int]),
+    "moy_linear": (C.c_int, [C.POINTER(LinearArgs), vp]),
+    "moy_linear_bwd": (C.c_int, [C.POINTER(LinearArgs), vp]),
+    "moy_linear_ws": (i64, [C.POINTER(LinearArgs)]),
+    "moy_linear_bwd_ws": (i64, [C.POINTER(LinearArgs)]),
     "moy_attention": (C.c_int, [C.POINTER(AttentionArgs), vp]),
     "moy_attention_bwd": (C.c_int, [C.POINTER(AttentionArgs), vp]),
     "moy_attention_ws": (i64, [C.POINTER(AttentionArgs)]),

@@ -22,7 +22,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libmoyolo.so")
 LIB_DIAG = os.path.join(HERE, "libmoyolo_diag.so")
-SOURCES = ["gemm.hip", "gemm_wreg.hip", "gemm_dma.hip", "conv_ws.hip", "stem_l1.hip", "c2f_fused.hip", "mlp_head.hip", "dec_tail.hip", "dec_mid.hip", "msda_raw.hip", "ops.hip", "layer_norm.hip", "attention.hip"]
+SOURCES = ["gemm.hip", "gemm_wreg.hip", "gemm_dma.hip", "conv_ws.hip", "stem_l1.hip", "c2f_fused.hip", "mlp_head.hip", "dec_tail.hip", "dec_mid.hip", "msda_raw.hip", "ops.hip", "layer_norm.hip", "linear.hip", "attention.hip"]
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++20", "-fPIC", "-Wall", "-Wno-unused-function", "-Rpass-analysis=kernel-resource-usage",
          # no packed fp32 arithmetic (v_pk_add / mul / fma_f32): some of its forms have given wrong results on this hardware now and then, and
          # hipcc forms them by itself from ordinary float code.  The host pass warns that it does not know the feature: harmless

@@ -10,7 +10,7 @@
 // of dw / db stay in registers until a block's last row: one partial row per block goes to the workspace and a second kernel adds the partials in
 // block order, so results do not depend on the order in which blocks run.  Sums and statistics are fp32; y / dx are rounded once.
 // Loads and stores are 16 bytes at any alignment (the hardware splits what crosses a line), so an odd width costs only its last chunk.
-#include "common.hpp"
+#include "chunk.hpp"
 
 namespace moy {
 
@@ -23,48 +23,6 @@ struct LnParams {
   void* y; int64_t ldy;                    // forward: y; backward: dx
   float* mean; float* rstd;
   float* part;                             // backward: [gridDim.x][2][C] partial sums of dw, db (NULL: not wanted)
-};
-
-template <typename T>
-struct Chunk {                             // 16 bytes of a row at any element alignment, as fp32
-  static constexpr int VEC = DT<T>::KPB;
-  static __device__ __forceinline__ void load(const T* p, int n, float (&v)[VEC]) {
-    if (n >= VEC) {
-      u32x4 t;
-      __builtin_memcpy(&t, __builtin_assume_aligned(p, sizeof(T)), 16);
-      unpack(t, v);
-    } else {
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) v[e] = e < n ? DT<T>::load1(p + e) : 0.f;
-    }
-  }
-  static __device__ __forceinline__ void unpack(const u32x4& t, float (&v)[VEC]) {
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const uint32_t u = t[k];             // (a value: a bit cast of the vector's element itself reads element 0)
-      if constexpr (VEC == 4) {
-        v[k] = __builtin_bit_cast(float, u);
-      } else {
-        v[2 * k] = DT<T>::lo(u);
-        v[2 * k + 1] = DT<T>::hi(u);
-      }
-    }
-  }
-  static __device__ __forceinline__ void store(T* p, int n, const float (&v)[VEC]) {
-    if (n >= VEC) {
-      u32x4 t;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        if constexpr (VEC == 4) t[k] = __builtin_bit_cast(uint32_t, v[k]);
-        else t[k] = DT<T>::pack2(v[2 * k], v[2 * k + 1]);
-      }
-      __builtin_memcpy(__builtin_assume_aligned(p, sizeof(T)), &t, 16);
-    } else {
-#pragma unroll
-      for (int e = 0; e < VEC; ++e)
-        if (e < n) DT<T>::store1(p + e, v[e]);
-    }
-  }
 };
 
 // The weights of a lane's chunk, in their own type (fp32, or the activations'): one branch for the chunk, so that its loads go out together.
@@ -85,12 +43,6 @@ __device__ __forceinline__ void ln_weights(const void* p, int dtype, int c, int 
     for (int e = 0; e < VEC; ++e) v[e] = e < 4 ? lo[e] : hi[e & 3];
   }
 }
-__device__ __forceinline__ void ln_weight_store(void* p, int dtype, int i, float v) {
-  if (dtype == MOY_F32) static_cast<float*>(p)[i] = v;
-  else if (dtype == MOY_BF16) DT<bf16_t>::store1(static_cast<bf16_t*>(p) + i, v);
-  else DT<f16_t>::store1(static_cast<f16_t*>(p) + i, v);
-}
-
 // Sum over the TPR lanes (16, a wave, or the block) that hold one row; every lane gets it.  slots: LDS of one reduction round, not used again
 // before another round's barrier has passed.
 template <int TPR>
@@ -274,28 +226,6 @@ __global__ __launch_bounds__(LnGeom<TPR>::THREADS) void ln_bwd_kernel(const LnPa
     }
 }
 
-// dw | db [2 C] = the partial rows added in block order: a block takes 32 columns, 32 threads to a column take every 32nd row, and the 32 sums are
-// added in order.
-__global__ __launch_bounds__(1024) void ln_reduce_kernel(const float* __restrict__ part, int nb, int C, void* dw, void* db, int w_dtype) {
-  __shared__ float s[32][33];
-  const int c = threadIdx.x & 31, k = threadIdx.x >> 5;
-  const int col = blockIdx.x * 32 + c;
-  float v = 0.f;
-  if (col < 2 * C) {
-#pragma unroll 8
-    for (int b = k; b < nb; b += 32) v += part[(int64_t)b * 2 * C + col];
-  }
-  s[k][c] = v;
-  __syncthreads();
-  if (k == 0 && col < 2 * C) {
-    v = 0.f;
-#pragma unroll
-    for (int i = 0; i < 32; ++i) v += s[i][c];
-    void* out = col < C ? dw : db;
-    if (out) ln_weight_store(out, w_dtype, col < C ? col : col - C, v);
-  }
-}
-
 // Lanes and chunks for a row of `chunks` 16-byte pieces: the fewest lanes that hold it in one or two chunks each (registers), 2048 chunks at most
 // (16384 channels of 16 bits, 8192 of fp32).
 static int ln_lanes(int chunks) { return chunks <= 32 ? 16 : chunks <= 128 ? 64 : chunks <= 512 ? 256 : chunks <= 2048 ? 1024 : 0; }
@@ -343,8 +273,6 @@ static int ln_check(int64_t rows, int C, int dtype, int w_dtype, bool weights) {
   return ln_lanes(ln_chunks(C, dtype)) ? MOY_OK : MOY_ENOSYS;
 }
 
-static bool ln_aligned(const void* p, int dtype) { return reinterpret_cast<uintptr_t>(p) % (dtype == MOY_F32 ? 4 : 2) == 0; }
-
 }  // namespace moy
 
 using namespace moy;
@@ -355,7 +283,7 @@ extern "C" int moy_layer_norm(const void* x, int64_t ldx, const void* r, int64_t
   if (rc != MOY_OK) return rc;
   if (!x || !y || (mean == nullptr) != (rstd == nullptr) || !(eps >= 0.f)) return MOY_EINVAL;
   if (rows > 1 && (ldx < 0 || ldy < C || (r && ldr < 0))) return MOY_EINVAL;
-  if (!ln_aligned(x, dtype) || !ln_aligned(y, dtype) || !ln_aligned(r, dtype) || !ln_aligned(w, w_dtype) || !ln_aligned(b, w_dtype)) return MOY_EINVAL;
+  if (!aligned_as(x, dtype) || !aligned_as(y, dtype) || !aligned_as(r, dtype) || !aligned_as(w, w_dtype) || !aligned_as(b, w_dtype)) return MOY_EINVAL;
   LnParams p{};
   p.x = x; p.ldx = ldx; p.r = r; p.ldr = ldr; p.w = w; p.b = b; p.w_dtype = w_dtype;
   p.rows = rows; p.C = C; p.eps = eps; p.y = y; p.ldy = ldy; p.mean = mean; p.rstd = rstd;
@@ -375,8 +303,8 @@ extern "C" int moy_layer_norm_bwd(const void* dy, int64_t ldd, const void* x, in
   if (rc != MOY_OK) return rc;
   if (!dy || !x || !mean || !rstd || (!dx && !dw && !db)) return MOY_EINVAL;
   if (rows > 1 && (ldd < 0 || ldx < 0 || (r && ldr < 0) || (dx && ldo < C))) return MOY_EINVAL;
-  if (!ln_aligned(dy, dtype) || !ln_aligned(x, dtype) || !ln_aligned(r, dtype) || !ln_aligned(dx, dtype) || !ln_aligned(w, w_dtype) ||
-      !ln_aligned(dw, w_dtype) || !ln_aligned(db, w_dtype))
+  if (!aligned_as(dy, dtype) || !aligned_as(x, dtype) || !aligned_as(r, dtype) || !aligned_as(dx, dtype) || !aligned_as(w, w_dtype) ||
+      !aligned_as(dw, w_dtype) || !aligned_as(db, w_dtype))
     return MOY_EINVAL;
   const bool sums = dw || db;
   const int blocks = ln_blocks(rows, ln_lanes(ln_chunks(C, dtype)));
@@ -388,6 +316,6 @@ extern "C" int moy_layer_norm_bwd(const void* dy, int64_t ldd, const void* x, in
   hipStream_t st = static_cast<hipStream_t>(stream);
   const int k = ln_dispatch<true>(p, dtype, st);
   if (k != MOY_OK || !sums) return k;
-  hipLaunchKernelGGL(ln_reduce_kernel, dim3((2 * C + 31) / 32), dim3(1024), 0, st, ws, blocks, C, dw, db, w_dtype);
+  hipLaunchKernelGGL(column_sums_kernel, dim3((2 * C + 31) / 32), dim3(1024), 0, st, ws, blocks, C, C, dw, db, w_dtype);
   return launch_status();
 }

@@ -336,6 +336,32 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, residual=None):
     return ops.layer_norm_forward(x, weight, bias, eps, residual)
 
 
+class LinearFunction(torch.autograd.Function):
+    """Autograd of ops.linear_forward: gradients for x, weight, bias and the residual (the last is dy itself)."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, act, residual):
+        y, z = ops.linear_forward(x, weight, bias, act, residual, keep_pre=True)
+        ctx.save_for_backward(x, weight, z)
+        ctx.act, ctx.bias_dtype = act, None if bias is None else bias.dtype
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, weight, z = ctx.saved_tensors
+        nx, nw, nb, _, nr = ctx.needs_input_grad
+        dx, dw, db = ops.linear_backward(dy, x, weight, z, ctx.act, need=(nx, nw, nb), bias_dtype=ctx.bias_dtype)
+        return dx, dw, db, None, dy if nr else None
+
+
+def linear(x, weight, bias=None, act=L.ACT_NONE, residual=None):
+    """act(x weight^T + bias) + residual, differentiable (arguments as ops.linear_forward); without a gradient to compute, the forward alone."""
+    if _wants_grad(x, weight, bias, residual):
+        return LinearFunction.apply(x, weight, bias, act, residual)
+    return ops.linear_forward(x, weight, bias, act, residual)
+
+
 class BiasedAttentionFunction(torch.autograd.Function):
     """Autograd of ops.attention_forward: gradients for q, k, v and the bias table."""
 

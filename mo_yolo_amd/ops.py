@@ -627,6 +627,86 @@ def layer_norm_backward(dy, x, weight, mean, rstd, residual=None, need=(True, Tr
     return dx, dw, db
 
 
+
+def _linear_args(x, weight, bias, act, residual, bias_dtype=None):
+    """Checks the arguments and lays them out: (moy_linear_args, x as rows, tensors to keep until the launch)."""
+    _one_device(x, weight, bias, residual)
+    code = _code(x)
+    if weight.dim() != 2 or x.dim() == 0 or x.shape[-1] != weight.shape[1] or 0 in weight.shape:
+        raise ValueError("linear: x [..., K], weight [N, K]")
+    if weight.dtype != x.dtype:
+        raise TypeError("linear: x and weight must have one type")
+    n, k = weight.shape
+    if act not in (L.ACT_NONE, L.ACT_SILU, L.ACT_RELU, L.ACT_SIGMOID):
+        raise ValueError("linear: act is one of ACT_NONE, ACT_SILU, ACT_RELU, ACT_SIGMOID")
+    if bias is not None:
+        if tuple(bias.shape) != (n,) or bias.dtype not in (x.dtype, torch.float32):
+            raise ValueError("linear: bias must be [N] in x's type or float32")
+        bias, bias_dtype = bias.contiguous(), bias.dtype
+    if residual is not None and (residual.shape != (*x.shape[:-1], n) or residual.dtype != x.dtype):
+        raise ValueError("linear: residual must be [..., N] in x's type")
+    x2, w2, r2 = _as_rows(x, "x"), _as_rows(weight, "weight"), None if residual is None else _as_rows(residual, "residual")
+    if x2.shape[0] > 0x7fffffff:
+        raise ValueError("linear: more than 2^31 - 1 rows")
+    a = L.LinearArgs()
+    a.x, a.ldx, a.w, a.ldw, a.M, a.N, a.K, a.dtype, a.act = x2.data_ptr(), x2.stride(0), w2.data_ptr(), w2.stride(0), x2.shape[0], n, k, code, act
+    a.b, a.b_dtype = _ptr(bias), L.F32 if bias_dtype in (None, torch.float32) else code
+    if r2 is not None:
+        a.r, a.ldr = r2.data_ptr(), r2.stride(0)
+    return a, [x2, w2, bias, r2]
+
+
+def _linear_ws(a, query, what, dev):
+    n = query(C.byref(a))
+    if n < 0:
+        L.check(n, what)
+    ws = torch.empty(n, device=dev, dtype=torch.uint8) if n else None
+    a.ws, a.ws_len = _ptr(ws), n
+    return ws
+
+
+def linear_forward(x, weight, bias=None, act=L.ACT_NONE, residual=None, keep_pre=False):
+    """act(x weight^T + bias) + residual (moy_linear): x [..., K], weight [N, K] of one type (float32 / bfloat16 / float16), bias [N] in it or float32,
+    residual [..., N]; any sizes, row strides and alignments (rows that are not whole 16-byte steps cost a copy).  -> y, or with keep_pre (y, z):
+    z = what act was applied to, as linear_backward takes it (None for ACT_NONE)."""
+    a, keep = _linear_args(x, weight, bias, act, residual)
+    with _on(x):
+        y = torch.empty(*x.shape[:-1], a.N, device=x.device, dtype=x.dtype)
+        z = torch.empty(a.M, a.N, device=x.device, dtype=x.dtype) if keep_pre and act != L.ACT_NONE else None
+        if a.M:
+            a.y, a.ldy, a.z = y.data_ptr(), a.N, _ptr(z)
+            ws = _linear_ws(a, L.lib().moy_linear_ws, "moy_linear_ws", x.device)  # noqa: F841  (held until the launch)
+            L.check(L.lib().moy_linear(C.byref(a), _st()), "moy_linear")
+    return (y, z) if keep_pre else y
+
+
+def linear_backward(dy, x, weight, z=None, act=L.ACT_NONE, need=(True, True, True), bias_dtype=None):
+    """Gradients of linear_forward (moy_linear_bwd): (dx, dweight, dbias), None where `need` says so; the residual's gradient is dy.  z: linear_forward's
+    for an activation; bias_dtype: the type of dbias (float32, or x's)."""
+    if bias_dtype not in (None, torch.float32, x.dtype):
+        raise ValueError("linear_backward: bias_dtype is x's type or float32")
+    a, keep = _linear_args(x, weight, None, act, None, bias_dtype)
+    _one_device(x, dy, z)
+    if dy.shape != (*x.shape[:-1], a.N) or dy.dtype != x.dtype:
+        raise ValueError("linear_backward: dy must be [..., N] in x's type")
+    if act != L.ACT_NONE and (z is None or tuple(z.shape) != (a.M, a.N) or z.dtype != x.dtype or not z.is_contiguous()):
+        raise ValueError("linear_backward: z must be linear_forward's")
+    with _on(x):
+        dx = torch.empty(x.shape, device=x.device, dtype=x.dtype) if need[0] else None
+        dw = torch.empty(weight.shape, device=x.device, dtype=x.dtype) if need[1] else None
+        db = torch.empty(a.N, device=x.device, dtype=torch.float32 if a.b_dtype == L.F32 else x.dtype) if need[2] else None
+        if a.M == 0:
+            for t in (dw, db):
+                if t is not None:
+                    t.zero_()
+        elif any(need):
+            g = _as_rows(dy, "dy")
+            a.dy, a.ldd, a.z, a.dx, a.dw, a.db = g.data_ptr(), g.stride(0), _ptr(z), _ptr(dx), _ptr(dw), _ptr(db)
+            ws = _linear_ws(a, L.lib().moy_linear_bwd_ws, "moy_linear_bwd_ws", x.device)  # noqa: F841
+            L.check(L.lib().moy_linear_bwd(C.byref(a), _st()), "moy_linear_bwd")
+    return dx, dw, db
+
+
 def relative_buckets(num_buckets, max_distance, bidirectional=True, device="cuda"):
     """The bucket of every clamped distance key - query in [-max_distance, max_distance] as uint8 [2 * max_distance + 1], for attention_forward's
     `lut`: a bucket for each of the nearest distances (half of the buckets), then ranges that grow by a constant factor up to max_distance.

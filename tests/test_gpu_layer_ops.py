@@ -457,3 +457,165 @@ def test_attention_repeats_on_any_stream_and_in_graphs():
         g1.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(o2, want)) and torch.equal(o1, w1), n
+
+
+# ---------------------------------------------------------------------------------------------------------------------- linear
+ACT = {"none": L.ACT_NONE, "silu": L.ACT_SILU, "relu": L.ACT_RELU, "sigmoid": L.ACT_SIGMOID}
+
+
+def linear_reference(x, w, b, r, act, dy):
+    """({y, dx, dw, db} in 64 bits, tolerances)."""
+    dt, K = x.dtype, x.shape[1]
+    M, N = x.shape[0], w.shape[0]
+    xd, wd, g = x.double(), w.double(), dy.double()
+    z, zm = xd @ wd.t(), xd.abs() @ wd.abs().t()
+    if b is not None:
+        z, zm = z + b.double(), zm + b.double().abs()
+    ez = (K + 8) * U32 * zm                                                   # of z in 32 bits
+    s = torch.sigmoid(z)
+    f, d1, d2 = {"none": (z, torch.ones_like(z), 0 * z), "relu": (z.clamp(min=0), (z > 0).double(), 0 * z), "sigmoid": (s, s * (1 - s), s * (1 - s)),
+                 "silu": (z * s, s * (1 + z * (1 - s)), torch.full_like(z, 0.5))}[act]
+    slope = 1.1                                                               # bounds every |act'|
+    y = f + (0 if r is None else r.double())
+    ty = half_step(dt) * y.abs() + tiny(dt) + slope * ez + 16 * U32 * (f.abs() + y.abs() + (s * (1 + z.abs()) if act in ("silu", "sigmoid") else 0))
+    rz = half_step(dt) * z.abs() + tiny(dt) if dt != torch.float32 else 0     # the z that is kept
+    dz = g * d1
+    flip = ((z.abs() <= ez).double() * g.abs()) if act == "relu" else 0       # the sign of a z near 0 may come out either way
+    tz = g.abs() * d2.abs().clamp(max=0.5) * (ez + rz) + 32 * U32 * g.abs() + flip
+    tzr = tz + (half_step(dt) * dz.abs() + tiny(dt) if dt != torch.float32 and act != "none" else 0)
+    dx, dw, db = dz @ wd, dz.t() @ xd, dz.sum(0)
+    e = 1 + half_step(dt)
+    tol = dict(y=ty, dx=e * (tzr @ wd.abs() + (N + 32) * U32 * (dz.abs() @ wd.abs())) + half_step(dt) * dx.abs() + tiny(dt),
+               dw=e * (tzr.t() @ xd.abs() + (M + 32) * U32 * (dz.abs().t() @ xd.abs())) + half_step(dt) * dw.abs() + tiny(dt),
+               db=tz.sum(0) + (M + 600) * U32 * dz.abs().sum(0))
+    return dict(y=y, dx=dx, dw=dw, db=db), tol
+
+
+def check_linear(x, w, b, r, act, dy):
+    leaves = [t for t in (x, w, b, r) if t is not None]
+    for t in leaves:
+        t.requires_grad_(True)
+    y = modules.linear(x, w, b, ACT[act], r)
+    grads = dict(zip([n for n, t in zip(("dx", "dw", "db", "dr"), (x, w, b, r)) if t is not None], torch.autograd.grad(y, leaves, dy)))
+    with torch.no_grad():
+        assert torch.equal(modules.linear(x, w, b, ACT[act], r), y)
+    d = lambda t: None if t is None else t.detach()  # noqa: E731
+    out, tol = linear_reference(d(x), d(w), d(b), d(r), act, dy)
+    if b is not None:
+        tol["db"] = tol["db"] * (1 + half_step(b.dtype)) + half_step(b.dtype) * out["db"].abs() + tiny(b.dtype)
+    close(y, out["y"], tol["y"], "y")
+    for n in ("dx", "dw", "db"):
+        if n in grads:
+            close(grads[n], out[n], tol[n], n)
+    if r is not None:
+        assert torch.equal(grads["dr"], dy)
+
+
+LINEAR = [
+    # M, N, K, act, bias, residual
+    (1, 1, 1, "none", None, False), (1, 4096, 1024, "silu", "own", False), (3, 70, 33, "relu", "f32", True), (16, 256, 256, "sigmoid", "own", True),
+    (17, 130, 520, "none", "own", True), (32, 48, 2050, "silu", "f32", False), (33, 64, 64, "relu", "own", False), (300, 1024, 256, "relu", "f32", True),
+    (300, 256, 1024, "none", "own", True), (127, 129, 131, "silu", "own", True), (1000, 8, 8, "sigmoid", None, False), (4096, 24, 40, "silu", "own", False),
+    (64, 1000, 5000, "none", None, False), (1803, 770, 514, "sigmoid", "own", True), (2500, 640, 128, "silu", "own", False), (70, 3, 4100, "none", "f32", True),
+]
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("shape", LINEAR, ids=lambda s: "-".join(map(str, s)))
+def test_linear(shape, dtype):
+    M, N, K, act, bias, residual = shape
+    dt, gen = DT[dtype], gen_of(M * 31 + N)
+    x, w, dy = rand(gen, M, K, dtype=dt), rand(gen, N, K, dtype=dt, scale=K ** -0.5), rand(gen, M, N, dtype=dt)
+    b = None if bias is None else rand(gen, N, dtype=dt if bias == "own" else torch.float32)
+    check_linear(x, w, b, rand(gen, M, N, dtype=dt) if residual else None, act, dy)
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+def test_linear_large_tiles(dtype):
+    """Enough tiles for the 256-row blocks in every product, with edges that are no multiple of a tile."""
+    dt, gen = DT[dtype], gen_of(77)
+    M, N, K = 4000, 3600, 3500 if dtype == "f32" else 3496
+    x, w, dy = rand(gen, M, K, dtype=dt), rand(gen, N, K, dtype=dt, scale=K ** -0.5), rand(gen, M, N, dtype=dt)
+    check_linear(x, w, rand(gen, N, dtype=dt), rand(gen, M, N, dtype=dt), "silu", dy)
+
+
+def test_linear_exact_on_small_whole_numbers():
+    """Products of small integers are exact in every type and order: a wrong element, a tile too much or too little shows."""
+    for dtype, dt in DT.items():
+        for M, N, K in ((5, 37, 72), (200, 200, 200), (513, 257, 96), (1100, 700, 64), (3000, 2000, 40), (2048, 4096, 72)):
+            gen = gen_of(M)
+            ints = lambda *s: torch.randint(-1, 2, s, device="cuda", generator=gen).to(dt)  # noqa: E731
+            x, w, dy = ints(M, K).requires_grad_(True), ints(N, K).requires_grad_(True), ints(M, N) * (torch.rand(M, N, device="cuda", generator=gen) < 0.04)
+            y = modules.linear(x, w)
+            dx, dw = torch.autograd.grad(y, (x, w), dy)
+            with torch.no_grad():
+                for got, want in ((y, x.float() @ w.float().t()), (dx, dy.float() @ w.float()), (dw, dy.float().t() @ x.float())):
+                    assert float(want.abs().max()) <= 256 and torch.equal(got.float(), want), (dtype, M, N, K)
+
+
+def test_linear_strides_alignment_and_shapes():
+    gen = gen_of(21)
+    for dt in (torch.bfloat16, torch.float32):
+        wide = rand(gen, 90, 600, dtype=dt)
+        w, b = rand(gen, 64, 256, dtype=dt), rand(gen, 64, dtype=dt)
+        for x in (wide[:, 8:264], wide[:, 3:259], wide[::2, 16:272], wide.t()[:256].t()):     # 16-byte steps, odd ones, every other row, the other axis
+            r = wide[:x.shape[0], 5:69]
+            assert torch.equal(ops.linear_forward(x, w, b, L.ACT_SILU, r), ops.linear_forward(x.contiguous(), w, b, L.ACT_SILU, r.contiguous()))
+        wt = rand(gen, 256, 64, dtype=dt).t()
+        assert torch.equal(ops.linear_forward(wide[:, :256], wt), ops.linear_forward(wide[:, :256], wt.contiguous()))
+        x = rand(gen, 2, 5, 9, 256, dtype=dt)
+        assert torch.equal(ops.linear_forward(x, w, b), ops.linear_forward(x.view(90, 256), w, b).view(2, 5, 9, 64))
+        x = rand(gen, 90, 256, dtype=dt).requires_grad_(True)
+        y = modules.linear(x, w, b, L.ACT_RELU)
+        e = torch.autograd.grad(y, x, torch.ones(1, 1, device="cuda", dtype=dt).expand_as(y), retain_graph=True)[0]
+        assert torch.equal(e, torch.autograd.grad(y, x, torch.ones_like(y))[0])
+    w = rand(gen, 4, 8).requires_grad_(True)
+    y = modules.linear(torch.empty(0, 8, device="cuda"), w)
+    assert y.shape == (0, 4) and not torch.autograd.grad(y, w, torch.empty_like(y))[0].any()
+    # C ABI: y in a wider buffer, its other columns left alone
+    x, w = rand(gen, 70, 64, dtype=torch.bfloat16), rand(gen, 30, 64, dtype=torch.bfloat16)
+    buf = torch.full((70, 48), 3.0, device="cuda", dtype=torch.bfloat16)
+    a, keep = ops._linear_args(x, w, None, L.ACT_NONE, None)
+    a.y, a.ldy = buf.data_ptr(), 48
+    ws = ops._linear_ws(a, L.lib().moy_linear_ws, "ws", x.device)  # noqa: F841
+    import ctypes
+    L.check(L.lib().moy_linear(ctypes.byref(a), ops._st()))
+    assert torch.equal(buf[:, :30], ops.linear_forward(x, w)) and bool((buf[:, 30:] == 3.0).all())
+
+
+def test_linear_gradient_against_differences():
+    gen = gen_of(22)
+    x, w, b, r, dy = rand(gen, 40, 50), rand(gen, 30, 50, scale=0.14), rand(gen, 30), rand(gen, 40, 30), rand(gen, 40, 30)
+    for act in ("none", "silu", "sigmoid"):
+        leaves = [t.requires_grad_(True) for t in (x, w, b, r)]
+        grads = torch.autograd.grad(modules.linear(x, w, b, ACT[act], r), leaves, dy)
+        with torch.no_grad():
+            for t, g in zip(leaves, grads):
+                d, h = rand(gen, *t.shape), 2.0 ** -6
+                f = [float((modules.linear(*[u + s * h * d if u is t else u for u in (x, w, b)], ACT[act], r + s * h * d if t is r else r).double() * dy.double()).sum())
+                     for s in (1, -1)]
+                want, size = float((g.double() * d.double()).sum()), float((g.double().abs() * d.double().abs()).sum())
+                assert abs((f[0] - f[1]) / (2 * h) - want) < 1e-2 * size, act
+
+
+def test_linear_repeats_on_any_stream_and_in_graphs():
+    gen = gen_of(23)
+    x, w, b, r = (rand(gen, *s, dtype=torch.float16).requires_grad_(True) for s in ((700, 256), (1024, 256), (1024,), (700, 1024)))
+    dy = rand(gen, 700, 1024, dtype=torch.float16)
+    step = lambda: (lambda y: (y.detach(), *torch.autograd.grad(y, (x, w, b, r), dy)))(modules.linear(x, w, b, L.ACT_SILU, r))  # noqa: E731
+    want = step()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = step()
+    side.synchronize()
+    assert all(torch.equal(a, c) for a, c in zip(got, want))
+    g, out = captured(step)
+    for _ in range(4):
+        with torch.no_grad():
+            x.copy_(rand(gen, 700, 256, dtype=torch.float16))
+            dy.copy_(rand(gen, 700, 1024, dtype=torch.float16))
+        want = step()
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, c) for a, c in zip(out, want))

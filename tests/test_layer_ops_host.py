@@ -118,3 +118,52 @@ def test_attention_refuses_cpu_tensors():
         ops.attention_forward(q, q, q)
     with pytest.raises(RuntimeError, match="Not implemented on the CPU"):
         modules.biased_attention(q.requires_grad_(True), q, q)
+
+
+# ---------------------------------------------------------------------------------------------------------------------- linear
+def _lin(bwd=False, **kw):
+    a = _lib.LinearArgs()
+    a.x = a.w = a.ws = FAKE
+    a.M, a.N, a.K, a.ldx, a.ldw, a.dtype, a.act, a.ws_len = 100, 64, 128, 128, 128, _lib.BF16, _lib.ACT_SILU, 1 << 40
+    if bwd:
+        a.dy = a.z = a.dx = a.dw = a.db = FAKE
+        a.ldd = 64
+    else:
+        a.y, a.ldy = FAKE, 64
+    for n, x in kw.items():
+        setattr(a, n, x)
+    f = _lib.lib().moy_linear_bwd if bwd else _lib.lib().moy_linear
+    return f(C.byref(a), None), (_lib.lib().moy_linear_bwd_ws if bwd else _lib.lib().moy_linear_ws)(C.byref(a))
+
+
+@pytest.mark.parametrize("kw", [dict(x=None), dict(w=None), dict(M=0), dict(N=0), dict(K=-1), dict(dtype=3), dict(act=4), dict(act=-1), dict(b_dtype=_lib.F16),
+                                dict(x=FAKE + 1), dict(ldx=-128)])
+def test_linear_refuses(kw):
+    assert _lin(**kw) == (_lib.EINVAL, _lib.EINVAL) and _lin(True, **kw) == (_lib.EINVAL, _lib.EINVAL)
+
+
+def test_linear_refuses_by_direction_and_size():
+    for kw in (dict(y=None), dict(ldy=63), dict(r=FAKE, ldr=-1), dict(z=FAKE + 1)):
+        assert _lin(**kw)[0] == _lib.EINVAL, kw
+    for kw in (dict(dy=None), dict(z=None), dict(dx=None, dw=None, db=None), dict(dw=FAKE + 1), dict(ws=None), dict(ws_len=1), dict(ws=FAKE + 8)):
+        assert _lin(True, **kw)[0] == _lib.EINVAL, kw
+    assert _lin(K=1 << 22, ldx=1 << 22, ldw=1 << 22)[0] == _lib.ENOSYS and _lin(ldx=1 << 22)[0] == _lib.ENOSYS
+    # workspaces: none where the rows are whole 16-byte steps and the product fills the chip, padded copies otherwise
+    assert _lin(M=16, N=256, ldy=256)[1] == 0
+    assert _lin(M=16, K=100, ldx=100, ldw=100, N=256, ldy=256)[1] == -(-16 * 104 * 2 // 256) * 256 + 256 * 104 * 2
+
+
+def test_linear_args_layout_matches_header():
+    import os
+    import re
+    txt = open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include", "moyolo.h")).read()
+    body = txt[txt.index("typedef struct moy_linear_args {"):txt.index("} moy_linear_args;")].split("{", 1)[1]
+    assert [re.split(r"[ *]+", d.strip())[-1] for d in body.split(";") if d.strip()] == [f[0] for f in _lib.LinearArgs._fields_]
+
+
+def test_linear_refuses_cpu_tensors():
+    x, w = torch.zeros(2, 8), torch.zeros(4, 8)
+    with pytest.raises(RuntimeError, match="Not implemented on the CPU"):
+        ops.linear_forward(x, w)
+    with pytest.raises(RuntimeError, match="Not implemented on the CPU"):
+        modules.linear(x, w.requires_grad_(True))
