@@ -305,27 +305,41 @@ class MSDeformAttnFunction(torch.autograd.Function):
         return gv, None, None, gl, ga, None
 
 
+def _differentiable_once(backward):
+    """once_differentiable, whose guard is needed only where a graph of the backward is asked for (create_graph), and costs as much as a launch."""
+    guarded = torch.autograd.function.once_differentiable(backward)
+
+    def run(ctx, grad):
+        return guarded(ctx, grad) if torch.is_grad_enabled() else backward(ctx, grad)
+    return run
+
+
+def _wants_grad(*ts):
+    if torch.is_grad_enabled():
+        for t in ts:
+            if t is not None and t.requires_grad:
+                return True
+    return False
+
+
 class LayerNormFunction(torch.autograd.Function):
     """Autograd of ops.layer_norm_forward: gradients for x, weight, bias and the residual (x and the residual share theirs)."""
 
     @staticmethod
     def forward(ctx, x, weight, bias, eps, residual):
-        y, mean, rstd = ops.layer_norm_forward(x, weight, bias, eps, residual, stats=True)
-        ctx.save_for_backward(x, weight, residual, mean, rstd)
-        ctx.weight_dtype = None if bias is None else bias.dtype
+        y, stat = ops.layer_norm_forward(x, weight, bias, eps, residual, True)
+        ctx.save_for_backward(x, weight, residual, stat)
+        ctx.types = next((t.dtype for t in (weight, bias) if t is not None), torch.float32)
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_differentiable_once
     def backward(ctx, dy):
-        x, weight, residual, mean, rstd = ctx.saved_tensors
+        x, weight, residual, stat = ctx.saved_tensors
         nx, nw, nb, _, nr = ctx.needs_input_grad
-        dx, dw, db = ops.layer_norm_backward(dy, x, weight, mean, rstd, residual, need=(nx or nr, nw, nb), weight_dtype=ctx.weight_dtype)
+        wdt = ctx.types
+        dx, dw, db = ops._norm_backward(dy, x, weight, stat, residual, (nx or nr, nw, nb), ops._CODES[x.dtype], ops._CODES[wdt], wdt)
         return dx if nx else None, dw, db, None, dx if nr else None
-
-
-def _wants_grad(*ts):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5, residual=None):
@@ -341,17 +355,18 @@ class LinearFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, act, residual):
-        y, z = ops.linear_forward(x, weight, bias, act, residual, keep_pre=True)
+        y, z = ops.linear_forward(x, weight, bias, act, residual, True)
         ctx.save_for_backward(x, weight, z)
-        ctx.act, ctx.bias_dtype = act, None if bias is None else bias.dtype
+        ctx.how = act, torch.float32 if bias is None else bias.dtype
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_differentiable_once
     def backward(ctx, dy):
         x, weight, z = ctx.saved_tensors
         nx, nw, nb, _, nr = ctx.needs_input_grad
-        dx, dw, db = ops.linear_backward(dy, x, weight, z, ctx.act, need=(nx, nw, nb), bias_dtype=ctx.bias_dtype)
+        act, bias_dtype = ctx.how
+        dx, dw, db = ops._linear_backward(dy, x, weight, z, act, (nx, nw, nb), bias_dtype)
         return dx, dw, db, None, dy if nr else None
 
 
@@ -369,15 +384,16 @@ class BiasedAttentionFunction(torch.autograd.Function):
     def forward(ctx, q, k, v, table, lut, causal, q_start, k_len, attn_mask, scale):
         o, lse, rest = ops.attention_forward(q, k, v, table, lut, causal=causal, q_start=q_start, k_len=k_len, attn_mask=attn_mask, scale=scale, stats=True)
         ctx.save_for_backward(q, k, v, o, lse, rest, table, lut, k_len, attn_mask)
-        ctx.how = dict(causal=causal, q_start=q_start, scale=scale)
+        ctx.how = causal, q_start, scale
         return o
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_differentiable_once
     def backward(ctx, dout):
         q, k, v, o, lse, rest, table, lut, k_len, attn_mask = ctx.saved_tensors
-        grads = ops.attention_backward(dout, q, k, v, o, lse, rest, table, lut, k_len=k_len, attn_mask=attn_mask, need=ctx.needs_input_grad[:4], **ctx.how)
-        return (*grads, None, None, None, None, None, None)
+        causal, q_start, scale = ctx.how
+        dq, dk, dv, dtable = ops._attention_backward(dout, q, k, v, o, lse, rest, table, lut, causal, q_start, k_len, attn_mask, scale, ctx.needs_input_grad)
+        return dq, dk, dv, dtable, None, None, None, None, None, None
 
 
 def biased_attention(q, k, v, table=None, lut=None, *, causal=False, q_start=None, k_len=None, attn_mask=None, scale=None):

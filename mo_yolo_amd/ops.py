@@ -514,197 +514,239 @@ def sigmoid_f32(x):
 
 
 # ----------------------------------------------------------------------------- operators of a trained transformer layer
-class _NoGuard:
+# Their host side is on the path of every training step, much of it in autograd's own thread: checks are made once a call (the backward of a Function repeats
+# none of the forward's), and what a launch needs is read without building objects.
+_CODES = {torch.float32: L.F32, torch.bfloat16: L.BF16, torch.float16: L.F16}
+_current_device = torch.cuda.current_device
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+class _On:
+    """`with _On(tensor) as stream`: the tensor's device as the current one for a launch, on its current stream (raw handle)."""
+
+    __slots__ = ("index", "back")
+
+    def __init__(self, t):
+        self.index = t.device.index
+
     def __enter__(self):
-        return None
+        now = _current_device()
+        self.back = None if now == self.index else now
+        if self.back is not None:
+            torch.cuda.set_device(self.index)
+        return _raw_stream(self.index)
 
     def __exit__(self, *exc):
+        if self.back is not None:
+            torch.cuda.set_device(self.back)
         return False
-
-
-_NO_GUARD = _NoGuard()
-
-
-def _on(t):
-    """The tensor's device as the current one for a launch (its current stream is what _st() then names)."""
-    return _NO_GUARD if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
 
 
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def _one_device(*ts):
-    _need_gpu(*ts)
-    dev = None
-    for t in ts:
-        if t is not None:
-            dev = dev or t.device
-            if t.device != dev:
-                raise ValueError(f"tensors on {dev} and {t.device}")
+def _one_device(x, *others):
+    if not x.is_cuda:
+        _need_gpu(x)
+    dev = x.device
+    for t in others:
+        if t is not None and t.device != dev:
+            _need_gpu(t)
+            raise ValueError(f"tensors on {dev} and {t.device}")
 
 
-def _as_rows(t, what):
+def _type_code(x):
+    code = _CODES.get(x.dtype)
+    return _code(x) if code is None else code          # (raises)
+
+
+def _as_rows(t):
     """[..., C] -> a 2-D view [rows, C] with unit column stride (a copy where the strides allow none)."""
-    if t.dim() == 0:
-        raise ValueError(f"{what}: at least one axis expected")
-    t = t if t.dim() == 2 else t.reshape(-1, t.shape[-1]) if t.shape[-1] else t.reshape(0, 0)
+    if t.dim() != 2:
+        t = t.reshape(t.numel() // t.shape[-1], t.shape[-1])
     return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
 
 
-def _norm_check(x, weight, bias, residual, *more):
-    _one_device(x, weight, bias, residual, *more)
-    code = _code(x)
-    if x.dim() == 0 or x.shape[-1] == 0:
+def _norm_check(x, weight, bias, residual):
+    """-> (type code of x, of the weights, the weights' type)"""
+    _one_device(x, weight, bias, residual)
+    code, dt, shape = _type_code(x), x.dtype, x.shape
+    if not shape or shape[-1] == 0:
         raise ValueError("layer_norm: x must be [..., C] with C > 0")
-    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
+    if residual is not None and (residual.shape != shape or residual.dtype != dt):
         raise ValueError("layer_norm: residual must have x's shape and type")
     wdt = None
     for t in (weight, bias):
         if t is not None:
-            if t.dim() != 1 or t.shape[0] != x.shape[-1] or t.dtype not in (x.dtype, torch.float32) or (wdt or t.dtype) != t.dtype:
+            if t.shape != shape[-1:] or (t.dtype != dt and t.dtype != torch.float32) or (wdt is not None and t.dtype != wdt):
                 raise ValueError("layer_norm: weight and bias must be [C], both in x's type or both float32")
             wdt = t.dtype
-    return code, L.F32 if wdt in (None, torch.float32) else code
+    return (code, L.F32, torch.float32) if wdt is None else (code, _CODES[wdt], wdt)
 
 
 def layer_norm_forward(x, weight=None, bias=None, eps=1e-5, residual=None, stats=False):
     """Layer norm of x (+ residual) over the last axis (moy_layer_norm); weight / bias [C] in x's type or float32.  float32 / bfloat16 /
-    float16, any leading shape and row stride.  -> y, or with stats (y, mean, rstd) as layer_norm_backward takes them (fp32, one per row)."""
-    code, wcode = _norm_check(x, weight, bias, residual)
+    float16, any leading shape and row stride.  -> y, or with stats (y, stat) as layer_norm_backward takes it (fp32 [2, rows]: mean, 1 / deviation)."""
+    code, wcode, _ = _norm_check(x, weight, bias, residual)
     if not eps >= 0:
         raise ValueError("layer_norm: eps must not be negative")
-    x2 = _as_rows(x, "x")
-    r2 = None if residual is None else _as_rows(residual, "residual")
+    x2 = _as_rows(x)
+    r2 = None if residual is None else _as_rows(residual)
+    w, b = None if weight is None else weight.contiguous(), None if bias is None else bias.contiguous()
     rows, c = x2.shape
-    w, b = (None if t is None else t.contiguous() for t in (weight, bias))
-    with _on(x):
+    with _On(x) as stream:
         y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
-        mean = rstd = None
-        if stats:
-            mean, rstd = torch.empty(2, rows, device=x.device, dtype=torch.float32).unbind(0)
+        stat = torch.empty(2, rows, device=x.device, dtype=torch.float32) if stats else None
         if rows:
-            L.check(L.lib().moy_layer_norm(x2.data_ptr(), x2.stride(0), _ptr(r2), 0 if r2 is None else r2.stride(0), _ptr(w), _ptr(b), wcode, rows, c,
-                                           eps, y.data_ptr(), c, _ptr(mean), _ptr(rstd), code, _st()), "moy_layer_norm")
-    return (y, mean, rstd) if stats else y
+            at = None if stat is None else stat.data_ptr()
+            rc = L.lib().moy_layer_norm(x2.data_ptr(), x2.stride(0), _ptr(r2), 0 if r2 is None else r2.stride(0), _ptr(w), _ptr(b), wcode, rows, c, eps,
+                                        y.data_ptr(), c, at, None if at is None else at + 4 * rows, code, stream)
+            if rc:
+                L.check(rc, "moy_layer_norm")
+    return (y, stat) if stats else y
 
 
-def layer_norm_backward(dy, x, weight, mean, rstd, residual=None, need=(True, True, True), weight_dtype=None):
-    """Gradients of layer_norm_forward (moy_layer_norm_bwd): (dx, dweight, dbias); dx is the gradient of x and of the residual alike.  need: which of
-    the three are computed (None in the others' place); weight_dtype: the type of dweight / dbias where weight is None (float32)."""
-    code, wcode = _norm_check(x, weight, None, residual, dy, mean, rstd)
-    if weight is None and weight_dtype is not None:
-        if weight_dtype not in (x.dtype, torch.float32):
-            raise ValueError("layer_norm_backward: weight_dtype is x's type or float32")
-        wcode = L.F32 if weight_dtype == torch.float32 else code
-    if dy.shape != x.shape or dy.dtype != x.dtype:
-        raise ValueError("layer_norm_backward: dy must have x's shape and type")
-    x2, g2 = _as_rows(x, "x"), _as_rows(dy, "dy")
-    rows, c = x2.shape
-    for t in (mean, rstd):
-        if t.dtype != torch.float32 or t.numel() != rows or not t.is_contiguous():
-            raise ValueError("layer_norm_backward: mean and rstd must be contiguous float32, one per row")
-    if not any(need):
-        return None, None, None
-    r2 = None if residual is None else _as_rows(residual, "residual")
+def _norm_backward(dy, x, weight, stat, residual, need, code, wcode, wdt):
+    x2, g2 = _as_rows(x), _as_rows(dy)
+    r2 = None if residual is None else _as_rows(residual)
     w = None if weight is None else weight.contiguous()
-    wdt = torch.float32 if wcode == L.F32 else x.dtype
-    with _on(x):
-        dx = torch.empty(x.shape, device=x.device, dtype=x.dtype) if need[0] else None
-        dw, db = (torch.empty(c, device=x.device, dtype=wdt) if n else None for n in need[1:])
+    rows, c = x2.shape
+    with _On(x) as stream:
+        dev = x.device
+        dx = torch.empty(x.shape, device=dev, dtype=x.dtype) if need[0] else None
+        dw = torch.empty(c, device=dev, dtype=wdt) if need[1] else None
+        db = torch.empty(c, device=dev, dtype=wdt) if need[2] else None
         if rows == 0:
             for t in (dw, db):
                 if t is not None:
                     t.zero_()
-            return dx, dw, db
-        n = L.lib().moy_layer_norm_bwd_ws(rows, c, code) if (need[1] or need[2]) else 0
-        if n < 0:
-            L.check(n, "moy_layer_norm_bwd_ws")
-        ws = torch.empty(n, device=x.device, dtype=torch.float32) if n else None
-        L.check(L.lib().moy_layer_norm_bwd(g2.data_ptr(), g2.stride(0), x2.data_ptr(), x2.stride(0), _ptr(r2), 0 if r2 is None else r2.stride(0), _ptr(w),
-                                           wcode, mean.data_ptr(), rstd.data_ptr(), rows, c, _ptr(dx), c, _ptr(dw), _ptr(db), _ptr(ws), n, code,
-                                           _st()), "moy_layer_norm_bwd")
+        elif need[0] or need[1] or need[2]:
+            lib, n, ws = L.lib(), 0, None
+            if need[1] or need[2]:
+                n = lib.moy_layer_norm_bwd_ws(rows, c, code)
+                if n < 0:
+                    L.check(n, "moy_layer_norm_bwd_ws")
+                ws = torch.empty(n, device=dev, dtype=torch.float32)
+            at = stat.data_ptr()
+            rc = lib.moy_layer_norm_bwd(g2.data_ptr(), g2.stride(0), x2.data_ptr(), x2.stride(0), _ptr(r2), 0 if r2 is None else r2.stride(0), _ptr(w), wcode,
+                                        at, at + 4 * rows, rows, c, _ptr(dx), c, _ptr(dw), _ptr(db), _ptr(ws), n, code, stream)
+            if rc:
+                L.check(rc, "moy_layer_norm_bwd")
     return dx, dw, db
 
 
+def layer_norm_backward(dy, x, weight, stat, residual=None, need=(True, True, True), weight_dtype=None):
+    """Gradients of layer_norm_forward (moy_layer_norm_bwd): (dx, dweight, dbias); dx is the gradient of x and of the residual alike.  need: which of
+    the three are computed (None in the others' place); weight_dtype: the type of dweight / dbias where weight is None (float32)."""
+    code, wcode, wdt = _norm_check(x, weight, None, residual)
+    _one_device(x, dy, stat)
+    if weight is None and weight_dtype is not None:
+        if weight_dtype not in (x.dtype, torch.float32):
+            raise ValueError("layer_norm_backward: weight_dtype is x's type or float32")
+        wcode, wdt = _CODES[weight_dtype], weight_dtype
+    if dy.shape != x.shape or dy.dtype != x.dtype:
+        raise ValueError("layer_norm_backward: dy must have x's shape and type")
+    if stat.dtype != torch.float32 or tuple(stat.shape) != (2, x.numel() // x.shape[-1]) or not stat.is_contiguous():
+        raise ValueError("layer_norm_backward: stat must be layer_norm_forward's")
+    return _norm_backward(dy, x, weight, stat, residual, need, code, wcode, wdt)
 
-def _linear_args(x, weight, bias, act, residual, bias_dtype=None):
-    """Checks the arguments and lays them out: (moy_linear_args, x as rows, tensors to keep until the launch)."""
-    _one_device(x, weight, bias, residual)
-    code = _code(x)
-    if weight.dim() != 2 or x.dim() == 0 or x.shape[-1] != weight.shape[1] or 0 in weight.shape:
-        raise ValueError("linear: x [..., K], weight [N, K]")
-    if weight.dtype != x.dtype:
-        raise TypeError("linear: x and weight must have one type")
-    n, k = weight.shape
-    if act not in (L.ACT_NONE, L.ACT_SILU, L.ACT_RELU, L.ACT_SIGMOID):
-        raise ValueError("linear: act is one of ACT_NONE, ACT_SILU, ACT_RELU, ACT_SIGMOID")
-    if bias is not None:
-        if tuple(bias.shape) != (n,) or bias.dtype not in (x.dtype, torch.float32):
-            raise ValueError("linear: bias must be [N] in x's type or float32")
-        bias, bias_dtype = bias.contiguous(), bias.dtype
-    if residual is not None and (residual.shape != (*x.shape[:-1], n) or residual.dtype != x.dtype):
-        raise ValueError("linear: residual must be [..., N] in x's type")
-    x2, w2, r2 = _as_rows(x, "x"), _as_rows(weight, "weight"), None if residual is None else _as_rows(residual, "residual")
-    if x2.shape[0] > 0x7fffffff:
-        raise ValueError("linear: more than 2^31 - 1 rows")
+
+def _linear_args(x, weight, bias, act, residual):
+    """The launch arguments of tensors that have been checked: (moy_linear_args, tensors to keep until the launch)."""
+    x2, w2, r2 = _as_rows(x), _as_rows(weight), None if residual is None else _as_rows(residual)
     a = L.LinearArgs()
-    a.x, a.ldx, a.w, a.ldw, a.M, a.N, a.K, a.dtype, a.act = x2.data_ptr(), x2.stride(0), w2.data_ptr(), w2.stride(0), x2.shape[0], n, k, code, act
-    a.b, a.b_dtype = _ptr(bias), L.F32 if bias_dtype in (None, torch.float32) else code
+    a.x, a.ldx, a.w, a.ldw, a.act, a.dtype = x2.data_ptr(), x2.stride(0), w2.data_ptr(), w2.stride(0), act, _CODES[x.dtype]
+    a.M = x2.shape[0]
+    a.N, a.K = w2.shape
+    if bias is not None:
+        bias = bias.contiguous()
+        a.b, a.b_dtype = bias.data_ptr(), _CODES[bias.dtype]
     if r2 is not None:
         a.r, a.ldr = r2.data_ptr(), r2.stride(0)
-    return a, [x2, w2, bias, r2]
+    return a, (x2, w2, bias, r2)
 
 
-def _linear_ws(a, query, what, dev):
-    n = query(C.byref(a))
+def _linear_check(x, weight, bias, act, residual):
+    _one_device(x, weight, bias, residual)
+    _type_code(x)
+    dt, ws, xs = x.dtype, weight.shape, x.shape
+    if len(ws) != 2 or not xs or xs[-1] != ws[1] or ws[0] == 0 or ws[1] == 0:
+        raise ValueError("linear: x [..., K], weight [N, K]")
+    if weight.dtype != dt:
+        raise TypeError("linear: x and weight must have one type")
+    if act not in (L.ACT_NONE, L.ACT_SILU, L.ACT_RELU, L.ACT_SIGMOID):
+        raise ValueError("linear: act is one of ACT_NONE, ACT_SILU, ACT_RELU, ACT_SIGMOID")
+    if bias is not None and (bias.shape != ws[:1] or (bias.dtype != dt and bias.dtype != torch.float32)):
+        raise ValueError("linear: bias must be [N] in x's type or float32")
+    if residual is not None and (residual.shape != (*xs[:-1], ws[0]) or residual.dtype != dt):
+        raise ValueError("linear: residual must be [..., N] in x's type")
+    if x.numel() // ws[1] > 0x7fffffff:
+        raise ValueError("linear: more than 2^31 - 1 rows")
+
+
+def _linear_run(a, query, launch, what, dev, stream):
+    n = query(a)
     if n < 0:
         L.check(n, what)
-    ws = torch.empty(n, device=dev, dtype=torch.uint8) if n else None
-    a.ws, a.ws_len = _ptr(ws), n
-    return ws
+    if n:
+        ws = torch.empty(n, device=dev, dtype=torch.uint8)
+        a.ws, a.ws_len = ws.data_ptr(), n
+    rc = launch(a, stream)
+    if rc:
+        L.check(rc, what)
 
 
 def linear_forward(x, weight, bias=None, act=L.ACT_NONE, residual=None, keep_pre=False):
     """act(x weight^T + bias) + residual (moy_linear): x [..., K], weight [N, K] of one type (float32 / bfloat16 / float16), bias [N] in it or float32,
     residual [..., N]; any sizes, row strides and alignments (rows that are not whole 16-byte steps cost a copy).  -> y, or with keep_pre (y, z):
     z = what act was applied to, as linear_backward takes it (None for ACT_NONE)."""
+    _linear_check(x, weight, bias, act, residual)
     a, keep = _linear_args(x, weight, bias, act, residual)
-    with _on(x):
-        y = torch.empty(*x.shape[:-1], a.N, device=x.device, dtype=x.dtype)
-        z = torch.empty(a.M, a.N, device=x.device, dtype=x.dtype) if keep_pre and act != L.ACT_NONE else None
+    with _On(x) as stream:
+        dev, n = x.device, a.N
+        y = torch.empty((*x.shape[:-1], n), device=dev, dtype=x.dtype)
+        z = torch.empty(a.M, n, device=dev, dtype=x.dtype) if keep_pre and act != L.ACT_NONE else None
         if a.M:
-            a.y, a.ldy, a.z = y.data_ptr(), a.N, _ptr(z)
-            ws = _linear_ws(a, L.lib().moy_linear_ws, "moy_linear_ws", x.device)  # noqa: F841  (held until the launch)
-            L.check(L.lib().moy_linear(C.byref(a), _st()), "moy_linear")
+            a.y, a.ldy, a.z = y.data_ptr(), n, _ptr(z)
+            lib = L.lib()
+            _linear_run(a, lib.moy_linear_ws, lib.moy_linear, "moy_linear", dev, stream)
     return (y, z) if keep_pre else y
 
 
-def linear_backward(dy, x, weight, z=None, act=L.ACT_NONE, need=(True, True, True), bias_dtype=None):
-    """Gradients of linear_forward (moy_linear_bwd): (dx, dweight, dbias), None where `need` says so; the residual's gradient is dy.  z: linear_forward's
-    for an activation; bias_dtype: the type of dbias (float32, or x's)."""
-    if bias_dtype not in (None, torch.float32, x.dtype):
-        raise ValueError("linear_backward: bias_dtype is x's type or float32")
-    a, keep = _linear_args(x, weight, None, act, None, bias_dtype)
-    _one_device(x, dy, z)
-    if dy.shape != (*x.shape[:-1], a.N) or dy.dtype != x.dtype:
-        raise ValueError("linear_backward: dy must be [..., N] in x's type")
-    if act != L.ACT_NONE and (z is None or tuple(z.shape) != (a.M, a.N) or z.dtype != x.dtype or not z.is_contiguous()):
-        raise ValueError("linear_backward: z must be linear_forward's")
-    with _on(x):
-        dx = torch.empty(x.shape, device=x.device, dtype=x.dtype) if need[0] else None
-        dw = torch.empty(weight.shape, device=x.device, dtype=x.dtype) if need[1] else None
-        db = torch.empty(a.N, device=x.device, dtype=torch.float32 if a.b_dtype == L.F32 else x.dtype) if need[2] else None
+def _linear_backward(dy, x, weight, z, act, need, bias_dtype):
+    a, keep = _linear_args(x, weight, None, act, None)
+    a.b_dtype = _CODES[bias_dtype]
+    with _On(x) as stream:
+        dev, dt = x.device, x.dtype
+        dx = torch.empty(x.shape, device=dev, dtype=dt) if need[0] else None
+        dw = torch.empty(weight.shape, device=dev, dtype=dt) if need[1] else None
+        db = torch.empty(a.N, device=dev, dtype=bias_dtype) if need[2] else None
         if a.M == 0:
             for t in (dw, db):
                 if t is not None:
                     t.zero_()
-        elif any(need):
-            g = _as_rows(dy, "dy")
+        elif need[0] or need[1] or need[2]:
+            g = _as_rows(dy)
             a.dy, a.ldd, a.z, a.dx, a.dw, a.db = g.data_ptr(), g.stride(0), _ptr(z), _ptr(dx), _ptr(dw), _ptr(db)
-            ws = _linear_ws(a, L.lib().moy_linear_bwd_ws, "moy_linear_bwd_ws", x.device)  # noqa: F841
-            L.check(L.lib().moy_linear_bwd(C.byref(a), _st()), "moy_linear_bwd")
+            lib = L.lib()
+            _linear_run(a, lib.moy_linear_bwd_ws, lib.moy_linear_bwd, "moy_linear_bwd", dev, stream)
     return dx, dw, db
+
+
+def linear_backward(dy, x, weight, z=None, act=L.ACT_NONE, need=(True, True, True), bias_dtype=torch.float32):
+    """Gradients of linear_forward (moy_linear_bwd): (dx, dweight, dbias), None where `need` says so; the residual's gradient is dy.  z: linear_forward's
+    for an activation; bias_dtype: the type of dbias (float32, or x's)."""
+    _linear_check(x, weight, None, act, None)
+    _one_device(x, dy, z)
+    if bias_dtype not in (torch.float32, x.dtype):
+        raise ValueError("linear_backward: bias_dtype is x's type or float32")
+    n = weight.shape[0]
+    if dy.shape != (*x.shape[:-1], n) or dy.dtype != x.dtype:
+        raise ValueError("linear_backward: dy must be [..., N] in x's type")
+    if act != L.ACT_NONE and (z is None or tuple(z.shape) != (x.numel() // x.shape[-1], n) or z.dtype != x.dtype or not z.is_contiguous()):
+        raise ValueError("linear_backward: z must be linear_forward's")
+    return _linear_backward(dy, x, weight, z, act, need, bias_dtype)
 
 
 def relative_buckets(num_buckets, max_distance, bidirectional=True, device="cuda"):
@@ -727,64 +769,83 @@ def relative_buckets(num_buckets, max_distance, bidirectional=True, device="cuda
 
 
 def _strided(t):
-    """A view that the attention kernels address: unit stride within a head, 16-byte steps and base (a copy where the strides allow none)."""
-    es = t.element_size()
-    if t.stride(3) != 1 or t.data_ptr() % 16 or any(t.shape[i] > 1 and t.stride(i) * es % 16 for i in range(3)):
+    """(a view that the attention kernels address: unit stride within a head, 16-byte steps and base; its strides of batch, token and head).  A copy where
+    the strides allow none."""
+    sb, sl, sh, sd = t.stride()
+    step = 16 // t.element_size()
+    n = t.shape
+    if sd != 1 or t.data_ptr() % 16 or (sb % step and n[0] > 1) or (sl % step and n[1] > 1) or (sh % step and n[2] > 1):
         t = t.contiguous()
         if t.data_ptr() % 16:
             t = t.clone()
-    return t, [0 if t.shape[i] == 1 else t.stride(i) for i in range(3)]
+        sb, sl, sh, sd = t.stride()
+    return t, 0 if n[0] == 1 else sb, 0 if n[1] == 1 else sl, 0 if n[2] == 1 else sh
 
 
-def _attention_args(q, k, v, table, lut, causal, q_start, k_len, attn_mask, scale):
-    """Checks the arguments and lays them out: (moy_attention_args, tensors to keep until the launch)."""
+def _attention_check(q, k, v, table, lut, q_start, k_len, attn_mask, scale):
     _one_device(q, k, v, table, lut, k_len, attn_mask)
-    code = _code(q)
-    if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape or q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:
+    _type_code(q)
+    dt, qs, ks = q.dtype, q.shape, k.shape
+    if len(qs) != 4 or len(ks) != 4 or v.shape != ks or qs[0] != ks[0] or qs[3] != ks[3]:
         raise ValueError("attention: q [B, Lq, H, D], k and v [B, Lk, Hk, D]")
-    B, Lq, H, D = q.shape
-    Lk, Hk = k.shape[1:3]
-    if k.dtype != q.dtype or v.dtype != q.dtype:
+    if k.dtype != dt or v.dtype != dt:
         raise TypeError("attention: q, k and v must have one type")
+    B, Lq, H, D = qs
+    Lk, Hk = ks[1], ks[2]
     if Hk == 0 or H == 0 or H % Hk or D == 0 or D % 8 or D > 128:
         raise ValueError("attention: H must be a multiple of Hk and D a multiple of 8 up to 128")
-    a = L.AttentionArgs()
-    (q, (a.q_sb, a.q_sl, a.q_sh)), (k, (a.k_sb, a.k_sl, a.k_sh)), (v, (a.v_sb, a.v_sl, a.v_sh)) = _strided(q), _strided(k), _strided(v)
-    a.q, a.k, a.v, a.B, a.H, a.Hk, a.Lq, a.Lk, a.D, a.dtype = q.data_ptr(), k.data_ptr(), v.data_ptr(), B, H, Hk, Lq, Lk, D, code
-    a.scale = D ** -0.5 if scale is None else scale
-    if not 0 <= a.scale < float("inf"):
-        raise ValueError("attention: scale must be finite and not negative")
-    a.causal, a.q_from_end, a.q_start = int(bool(causal)), int(q_start is None), 0 if q_start is None else int(q_start)
-    if abs(a.q_start) > 1 << 30 or (q_start is not None and a.q_start != q_start):
-        raise ValueError("attention: q_start out of range")
-    keep = [q, k, v]
     if (table is None) != (lut is None):
         raise ValueError("attention: table and lut come together")
     if table is not None:
-        if table.dim() != 2 or table.shape[1] != H or not 1 <= table.shape[0] <= 64 or table.dtype != q.dtype:
+        if table.dim() != 2 or table.shape[1] != H or not 1 <= table.shape[0] <= 64 or table.dtype != dt:
             raise ValueError("attention: table must be [num_buckets <= 64, H] in q's type")
         if lut.dim() != 1 or lut.dtype != torch.uint8 or lut.shape[0] % 2 == 0 or not 3 <= lut.shape[0] <= 2049:
             raise ValueError("attention: lut must be uint8 [2 * max_distance + 1], max_distance in 1..1024")
-        table, lut = table.contiguous(), lut.contiguous()
-        a.table, a.lut, a.num_buckets, a.max_distance = table.data_ptr(), lut.data_ptr(), table.shape[0], lut.shape[0] // 2
-        keep += [table, lut]
-    if k_len is not None:
-        if k_len.dtype != torch.int32 or tuple(k_len.shape) != (B,):
-            raise ValueError("attention: k_len must be int32 [B]")
-        k_len = k_len.contiguous()
-        a.k_len = k_len.data_ptr()
-        keep.append(k_len)
+    if k_len is not None and (k_len.dtype != torch.int32 or k_len.dim() != 1 or k_len.shape[0] != B):
+        raise ValueError("attention: k_len must be int32 [B]")
     if attn_mask is not None:
         m = attn_mask
         if m.dtype not in (torch.bool, torch.uint8) or m.dim() not in (2, 4) or m.shape[-1] != Lk:
             raise ValueError("attention: attn_mask must be bool (True: hidden) [Lq or 1, Lk] or [B or 1, H or 1, Lq or 1, Lk]")
-        m = m[None, None] if m.dim() == 2 else m
-        if any(n not in (1, w) for n, w in zip(m.shape, (B, H, Lq))):
+        if any(n != 1 and n != w for n, w in zip(m.shape[-2::-1], (Lq, H, B))):
             raise ValueError("attention: attn_mask does not broadcast to [B, H, Lq, Lk]")
-        m = (m if m.stride(3) == 1 or Lk == 1 else m.contiguous()).view(torch.uint8)
-        a.mask, a.m_sb, a.m_sh, a.m_sq = m.data_ptr(), *(0 if n == 1 else m.stride(i) for i, n in enumerate(m.shape[:3]))
-        keep.append(m)
-    return a, keep
+    if q_start is not None and (q_start != int(q_start) or abs(q_start) > 1 << 30):
+        raise ValueError("attention: q_start out of range")
+    if scale is not None and not 0 <= scale < float("inf"):
+        raise ValueError("attention: scale must be finite and not negative")
+
+
+def _attention_args(q, k, v, table, lut, causal, q_start, k_len, attn_mask, scale):
+    """The launch arguments of tensors that have been checked: (moy_attention_args, tensors to keep until the launch)."""
+    a = L.AttentionArgs()
+    q, a.q_sb, a.q_sl, a.q_sh = _strided(q)
+    k, a.k_sb, a.k_sl, a.k_sh = _strided(k)
+    v, a.v_sb, a.v_sl, a.v_sh = _strided(v)
+    a.q, a.k, a.v, a.dtype = q.data_ptr(), k.data_ptr(), v.data_ptr(), _CODES[q.dtype]
+    a.B, a.Lq, a.H, a.D = q.shape
+    a.Lk, a.Hk = k.shape[1:3]
+    a.scale = a.D ** -0.5 if scale is None else scale
+    a.causal = 1 if causal else 0
+    if q_start is None:
+        a.q_from_end = 1
+    else:
+        a.q_start = int(q_start)
+    if table is not None:
+        table, lut = table.contiguous(), lut.contiguous()
+        a.table, a.lut, a.num_buckets, a.max_distance = table.data_ptr(), lut.data_ptr(), table.shape[0], lut.shape[0] // 2
+    if k_len is not None:
+        k_len = k_len.contiguous()
+        a.k_len = k_len.data_ptr()
+    m = attn_mask
+    if m is not None:
+        if m.stride(-1) != 1 and m.shape[-1] > 1:
+            m = m.contiguous()
+        a.mask = m.data_ptr()
+        sizes, strides = m.shape, m.stride()
+        a.m_sq = 0 if sizes[-2] == 1 else strides[-2]
+        if len(sizes) == 4:
+            a.m_sb, a.m_sh = 0 if sizes[0] == 1 else strides[0], 0 if sizes[1] == 1 else strides[1]
+    return a, (q, k, v, table, lut, k_len, m)
 
 
 def attention_forward(q, k, v, table=None, lut=None, *, causal=False, q_start=None, k_len=None, attn_mask=None, scale=None, stats=False):
@@ -796,54 +857,74 @@ def attention_forward(q, k, v, table=None, lut=None, *, causal=False, q_start=No
     [Lq, Lk] or [B, H, Lq, Lk] with axes of 1 where it does not differ; hidden rows of k / v must still be finite, unless the mask differs
     neither by query nor by head.  scale: >= 0, D ** -0.5.  A query that sees no key gets zeros.
     -> o [B, Lq, H, D], or with stats (o, lse, rest) as attention_backward takes them (rest: what the rounding of a 16-bit o left out, else None)."""
+    _attention_check(q, k, v, table, lut, q_start, k_len, attn_mask, scale)
     a, keep = _attention_args(q, k, v, table, lut, causal, q_start, k_len, attn_mask, scale)
-    with _on(q):
-        o = torch.empty(a.B, a.Lq, a.H, a.D, device=q.device, dtype=q.dtype)
-        lse = torch.empty(a.B, a.H, a.Lq, device=q.device, dtype=torch.float32) if stats else None
-        rest = torch.empty_like(o) if stats and o.dtype != torch.float32 else None
+    with _On(q) as stream:
+        dev = q.device
+        o = torch.empty(q.shape, device=dev, dtype=q.dtype)
+        lse = rest = None
+        if stats:
+            lse = torch.empty(a.B, a.H, a.Lq, device=dev, dtype=torch.float32)
+            rest = torch.empty(q.shape, device=dev, dtype=q.dtype) if a.dtype != L.F32 else None
         if o.numel() and a.Lk == 0:
-            o.zero_()
+            for t in (o, rest):
+                if t is not None:
+                    t.zero_()
             if stats:
                 lse.fill_(float("-inf"))
         elif o.numel():
+            lib = L.lib()
             a.o, a.o_rest, a.lse = o.data_ptr(), _ptr(rest), _ptr(lse)
-            n = L.lib().moy_attention_ws(C.byref(a))
+            n = lib.moy_attention_ws(a)
             if n < 0:
                 L.check(n, "moy_attention_ws")
             if n:
-                ws = torch.empty(n, device=q.device, dtype=torch.float32)
+                ws = torch.empty(n, device=dev, dtype=torch.float32)
                 a.ws, a.ws_len = ws.data_ptr(), n
-            L.check(L.lib().moy_attention(C.byref(a), _st()), "moy_attention")
+            rc = lib.moy_attention(a, stream)
+            if rc:
+                L.check(rc, "moy_attention")
     return (o, lse, rest) if stats else o
+
+
+def _attention_backward(dout, q, k, v, o, lse, rest, table, lut, causal, q_start, k_len, attn_mask, scale, need):
+    with _On(q) as stream:
+        dev, dt = q.device, q.dtype
+        dq = torch.empty(q.shape, device=dev, dtype=dt) if need[0] else None
+        dk = torch.empty(k.shape, device=dev, dtype=dt) if need[1] else None
+        dv = torch.empty(k.shape, device=dev, dtype=dt) if need[2] else None
+        dtable = torch.empty(table.shape, device=dev, dtype=dt) if need[3] and table is not None else None
+        out = (dq, dk, dv, dtable)
+        if q.numel() == 0 or k.numel() == 0:
+            for t in out:
+                if t is not None:
+                    t.zero_()
+        elif any(t is not None for t in out):
+            a, keep = _attention_args(q, k, v, table, lut, causal, q_start, k_len, attn_mask, scale)
+            g, a.g_sb, a.g_sl, a.g_sh = _strided(dout)
+            a.dout, a.o, a.o_rest, a.lse = g.data_ptr(), o.data_ptr(), _ptr(rest), lse.data_ptr()
+            a.dq, a.dk, a.dv, a.dtable = _ptr(dq), _ptr(dk), _ptr(dv), _ptr(dtable)
+            lib = L.lib()
+            n = lib.moy_attention_bwd_ws(a)
+            if n < 0:
+                L.check(n, "moy_attention_bwd_ws")
+            ws = torch.empty(n, device=dev, dtype=torch.float32)
+            a.ws, a.ws_len = ws.data_ptr(), n
+            rc = lib.moy_attention_bwd(a, stream)
+            if rc:
+                L.check(rc, "moy_attention_bwd")
+    return out
 
 
 def attention_backward(dout, q, k, v, o, lse, rest=None, table=None, lut=None, *, causal=False, q_start=None, k_len=None, attn_mask=None, scale=None,
                        need=(True, True, True, True)):
     """Gradients of attention_forward (moy_attention_bwd): (dq, dk, dv, dtable), None where `need` says so.  float16: P and dS are rounded to
     float16 for the matrix cores, so dout wants the usual loss scaling."""
-    a, keep = _attention_args(q, k, v, table, lut, causal, q_start, k_len, attn_mask, scale)
+    _attention_check(q, k, v, table, lut, q_start, k_len, attn_mask, scale)
     _one_device(q, dout, o, lse, rest)
-    if dout.shape != q.shape or dout.dtype != q.dtype or o.shape != q.shape or o.dtype != q.dtype or not o.is_contiguous():
-        raise ValueError("attention_backward: dout and o must have q's shape and type, o contiguous")
-    if rest is not None and (rest.shape != q.shape or rest.dtype != q.dtype or not rest.is_contiguous()):
-        raise ValueError("attention_backward: rest must be the forward's")
-    if lse.dtype != torch.float32 or tuple(lse.shape) != (a.B, a.H, a.Lq) or not lse.is_contiguous():
+    for t in (dout, o, rest):
+        if t is not None and (t.shape != q.shape or t.dtype != q.dtype or (t is not dout and not t.is_contiguous())):
+            raise ValueError("attention_backward: dout, o and rest must have q's shape and type, o and rest as the forward gave them")
+    if lse.dtype != torch.float32 or tuple(lse.shape) != (q.shape[0], q.shape[2], q.shape[1]) or not lse.is_contiguous():
         raise ValueError("attention_backward: lse must be the forward's")
-    need = (*need[:3], need[3] and table is not None)
-    with _on(q):
-        new = lambda t, n: torch.empty(t.shape, device=t.device, dtype=t.dtype) if n else None  # noqa: E731
-        out = [new(t, n) for t, n in zip((q, k, v, table), need)]
-        if not any(need):
-            return tuple(out)
-        if q.numel() == 0 or k.numel() == 0:
-            return tuple(t if t is None else t.zero_() for t in out)
-        g, (a.g_sb, a.g_sl, a.g_sh) = _strided(dout)
-        a.dout, a.o, a.o_rest, a.lse = g.data_ptr(), o.data_ptr(), _ptr(rest), lse.data_ptr()
-        a.dq, a.dk, a.dv, a.dtable = (_ptr(t) for t in out)
-        n = L.lib().moy_attention_bwd_ws(C.byref(a))
-        if n < 0:
-            L.check(n, "moy_attention_bwd_ws")
-        ws = torch.empty(n, device=q.device, dtype=torch.float32)
-        a.ws, a.ws_len = ws.data_ptr(), n
-        L.check(L.lib().moy_attention_bwd(C.byref(a), _st()), "moy_attention_bwd")
-    return tuple(out)
+    return _attention_backward(dout, q, k, v, o, lse, rest, table, lut, causal, q_start, k_len, attn_mask, scale, need)

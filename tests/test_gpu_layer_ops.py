@@ -107,8 +107,8 @@ def test_layer_norm_widest_rows_and_far_mean():
     gen = gen_of(3)
     for dt, c in ((torch.bfloat16, 16384), (torch.float16, 16383), (torch.float32, 8191)):
         x, dy = rand(gen, 3, c, dtype=dt), rand(gen, 3, c, dtype=dt)
-        y, mean, rstd = ops.layer_norm_forward(x, stats=True)
-        dx, dw, db = ops.layer_norm_backward(dy, x, None, mean, rstd)
+        y, stat = ops.layer_norm_forward(x, stats=True)
+        dx, dw, db = ops.layer_norm_backward(dy, x, None, stat)
         out, mag = norm_reference(x, None, None, None, dy, 1e-5)
         for name, got in (("y", y), ("dx", dx), ("dw", dw), ("db", db)):
             close(got, out[name], norm_tolerance(out, mag, name, 3, got.dtype), f"{name} {c}")
@@ -144,8 +144,8 @@ def test_layer_norm_leaves_neighbours_alone_and_repeats():
     x, dy, w = rand(gen, 3001, 97, dtype=torch.float16), rand(gen, 3001, 97, dtype=torch.float16), rand(gen, 97)
     runs = []
     for _ in range(3):
-        y, mean, rstd = ops.layer_norm_forward(x, w, stats=True)
-        runs.append((y, *ops.layer_norm_backward(dy, x, w, mean, rstd)))
+        y, stat = ops.layer_norm_forward(x, w, stats=True)
+        runs.append((y, *ops.layer_norm_backward(dy, x, w, stat)))
     for a in runs[1:]:
         assert all(torch.equal(u, v) for u, v in zip(a, runs[0]))
     pad = torch.full((10, 128), 5.0, device="cuda", dtype=torch.float16)      # C ABI: rows of a wider buffer
@@ -577,9 +577,7 @@ def test_linear_strides_alignment_and_shapes():
     buf = torch.full((70, 48), 3.0, device="cuda", dtype=torch.bfloat16)
     a, keep = ops._linear_args(x, w, None, L.ACT_NONE, None)
     a.y, a.ldy = buf.data_ptr(), 48
-    ws = ops._linear_ws(a, L.lib().moy_linear_ws, "ws", x.device)  # noqa: F841
-    import ctypes
-    L.check(L.lib().moy_linear(ctypes.byref(a), ops._st()))
+    ops._linear_run(a, L.lib().moy_linear_ws, L.lib().moy_linear, "moy_linear", x.device, ops._st())
     assert torch.equal(buf[:, :30], ops.linear_forward(x, w)) and bool((buf[:, 30:] == 3.0).all())
 
 
