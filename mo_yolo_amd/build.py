@@ -28,7 +28,8 @@ FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++20", "-fPIC", "-Wall", "-Wno-u
          # hipcc forms them by itself from ordinary float code.  The host pass warns that it does not know the feature: harmless
          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 # kernels whose vector-memory queue is bookkept by hand (counted vmcnt): no scratch traffic allowed
-RING_KERNELS = ("gemm_wreg_kernel", "conv_ws_kernel", "conv_s2_kernel", "conv_ws_pp_kernel", "conv_ws_pipe_kernel", "gemm_dma_kernel")
+RING_KERNELS = ("gemm_wreg_kernel", "conv_ws_kernel", "conv_s2_kernel", "conv_ws_pp_kernel", "conv_ws_pipe_kernel", "gemm_dma_kernel",
+                "lin_gemm_kernel")
 
 
 def _hipcc():

@@ -10,7 +10,10 @@
 // with one barrier per tile of k.  Products with too few tiles for the chip are split over k: fp32 partial results, joined in order by a second kernel that
 // also runs the epilogue.  Up to 32 rows (a new token of each sequence) take lin_few_kernel, which streams W once through registers.
 // dz is its own pass (it feeds two products and the sums of db; in the products' prologues it would be recomputed for every column tile).
-// Rows whose length or address is not a whole number of 16-byte steps are copied into padded rows first.
+// Loads are 16 bytes from any dword on; where a row ends inside one, the tail is cleared in LDS.  16-bit rows of odd length or at odd elements are
+// copied into padded rows first.
+#include <type_traits>
+
 #include "chunk.hpp"
 
 namespace moy {
@@ -18,6 +21,7 @@ namespace moy {
 struct LinParams {
   const void *a, *b;                       // operands: ROW [M or N][K], COL [K][M or N], row strides lda / ldb (elements)
   int64_t lda, ldb;
+  int64_t a_bytes, b_bytes;                // from the first element to the last one's end
   int M, N, K;
   const void* bias; int bias_dtype, act;
   const void* r; int64_t ldr;
@@ -25,6 +29,7 @@ struct LinParams {
   void* z; int64_t ldz;                    // z as well (NULL: no)
   float* part; int splits, split_tiles;    // split over k: fp32 [splits][M][N], each split_tiles tiles of k
   int tiles_m, tiles_n, vec;               // vec: four neighbouring outputs are one aligned access
+  int clamp;                               // a row of an operand is no whole number of 16-byte pieces
 };
 
 template <typename T>
@@ -75,41 +80,98 @@ __device__ __forceinline__ float lin_act_grad(float v, int act) {
   }
 }
 
-// four outputs of row m from column n on: bias, z, activation, residual
+// the bias of columns n .. n + 3 (zeros without one)
+__device__ __forceinline__ f32x4 lin_bias(const LinParams& p, int n) {
+  f32x4 b = f32x4{0.f, 0.f, 0.f, 0.f};
+  if (p.bias) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (n + e < p.N) b[e] = typed_load(p.bias, p.bias_dtype, n + e);
+  }
+  return b;
+}
+
+// four outputs of row m from column n on, their bias added: z, activation, residual (r: loaded ahead where outputs are whole vectors)
+template <typename T>
+__device__ __forceinline__ void lin_finish_vec(const LinParams& p, int m, int n, f32x4 v, f32x4 r) {
+  if (p.z) DT<T>::store4(static_cast<T*>(p.z) + (int64_t)m * p.ldz + n, v);
+  if (p.act != MOY_ACT_NONE) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = lin_act<T>(v[e], p.act);
+  }
+  DT<T>::store4(static_cast<T*>(p.y) + (int64_t)m * p.ldy + n, p.r ? v + r : v);
+}
+template <typename T>
+__device__ __forceinline__ void lin_finish_each(const LinParams& p, int m, int n, f32x4 v) {
+#pragma unroll 1
+  for (int e = 0; e < 4; ++e) {
+    if (n + e >= p.N) break;
+    float u = e == 0 ? v.x : e == 1 ? v.y : e == 2 ? v.z : v.w;
+    const int64_t at = (int64_t)m * p.ldy + n + e;
+    if (p.z) DT<T>::store1(static_cast<T*>(p.z) + (int64_t)m * p.ldz + n + e, u);
+    u = lin_act<T>(u, p.act);
+    if (p.r) u += DT<T>::load1(static_cast<const T*>(p.r) + (int64_t)m * p.ldr + n + e);
+    DT<T>::store1(static_cast<T*>(p.y) + at, u);
+  }
+}
+template <typename T>
+__device__ __forceinline__ f32x4 lin_residual(const LinParams& p, int m, int n) {
+  return p.r ? DT<T>::load4(static_cast<const T*>(p.r) + (int64_t)m * p.ldr + n) : f32x4{0.f, 0.f, 0.f, 0.f};
+}
 template <typename T>
 __device__ __forceinline__ void lin_finish(const LinParams& p, int m, int n, f32x4 v) {
   if (m >= p.M || n >= p.N) return;
-  T* y = static_cast<T*>(p.y) + (int64_t)m * p.ldy + n;
-  T* z = p.z ? static_cast<T*>(p.z) + (int64_t)m * p.ldz + n : nullptr;
-  const T* r = p.r ? static_cast<const T*>(p.r) + (int64_t)m * p.ldr + n : nullptr;
-  if (p.vec) {                             // (N is a multiple of 4 then)
-    if (p.bias) v += f32x4{typed_load(p.bias, p.bias_dtype, n), typed_load(p.bias, p.bias_dtype, n + 1), typed_load(p.bias, p.bias_dtype, n + 2),
-                           typed_load(p.bias, p.bias_dtype, n + 3)};
-    if (z) DT<T>::store4(z, v);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = lin_act<T>(v[e], p.act);
-    if (r) v += DT<T>::load4(r);
-    DT<T>::store4(y, v);
-  } else {
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (n + e < p.N) {
-        float u = v[e] + (p.bias ? typed_load(p.bias, p.bias_dtype, n + e) : 0.f);
-        if (z) DT<T>::store1(z + e, u);
-        u = lin_act<T>(u, p.act);
-        DT<T>::store1(y + e, r ? u + DT<T>::load1(r + e) : u);
-      }
-  }
+  v += lin_bias(p, n);
+  if (p.vec) lin_finish_vec<T>(p, m, n, v, lin_residual<T>(p, m, n));
+  else lin_finish_each<T>(p, m, n, v);
 }
+
+// the activation on four values, its choice taken once
+template <typename T>
+__device__ __forceinline__ f32x4 lin_act4(f32x4 v, int act) {
+  if (act == MOY_ACT_RELU) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = v[e] < 0.f ? 0.f : v[e];
+  } else if (act != MOY_ACT_NONE) {
+    const f32x4 u = v;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = lin_sigmoid<T>(v[e]);
+    if (act == MOY_ACT_SILU) v = u * v;
+  }
+  return v;
+}
+
+// Quads of a matrix from row m0, column n0 on; a lane that is not `in` reads zeros and writes nothing.
+template <typename T>
+struct Out {
+  __amdgpu_buffer_rsrc_t rs;
+  int64_t pitch;
+  __device__ __forceinline__ Out(const void* p, int64_t ld, int m0, int n0) : pitch(ld * (int)sizeof(T)) {
+    rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(static_cast<const T*>(p) + m0 * ld + n0), 0, 0x7fffffffu, 0x00020000);
+  }
+  __device__ __forceinline__ uint32_t at(int row, int quad, bool in) const { return in ? (uint32_t)(row * (int)pitch + quad * 4 * (int)sizeof(T)) : 0x80000000u; }
+  __device__ __forceinline__ void store4(int row, int quad, bool in, f32x4 v) const {
+    if constexpr (sizeof(T) == 4) __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), rs, at(row, quad, in), 0, 0);
+    else __builtin_amdgcn_raw_buffer_store_b64(u32x2{DT<T>::pack2(v.x, v.y), DT<T>::pack2(v.z, v.w)}, rs, at(row, quad, in), 0, 0);
+  }
+  __device__ __forceinline__ f32x4 load4(int row, int quad, bool in) const {
+    if constexpr (sizeof(T) == 4) {
+      return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, at(row, quad, in), 0, 0));
+    } else {
+      const u32x2 w = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rs, at(row, quad, in), 0, 0));
+      const uint32_t a = w.x, b = w.y;
+      return f32x4{DT<T>::lo(a), DT<T>::hi(a), DT<T>::lo(b), DT<T>::hi(b)};
+    }
+  }
+};
 
 // 16 bytes for each lane from memory to LDS (wave-uniform LDS base + lane * 16); an offset past the descriptor's range brings zeros.  No register is written; the
 // kernel waits on vmcnt itself.
+// The first one waits out a descriptor that vector code may have written (the compiler does not see into the block).
+template <bool FIRST>
 __device__ __forceinline__ void lin_dma16(uint32_t voff, __amdgpu_buffer_rsrc_t rs, uint32_t lds) {
-  unsigned keep;
-  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %3, 0 offen lds\n\ts_mov_b32 m0, %0"
-               : "=&s"(keep)
-               : "v"(voff), "s"(lds), "s"(rs)
-               : "memory");
+  if constexpr (FIRST) asm volatile("s_mov_b32 m0, %1\n\ts_nop 4\n\tbuffer_load_dwordx4 %0, %2, 0 offen lds" ::"v"(voff), "s"(lds), "s"(rs) : "memory", "m0");
+  else asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %2, 0 offen lds" ::"v"(voff), "s"(lds), "s"(rs) : "memory", "m0");
 }
 
 typedef short lin_s16x4 __attribute__((ext_vector_type(4)));
@@ -143,11 +205,26 @@ struct LinTile {
       }
     }
   }
-  // base: of the tile's rows at this k; left: elements of k from here on
-  __device__ __forceinline__ void issue(const T* base, int left, uint32_t lds, int wave) const {
-    const auto rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(base), 0, 0x7fffffffu, 0x00020000);
+  // base: of the tile's rows at this k; range: bytes from there to the operand's end (the hardware clamps by dwords); left: elements of k from here on (0: a
+  // tile of zeros, which keeps the count of loads in flight)
+  __device__ __forceinline__ void issue(const T* base, uint32_t range, int left, uint32_t lds, int wave) const {
+    const auto rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(base), 0, range, 0x00020000);
 #pragma unroll
-    for (int i = 0; i < N; ++i) lin_dma16(at[i] < left ? off[i] : 0x80000000u, rs, lds + (i * WAVES + wave) * 1024);
+    for (int i = 0; i < N; ++i) {
+      const uint32_t o = at[i] < left ? off[i] : 0x80000000u, to = lds + (i * WAVES + wave) * 1024;
+      if (i == 0) lin_dma16<true>(o, rs, to);
+      else lin_dma16<false>(o, rs, to);
+    }
+  }
+  // a landed ROW tile whose rows end inside a 16-byte piece: what stands behind the row's `left` elements is cleared
+  static __device__ __forceinline__ void clear_tail(unsigned char* lds, int left, int tid, int threads) {
+    if constexpr (!COL) {
+      const int c = left / VEC, e0 = left % VEC;
+      for (int r = tid; r < R; r += threads) {
+        T* p = reinterpret_cast<T*>(lds + r * 128 + ((c ^ swz(r)) << 4));
+        for (int e = e0; e < VEC; ++e) DT<T>::store1(p + e, 0.f);
+      }
+    }
   }
   // the operand of 16 rows from r0 on, k panel kp (32 elements)
   static __device__ __forceinline__ LFrag<T> frag(const unsigned char* lds, int r0, int kp, int lane) {
@@ -180,7 +257,15 @@ struct LinTile {
   }
 };
 
-template <typename T, bool ACOL, bool BCOL, int WM, int WN, int MI, int NI>
+template <int N>
+__device__ __forceinline__ void lin_landed() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+template <typename T, bool ACOL, bool BCOL, int WM, int WN, int MI, int NI, int STAGES>
 __global__ __launch_bounds__(WM * WN * 64) void lin_gemm_kernel(const LinParams p) {
   constexpr int WAVES = WM * WN, BM = WM * MI * 16, BN = WN * NI * 16, KP = 4 / (int)sizeof(T);
   using TA = LinTile<T, ACOL, BM, WAVES>;
@@ -208,67 +293,147 @@ __global__ __launch_bounds__(WM * WN * 64) void lin_gemm_kernel(const LinParams 
   const T* ab = static_cast<const T*>(p.a) + (ACOL ? (int64_t)m0 : (int64_t)m0 * p.lda);
   const T* bb = static_cast<const T*>(p.b) + (BCOL ? (int64_t)n0 : (int64_t)n0 * p.ldb);
   const int64_t as = ACOL ? BK * p.lda : BK, bs = BCOL ? BK * p.ldb : BK;
+  // A 16-byte piece reaches past the operand's end only where a row is no whole number of pieces: elsewhere the range is left wide (p.clamp)
+  int64_t a_left = p.a_bytes - (reinterpret_cast<const char*>(ab) - static_cast<const char*>(p.a)) - t0 * as * (int64_t)sizeof(T);
+  int64_t b_left = p.b_bytes - (reinterpret_cast<const char*>(bb) - static_cast<const char*>(p.b)) - t0 * bs * (int64_t)sizeof(T);
+  ab += t0 * as;
+  bb += t0 * bs;
+  int left = p.K - t0 * BK;
+  if (t0 >= t1) left = 0;
+  int more = t1 - t0;                                                          // tiles that are still to be fetched
   const uint32_t lds = (uint32_t)reinterpret_cast<uintptr_t>(smem);
-  auto issue = [&](int t) {
-    const uint32_t to = lds + ((t - t0) & 1) * BUF;
-    ta.issue(ab + t * as, p.K - t * BK, to, wave);
-    tb.issue(bb + t * bs, p.K - t * BK, to + TA::BYTES, wave);
+  auto issue = [&](int slot) {
+    const uint32_t to = lds + slot * BUF;
+    uint32_t ra = 0x7fffffffu, rb = 0x7fffffffu;
+    if (p.clamp) {
+      ra = a_left < 0 ? 0u : a_left < 0x7fffffff ? (uint32_t)a_left : 0x7fffffffu;
+      rb = b_left < 0 ? 0u : b_left < 0x7fffffff ? (uint32_t)b_left : 0x7fffffffu;
+      a_left -= as * (int64_t)sizeof(T);
+      b_left -= bs * (int64_t)sizeof(T);
+    }
+    const int have = more > 0 ? left : 0;
+    ta.issue(ab, ra, have, to, wave);
+    tb.issue(bb, rb, have, to + TA::BYTES, wave);
+    ab += as;
+    bb += bs;
+    left -= BK;
+    --more;
   };
   f32x4 acc[MI][NI];
 #pragma unroll
   for (int i = 0; i < MI; ++i)
 #pragma unroll
     for (int j = 0; j < NI; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  if (t0 < t1) issue(t0);
+  // STAGES buffers: STAGES - 1 tiles are on their way ahead of the one in the matrix cores
+#pragma unroll
+  for (int x = 0; x < STAGES - 1; ++x) issue(x);
+  int slot = 0;
   for (int t = t0; t < t1; ++t) {
-    // tile t has landed for every wave, and every wave is done with the buffer that the next one fills
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_sched_barrier(0);
-    __builtin_amdgcn_s_barrier();
-    __builtin_amdgcn_sched_barrier(0);
-    if (t + 1 < t1) issue(t + 1);
-    const unsigned char* buf = smem + ((t - t0) & 1) * BUF;
+    // tile t has landed for every wave, and every wave is done with the buffer that is filled next
+    lin_landed<(STAGES - 2) * (TA::N + TB::N)>();
+    unsigned char* buf = smem + slot * BUF;
+    const int next = slot == 0 ? STAGES - 1 : slot - 1;
+    slot = slot == STAGES - 1 ? 0 : slot + 1;
+    if (t == nk - 1 && p.K % TA::VEC) {
+      TA::clear_tail(buf, p.K - t * BK, tid, WAVES * 64);
+      TB::clear_tail(buf + TA::BYTES, p.K - t * BK, tid, WAVES * 64);
+      lin_landed<63>();                                                        // (the loads in flight stay in flight)
+    }
+    // the first panel's operands are on their way out of LDS while the next tile's loads are issued, each further panel's while the one before is multiplied
+    LFrag<T> fa[KP][MI], fb[KP][NI];
+    auto read = [&](int kp) {
+#pragma unroll
+      for (int j = 0; j < NI; ++j) fb[kp][j] = TB::frag(buf + TA::BYTES, (wn * NI + j) * 16, kp, lane);
+#pragma unroll
+      for (int i = 0; i < MI; ++i) fa[kp][i] = TA::frag(buf, (wm * MI + i) * 16, kp, lane);
+    };
+    read(0);
+    issue(next);
 #pragma unroll
     for (int kp = 0; kp < KP; ++kp) {
-      LFrag<T> fb[NI];
+      if (kp + 1 < KP) read(kp + 1);
 #pragma unroll
-      for (int j = 0; j < NI; ++j) fb[j] = TB::frag(buf + TA::BYTES, (wn * NI + j) * 16, kp, lane);
+      for (int i = 0; i < MI; ++i)
 #pragma unroll
-      for (int i = 0; i < MI; ++i) {
-        const LFrag<T> fa = TA::frag(buf, (wm * MI + i) * 16, kp, lane);
-#pragma unroll
-        for (int j = 0; j < NI; ++j) acc[i][j] = lin_mma(acc[i][j], fb[j], fa);
-      }
+        for (int j = 0; j < NI; ++j) acc[i][j] = lin_mma(acc[i][j], fb[kp][j], fa[kp][i]);
     }
     __builtin_amdgcn_sched_barrier(0);
   }
-  // Epilogue: 16 rows of the wave at a time by way of its own corner of LDS, so that memory is read and written in whole row pieces
-  constexpr int PITCH = NI * 16 + 4, QUADS = NI * 4, ROWS = 64 / QUADS;
-  static_assert(WAVES * 16 * PITCH * 4 <= 2 * BUF, "the corners fit the tiles");
-  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");                  // (every wave's reads of the tiles are back)
-  __builtin_amdgcn_sched_barrier(0);
-  __builtin_amdgcn_s_barrier();
-  __builtin_amdgcn_sched_barrier(0);
-  float* corner = reinterpret_cast<float*>(smem) + wave * 16 * PITCH;
+  // Epilogue: H * 16 rows of the wave at a time by way of its own corner of LDS (quads at quad ^ row: no conflicts either way), so that memory is read and
+  // written in whole row pieces, and by a loop whose code is small: every block meets it once, cold.
+  constexpr int QUADS = NI * 4, ROWS = 64 / QUADS, H = MI < 4 ? MI : 4;
+  static_assert(WAVES * H * 16 * NI * 16 * 4 <= STAGES * BUF, "the corners fit the tiles");
+  lin_landed<0>();                                                             // every wave's reads of the tiles are back, no load is on its way
+  float* corner = reinterpret_cast<float*>(smem) + wave * H * 16 * NI * 16;
+  const int row0 = lane / QUADS, quad = lane % QUADS, n = n0 + wn * NI * 16 + quad * 4;
+  const bool inside = n < p.N;
+  const f32x4 bias = p.part ? f32x4{0.f, 0.f, 0.f, 0.f} : lin_bias(p, n);
+  const bool whole = p.part ? p.N % 4 == 0 : p.vec;                            // four neighbours are one access
+  // Whole quads go by descriptors whose range drops what lies outside C: no branch, so that a wait for a residual never waits for the stores behind it.
+  // A residual is fetched four row pieces ahead.
+  const int mw = m0 + wm * MI * 16, nw = n0 + wn * NI * 16;                    // the wave's corner of C
+  Out<T> oy(p.y, p.ldy, mw, nw), oz(p.z, p.ldz, mw, nw), orr(p.r, p.ldr, mw, nw);
+  Out<float> op(p.part ? p.part + (int64_t)split * p.M * p.N : nullptr, p.N, mw, nw);
 #pragma unroll
-  for (int i = 0; i < MI; ++i) {
+  for (int half = 0; half < MI / H; ++half) {
 #pragma unroll
-    for (int j = 0; j < NI; ++j) *reinterpret_cast<f32x4*>(corner + c * PITCH + j * 16 + g * 4) = acc[i][j];
+    for (int i = 0; i < H; ++i)
+#pragma unroll
+      for (int j = 0; j < NI; ++j)
+        *reinterpret_cast<f32x4*>(corner + (i * 16 + c) * (NI * 16) + (((j * 4 + g) ^ (c & (QUADS - 1))) << 2)) = acc[half * H + i][j];
     __builtin_amdgcn_wave_barrier();
+    const int down = half * H * 16 + row0;                                     // the lane's first row below the wave's corner
+    auto value = [&](int x) {                                                  // x rows further down
+      const int row = row0 + x;
+      return *reinterpret_cast<const f32x4*>(corner + row * (NI * 16) + ((quad ^ (row & (QUADS - 1))) << 2)) + bias;
+    };
+    auto there = [&](int x) { return inside && mw + down + x < p.M; };
+    auto rows = [&](auto res) {
+      constexpr bool RES = decltype(res)::value;
+      f32x4 r[4];
+      if constexpr (RES) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) r[k] = orr.load4(down + k * ROWS, quad, there(k * ROWS));
+      }
 #pragma unroll 1
-    for (int row = lane / QUADS; row < 16; row += ROWS) {
-      const int m = m0 + (wm * MI + i) * 16 + row, n = n0 + wn * NI * 16 + lane % QUADS * 4;
-      const f32x4 v = *reinterpret_cast<const f32x4*>(corner + row * PITCH + lane % QUADS * 4);
-      if (!p.part) {
-        lin_finish<T>(p, m, n, v);
-      } else if (m < p.M && n < p.N) {
-        float* o = p.part + ((int64_t)split * p.M + m) * p.N + n;
-        if (p.N % 4 == 0) {
-          *reinterpret_cast<f32x4*>(o) = v;
-        } else {
+      for (int x = 0; x < H * 16; x += 4 * ROWS) {
+        f32x4 now[4];
+        if constexpr (RES) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) now[k] = r[k];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) r[k] = orr.load4(down + x + (4 + k) * ROWS, quad, x + (4 + k) * ROWS < H * 16 && there(x + (4 + k) * ROWS));
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          f32x4 v = value(x + k * ROWS);
+          const bool in = there(x + k * ROWS);
+          if (p.z) oz.store4(down + x + k * ROWS, quad, in, v);
+          v = lin_act4<T>(v, p.act);
+          if constexpr (RES) v += now[k];
+          oy.store4(down + x + k * ROWS, quad, in, v);
+        }
+      }
+    };
+    static_assert(H * 16 % (4 * ROWS) == 0, "whole steps");
+    if (p.part && whole) {
+#pragma unroll 2
+      for (int x = 0; x < H * 16; x += ROWS) op.store4(down + x, quad, there(x), value(x));
+    } else if (whole && p.r) {
+      rows(std::true_type{});
+    } else if (whole) {
+      rows(std::false_type{});
+    } else if (inside) {
+#pragma unroll 1
+      for (int x = 0; x < H * 16 && there(x); x += ROWS) {
+        const f32x4 v = value(x);
+        if (p.part) {
+          float* o = p.part + ((int64_t)split * p.M + mw + down + x) * p.N + n;
 #pragma unroll
           for (int e = 0; e < 4; ++e)
             if (n + e < p.N) o[e] = v[e];
+        } else {
+          lin_finish_each<T>(p, mw + down + x, n, v);
         }
       }
     }
@@ -311,13 +476,19 @@ __global__ __launch_bounds__(512) void lin_few_kernel(const LinParams p) {
   f32x4 acc[MI];
 #pragma unroll
   for (int i = 0; i < MI; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-  auto get = [&](const T* q, bool in) {
+  // eight elements at any alignment, `left` of them there
+  auto get = [&](const T* q, int left) {
     LFrag<T> f;
-    if constexpr (sizeof(T) == 2) {
-      f.w = in ? *reinterpret_cast<const u32x4*>(q) : u32x4{0u, 0u, 0u, 0u};
-    } else {                                                                  // (K is a multiple of 4 here, the lane's eight may be half there)
-      f.lo = in ? *reinterpret_cast<const f32x4*>(q) : f32x4{0.f, 0.f, 0.f, 0.f};
-      f.hi = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (left >= 8) {
+      __builtin_memcpy(&f, __builtin_assume_aligned(q, sizeof(T)), 8 * sizeof(T));
+    } else {
+      T v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        DT<T>::store1(v + e, 0.f);
+        if (e < left) v[e] = q[e];
+      }
+      __builtin_memcpy(&f, v, 8 * sizeof(T));
     }
     return f;
   };
@@ -325,17 +496,10 @@ __global__ __launch_bounds__(512) void lin_few_kernel(const LinParams p) {
     LFrag<T> fw[U], fx[U][MI];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int k = k0 + u * 32 + g * 8;
-      fw[u] = get(w + k0 + u * 32, n < p.N && k < p.K);
-      if constexpr (sizeof(T) == 4)
-        if (n < p.N && k + 4 < p.K) fw[u].hi = *reinterpret_cast<const f32x4*>(w + k0 + u * 32 + 4);
+      const int left = p.K - (k0 + u * 32 + g * 8);
+      fw[u] = get(w + k0 + u * 32, n < p.N ? left : 0);
 #pragma unroll
-      for (int i = 0; i < MI; ++i) {
-        const bool row = i * 16 + c < p.M;
-        fx[u][i] = get(x + (int64_t)i * 16 * p.lda + k0 + u * 32, row && k < p.K);
-        if constexpr (sizeof(T) == 4)
-          if (row && k + 4 < p.K) fx[u][i].hi = *reinterpret_cast<const f32x4*>(x + (int64_t)i * 16 * p.lda + k0 + u * 32 + 4);
-      }
+      for (int i = 0; i < MI; ++i) fx[u][i] = get(x + (int64_t)i * 16 * p.lda + k0 + u * 32, i * 16 + c < p.M ? left : 0);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u)
@@ -414,31 +578,42 @@ struct LinPick {
   int splits, split_tiles;
 };
 
-// The largest tile that still gives the chip's 256 compute units a block each, splits of at least four tiles of k counted in (16 at most); 64 otherwise.
+// Tile and splits by an estimate in cycles, from what the kernel measured (bf16 / fp32, 14 shapes from 300 x 256 x 256 to 8192 x 4096 x 4096, every tile and
+// 1 to 16 splits): a compute unit works a 64- / 128- / 256-row tile's 128 bytes of k off in 455 / 1214 / 3825 cycles (fp32: 1367 / 5500) where blocks share it, in no
+// less than 624 / 1170 / 2930 (2100 / 5500) alone; a block costs 1500 / 3000 / 8000 besides, a launch 8700 / 13500 / 20400 (the larger tiles' first loads and last
+// stores).  A split keeps four tiles of k, and adds its partial results' way through memory (2 KB a cycle) and a launch of 10000.  Within 10 % of the best
+// choice on 37 of the 42 products.
 static LinPick lin_pick(int M, int N, int K, int es) {
-  const int nk = (int)(((int64_t)K * es + 127) / 128);
-  for (int tile : {256, 128, 64}) {
-    const int64_t tiles = (int64_t)((M + tile - 1) / tile) * ((N + tile - 1) / tile);
-    int64_t s = 1;
-    if (tiles < 256) {
-      s = (512 + tiles - 1) / tiles;
-      if (s > nk / 4) s = nk / 4;
-      if (s > 16) s = 16;
-      if (s < 1) s = 1;
-    }
-    if (tile == 256 && s > 1) continue;    // (partial results of a split cost more than the larger tile saves)
-    if (tiles * s >= 192 || tile == 64) {
-      const int per = (int)((nk + s - 1) / s);
-      return {tile, (nk + per - 1) / per, per};
+  static const struct { int tile; double shared[2], alone[2], block, launch; } kind[3] = {
+      {64, {455, 1367}, {624, 2100}, 1500, 8700}, {128, {1214, 5500}, {1170, 5500}, 3000, 13500}, {256, {3825, 0}, {2930, 0}, 8000, 20400}};
+  const int nk = (int)(((int64_t)K * es + 127) / 128), wide = es == 4;
+  LinPick best{64, 1, nk};
+  double least = 0;
+  for (const auto& q : kind) {
+    if (q.tile == 256 && wide) break;                                          // (fp32: 3 times the 64-row tiles' time)
+    const int64_t tiles = (int64_t)((M + q.tile - 1) / q.tile) * ((N + q.tile - 1) / q.tile);
+    for (int s = 1; s <= 16 && (s == 1 || (q.tile < 256 && nk / s >= 4)); ++s) {
+      const int per = (nk + s - 1) / s;
+      if ((nk + per - 1) / per != s) continue;                                 // (the same as a smaller split)
+      const double busy = (double)((tiles * s + 255) / 256);
+      const double work = per * (busy * q.shared[wide] > q.alone[wide] ? busy * q.shared[wide] : q.alone[wide]);
+      const double cost = work + busy * q.block + q.launch + (s > 1 ? 10000 + (double)(s + 1) * M * N * 4 / 2000 : 0);
+      if (least == 0 || cost < least) {
+        least = cost;
+        best = {q.tile, s, per};
+      }
     }
   }
-  return {64, 1, nk};
+  return best;
 }
 
 static int64_t lin_round(int64_t bytes) { return (bytes + 255) / 256 * 256; }
 static int lin_es(int dtype) { return dtype == MOY_F32 ? 4 : 2; }
-// rows of n elements that the kernels can take as they are
-static bool lin_direct(const void* p, int64_t ld, int n, int es) { return aligned16(p) && ld * es % 16 == 0 && (int64_t)n * es % 16 == 0; }
+// rows of n elements that the tiled kernel can take as they are: whole dwords
+static bool lin_direct(const void* p, int64_t ld, int n, int es) {
+  return reinterpret_cast<uintptr_t>(p) % 4 == 0 && ld * es % 4 == 0 && (int64_t)n * es % 4 == 0;
+}
+static int64_t lin_span(int64_t rows, int64_t ld, int64_t n, int es) { return ((rows - 1) * ld + n) * es; }
 static int64_t lin_pitch(int n, int es) { return ((int64_t)n * es + 15) / 16 * 16 / es; }
 
 static bool lin_few(int M) { return M <= 32; }
@@ -454,17 +629,20 @@ static int lin_gemm(LinParams p, float* part, hipStream_t st) {
   p.vec = p.N % 4 == 0 && p.ldy % 4 == 0 && reinterpret_cast<uintptr_t>(p.y) % (4 * sizeof(T)) == 0 &&
           (!p.z || (p.ldz % 4 == 0 && reinterpret_cast<uintptr_t>(p.z) % (4 * sizeof(T)) == 0)) &&
           (!p.r || (p.ldr % 4 == 0 && reinterpret_cast<uintptr_t>(p.r) % (4 * sizeof(T)) == 0));
+  constexpr int VEC = 16 / (int)sizeof(T);
+  p.clamp = (ACOL ? p.M : p.K) % VEC != 0 || (BCOL ? p.N : p.K) % VEC != 0;
   const dim3 grid((unsigned)((int64_t)p.tiles_m * p.tiles_n * k.splits));
-#define MOY_LIN(WM, WN, MI, NI)                                                                                                     \
+#define MOY_LIN(WM, WN, MI, NI, ST)                                                                                                     \
   {                                                                                                                                 \
-    auto kern = lin_gemm_kernel<T, ACOL, BCOL, WM, WN, MI, NI>;                                                                     \
+    auto kern = lin_gemm_kernel<T, ACOL, BCOL, WM, WN, MI, NI, ST>;                                                                     \
     static const bool ready = hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024) == hipSuccess; \
     if (!ready) return MOY_ELAUNCH;                                                                                                 \
-    hipLaunchKernelGGL(kern, grid, dim3(WM * WN * 64), 2 * 128 * (WM * MI * 16 + WN * NI * 16), st, p);                                \
+    hipLaunchKernelGGL(kern, grid, dim3(WM * WN * 64), ST * 128 * (WM * MI * 16 + WN * NI * 16), st, p);                               \
   }
-  if (k.tile == 256) MOY_LIN(2, 4, 8, 4)
-  else if (k.tile == 128) MOY_LIN(2, 2, 4, 4)
-  else MOY_LIN(2, 2, 2, 2)
+  if (sizeof(T) == 2 && k.tile == 256) {
+    if constexpr (sizeof(T) == 2) MOY_LIN(2, 4, 8, 4, 2)
+  } else if (k.tile == 128) MOY_LIN(2, 2, 4, 4, 2)
+  else MOY_LIN(2, 2, 2, 2, 3)
 #undef MOY_LIN
   const int rc = launch_status();
   if (rc != MOY_OK || k.splits == 1) return rc;
@@ -494,6 +672,7 @@ static int lin_check(const moy_linear_args* a, bool bwd) {
   if ((int64_t)((a->M + 63) / 64) * ((a->N + 63) / 64) * 16 > 0x7fffffffLL || (int64_t)((a->M + 63) / 64) * ((a->K + 63) / 64) * 16 > 0x7fffffffLL) return MOY_ENOSYS;
   if ((int64_t)a->M * (a->N > a->K ? a->N : a->K) / 4 / 256 > 0x3fffffffLL) return MOY_ENOSYS;
   if (!bwd) {
+    if (a->ldy * lin_es(d) > (1 << 22) || a->ldr * lin_es(d) > (1 << 22)) return MOY_ENOSYS;
     if (!a->y || !aligned_as(a->y, d) || (a->M > 1 && a->ldy < a->N) || !aligned_as(a->b, a->b_dtype)) return MOY_EINVAL;
     if (!aligned_as(a->r, d) || (a->r && a->M > 1 && a->ldr < 0) || !aligned_as(a->z, d)) return MOY_EINVAL;
   } else {
@@ -514,8 +693,9 @@ struct LinPlan {
 static LinPlan lin_plan(const moy_linear_args* a, bool bwd) {
   const int es = lin_es(a->dtype);
   LinPlan p{};
-  p.pad_x = (!bwd || a->dw) && !lin_direct(a->x, a->ldx, a->K, es);
-  p.pad_w = (!bwd || a->dx) && !lin_direct(a->w, a->ldw, a->K, es);
+  const bool few = !bwd && lin_few(a->M);                                       // (takes any rows)
+  p.pad_x = !few && (!bwd || a->dw) && !lin_direct(a->x, a->ldx, a->K, es);
+  p.pad_w = !few && (!bwd || a->dx) && !lin_direct(a->w, a->ldw, a->K, es);
   int64_t at = 0;
   p.x = at;
   if (p.pad_x) at += lin_round(a->M * lin_pitch(a->K, es) * es);
@@ -555,9 +735,9 @@ static int lin_fwd(const moy_linear_args* a, const LinPlan& plan, hipStream_t st
   p.lda = plan.pad_x ? pitch : a->ldx;
   p.b = plan.pad_w ? ws + plan.w : a->w;
   p.ldb = plan.pad_w ? pitch : a->ldw;
-  p.M = a->M; p.N = a->N;
-  p.K = (int)pitch;                        // both rows hold zeros behind K up to a whole 16-byte piece (or K is one already)
-  if (!plan.pad_x || !plan.pad_w) p.K = a->K;
+  p.a_bytes = lin_span(a->M, p.lda, plan.pad_x ? pitch : a->K, sizeof(T));
+  p.b_bytes = lin_span(a->N, p.ldb, plan.pad_w ? pitch : a->K, sizeof(T));
+  p.M = a->M; p.N = a->N; p.K = a->K;
   p.bias = a->b; p.bias_dtype = a->b_dtype; p.act = a->act;
   p.r = a->r; p.ldr = a->ldr; p.y = a->y; p.ldy = a->ldy; p.z = a->z; p.ldz = a->N;
   if (lin_few(a->M)) {
@@ -602,6 +782,8 @@ static int lin_bwd(const moy_linear_args* a, const LinPlan& plan, hipStream_t st
     p.a = dz; p.lda = ldz;
     p.b = plan.pad_w ? ws + plan.w : a->w;
     p.ldb = plan.pad_w ? kp : a->ldw;
+    p.a_bytes = lin_span(a->M, ldz, plan.make_dz ? np : a->N, ES);
+    p.b_bytes = lin_span(a->N, p.ldb, plan.pad_w ? kp : a->K, ES);
     p.M = a->M; p.N = a->K; p.K = a->N;
     p.y = a->dx; p.ldy = a->K;
     if ((rc = lin_gemm<T, false, true>(p, part, st)) != MOY_OK) return rc;
@@ -611,6 +793,8 @@ static int lin_bwd(const moy_linear_args* a, const LinPlan& plan, hipStream_t st
     p.a = dz; p.lda = ldz;
     p.b = plan.pad_x ? ws + plan.x : a->x;
     p.ldb = plan.pad_x ? kp : a->ldx;
+    p.a_bytes = lin_span(a->M, ldz, plan.make_dz ? np : a->N, ES);
+    p.b_bytes = lin_span(a->M, p.ldb, plan.pad_x ? kp : a->K, ES);
     p.M = a->N; p.N = a->K; p.K = a->M;
     p.y = a->dw; p.ldy = a->K;
     if ((rc = lin_gemm<T, true, true>(p, part, st)) != MOY_OK) return rc;

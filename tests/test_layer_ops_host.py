@@ -148,9 +148,10 @@ def test_linear_refuses_by_direction_and_size():
     for kw in (dict(dy=None), dict(z=None), dict(dx=None, dw=None, db=None), dict(dw=FAKE + 1), dict(ws=None), dict(ws_len=1), dict(ws=FAKE + 8)):
         assert _lin(True, **kw)[0] == _lib.EINVAL, kw
     assert _lin(K=1 << 22, ldx=1 << 22, ldw=1 << 22)[0] == _lib.ENOSYS and _lin(ldx=1 << 22)[0] == _lib.ENOSYS
-    # workspaces: none where the rows are whole 16-byte steps and the product fills the chip, padded copies otherwise
-    assert _lin(M=16, N=256, ldy=256)[1] == 0
-    assert _lin(M=16, K=100, ldx=100, ldw=100, N=256, ldy=256)[1] == -(-16 * 104 * 2 // 256) * 256 + 256 * 104 * 2
+    # workspaces: none where the rows are whole dwords and the product fills the chip, padded copies of odd 16-bit rows
+    assert _lin(M=16, N=256, ldy=256)[1] == 0 and _lin(M=16, K=101, ldx=101, ldw=101)[1] == 0
+    assert _lin(M=40, K=102, ldx=102, ldw=102)[1] == 0 and _lin(M=40, K=101, ldx=101, ldw=101, dtype=_lib.F32)[1] == 0
+    assert _lin(M=40, K=101, ldx=101, ldw=101, N=256, ldy=256)[1] == -(-40 * 104 * 2 // 256) * 256 + 256 * 104 * 2
 
 
 def test_linear_args_layout_matches_header():
