@@ -239,12 +239,9 @@ __device__ __forceinline__ uint32_t mask4(const uint8_t* m, int j, int lk) {
   return w;
 }
 
+// keys (backward of dK, dV: queries) of an LDS tile
 template <typename T, int DP>
-struct AttnGeom {
-  static constexpr int KP = DP / 32, DT16 = DP / 16;
-  static constexpr int NQ = sizeof(T) == 2 && DP <= 64 ? 2 : 1;       // 16-query tiles of a wave
-  static constexpr int BK = sizeof(T) * DP <= 128 ? 64 : 32;          // keys of an LDS tile
-};
+constexpr int attn_bk() { return sizeof(T) * DP <= 128 ? 64 : 32; }
 
 // ------------------------------------------------------------------------------------------------------------------------------ forward
 template <typename T, int DP, int NQ, int BK>
@@ -587,12 +584,10 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnParams p) {
 }
 
 // ----------------------------------------------------------------------------------------------------------------------------- backward
-// an LDS address that only this lane touches: the order of its additions is the program's
-__device__ __forceinline__ void lane_add(float* p, float v) { __hip_atomic_fetch_add(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT); }
-
 // dQ, delta and the sums of dS by bucket.  As the forward: a lane owns a query's column, K and V tiles stream through LDS; dQ^T += K^T dS^T.
-// The sums by bucket: each lane adds into its own column of a [bucket][lane] table of its wave in LDS (no two lanes share an address, so the order of additions
-// is the program's), tiles wholly beyond `far` add into two registers instead.
+// The sums by bucket go by distance first, since a distance is a diagonal of dS: 16 queries by 32 keys of dS are laid into the wave's corner of LDS with zeros around
+// them, 47 lanes add a diagonal's 16 entries each and keep it in a table by distance (no two lanes share an entry, so results do not depend on any order); tiles
+// wholly beyond `far` add into two registers instead.  (One LDS addition for each element by bucket took 66 us of 104 on 16 x 300 queries, 8 heads of 32; this takes 10.)
 template <typename T, int DP, int NQ, int BK>
 __global__ __launch_bounds__(256, 2) void attn_dq_kernel(const AttnParams p) {
   constexpr int KP = DP / 32, DT16 = DP / 16, BQ = 64 * NQ;
@@ -601,9 +596,10 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(const AttnParams p) {
   T* kt_ = reinterpret_cast<T*>(smem);
   T* vt_ = reinterpret_cast<T*>(smem + 2 * TL::BYTES);
   float* bias = reinterpret_cast<float*>(smem + 4 * TL::BYTES);
-  const int entries = p.table ? 2 * p.far + 9 : 0;
-  uint32_t* place = reinterpret_cast<uint32_t*>(bias + entries);               // bucket * 64 by distance; RUN: the next three distances share it
-  float* hist = reinterpret_cast<float*>(place + (p.part ? entries : 0));      // [wave][bucket][lane]
+  constexpr int DROW = 68, DIAG = 16 * DROW;                                   // the wave's corner: 16 zeros, 32 keys, 16 zeros and 4 to spread the banks
+  const int entries = p.table ? (2 * p.far + 12) / 4 * 4 : 0, ends = 2 * p.far + 1;   // (whole 16 bytes)
+  float* diag = bias + entries;                                                // [wave][16][DROW]
+  float* by = diag + 4 * DIAG;                                                 // [wave][2 far + 1]: sums by distance
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
   const int id = xcd_order(blockIdx.x, gridDim.x);
   int bh, qt;
@@ -656,24 +652,13 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(const AttnParams p) {
   for (int n = 0; n < NQ; ++n)
 #pragma unroll
     for (int d = 0; d < DT16; ++d) dq[d][n] = f32x4{0.f, 0.f, 0.f, 0.f};
-  float* mine = hist + wave * p.nb * 64 + lane;
-  constexpr uint32_t RUN = 0x80000000u;
-  float before = 0.f, after = 0.f, run[NQ];                                    // run: the sum of the lane's current bucket at[]
-  uint32_t at_[NQ];
+  float* corner = diag + wave * DIAG;
+  float* mine = by + wave * ends;
+  float before = 0.f, after = 0.f;
   if (p.table) load_bias<T>(p, h, bias, 256);
   if (p.part) {
-    for (int e = tid; e < entries; e += 256) {
-      uint32_t k[4];
-#pragma unroll
-      for (int x = 0; x < 4; ++x) k[x] = (uint32_t)min((int)p.lut[min(max(e + x - 4, 0), 2 * p.far)], p.nb - 1) * 64;
-      place[e] = k[0] | (k[0] == k[1] && k[0] == k[2] && k[0] == k[3] ? RUN : 0u);
-    }
-    for (int k = 0; k < p.nb; ++k) mine[k * 64] = 0.f;
-  }
-#pragma unroll
-  for (int n = 0; n < NQ; ++n) {
-    run[n] = 0.f;
-    at_[n] = RUN;                                                              // (bucket 0)
+    for (int e = lane; e < DIAG; e += 64) corner[e] = 0.f;
+    for (int e = lane; e < ends; e += 64) mine[e] = 0.f;
   }
   if (nt > 0) {
     kr.store(kt_, tid);
@@ -732,28 +717,23 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(const AttnParams p) {
             s[kt][n][e] = d;
           }
           if (p.part) {
-            const float four = (s[kt][n].x + s[kt][n].y) + (s[kt][n].z + s[kt][n].w);
-            sum += four;
-            if (!far) {
-              // a lane's keys follow one another, so its buckets come in runs: a register holds the current one's sum, and LDS is touched where it changes
-              const uint32_t k = place[at];
-              if (!__any(k != at_[n])) {
-                run[n] += four;
-              } else if (k == at_[n]) {
-                run[n] += four;
-              } else if (k & RUN) {
-                lane_add(mine + (at_[n] & ~RUN), run[n]);
-                at_[n] = k;
-                run[n] = four;
-              } else {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) lane_add(mine + (place[at + e] & ~RUN), s[kt][n][e]);
-              }
-            }
+            if (far) sum += (s[kt][n].x + s[kt][n].y) + (s[kt][n].z + s[kt][n].w);
+            else *reinterpret_cast<f32x4*>(corner + c * DROW + 16 + kt * 16 + 4 * g) = s[kt][n];
           }
         }
         if (far < 0) before += sum;
         if (far > 0) after += sum;
+        if (p.part && !far) {
+          __builtin_amdgcn_wave_barrier();
+          float v = 0.f;
+#pragma unroll
+          for (int x = 0; x < 16; ++x) v += lane < 48 ? corner[x * (DROW + 1) + lane] : 0.f;   // diagonal key - query = lane - 16
+          const int dist = j0 + kc * 32 - (q0 + n * 16 + sp.start) + lane - 16;
+          if (dist <= -p.far) before += v;
+          else if (dist >= p.far) after += v;
+          else if (lane < 48) mine[dist + p.far] += v;
+          __builtin_amdgcn_wave_barrier();
+        }
         df[n] = frag_of<T>(s[0][n], s[1][n]);
       }
 #pragma unroll
@@ -781,16 +761,24 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(const AttnParams p) {
     }
   }
   if (p.part) {
-#pragma unroll
-    for (int n = 0; n < NQ; ++n) lane_add(mine + (at_[n] & ~RUN), run[n]);
-    lane_add(mine + (place[0] & ~RUN), before);
-    lane_add(mine + (place[entries - 1] & ~RUN), after);
+    before = wave_sum(before);
+    after = wave_sum(after);
+    if (lane == 0) {
+      mine[0] = before;
+      mine[ends - 1] = after;
+    }
+    __syncthreads();
+    int* place = reinterpret_cast<int*>(diag);                                 // (the corners are free now)
+    for (int e = tid; e < ends; e += 256) {
+      by[e] = ((by[e] + by[ends + e]) + by[2 * ends + e]) + by[3 * ends + e];
+      place[e] = min((int)p.lut[e], p.nb - 1);
+    }
     __syncthreads();
     float* out = p.part + ((int64_t)h * p.B * p.tiles + (int64_t)b * p.tiles + qt) * p.nb;
-    for (int k = wave; k < p.nb; k += 4) {                                     // a wave adds a bucket's 4 x 64 lanes
+    for (int k = wave; k < p.nb; k += 4) {                                     // a wave adds the distances of a bucket
       float v = 0.f;
-#pragma unroll
-      for (int w = 0; w < 4; ++w) v += hist[(w * p.nb + k) * 64 + lane];
+#pragma unroll 4
+      for (int e = lane; e < ends; e += 64) v += place[e] == k ? by[e] : 0.f;
       v = wave_sum(v);
       if (lane == 0) out[k] = v;
     }
@@ -1040,21 +1028,16 @@ static int attn_lds_opt_in(const void* kern) {
   return hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024) == hipSuccess ? MOY_OK : MOY_ELAUNCH;
 }
 
-static size_t attn_bias_bytes(const moy_attention_args* a) { return a->table ? (2 * (size_t)a->max_distance + 9) * 4 : 0; }
+static size_t attn_bias_bytes(const moy_attention_args* a) { return a->table ? (2 * (size_t)a->max_distance + 12) / 4 * 16 : 0; }
 
-template <typename T, int DP>
-static int attn_fwd(const moy_attention_args* a, AttnParams p, hipStream_t st) {
-  using G = AttnGeom<T, DP>;
-  if (attn_uses_split(a)) {
-    attn_splits(a, &p.tiles, &p.splits, &p.split_keys);
-    p.part = a->ws;
-    hipLaunchKernelGGL((attn_split_kernel<T, DP>), dim3((unsigned)((int64_t)a->B * a->Hk * p.tiles * p.splits)), dim3(256), 0, st, p);
-    const int rc = launch_status();
-    if (rc != MOY_OK || p.splits == 1) return rc;
-    hipLaunchKernelGGL((attn_join_kernel<T>), dim3((unsigned)(((int64_t)a->B * a->H * a->Lq + 3) / 4)), dim3(256), 0, st, p);
-    return launch_status();
-  }
-  constexpr int NQ = G::NQ, BK = G::BK;
+// 16-bit heads of 40 to 64: 32 queries (keys) to a wave where that leaves two blocks to a compute unit (8 x 1024 x 8 heads of 64: forward 43 us against 48, dQ
+// 88 against 102, dK and dV 61 against 75; 2 x 1024 x 16, half the blocks: 33.5 against 28, 68 against 54, 54 against 41), 16 otherwise; heads up to 32 have
+// the registers for twice the waves and are faster with 16 at any size (64 x 300 x 8: 33.9 against 31.4, 50.7 against 45.1).
+static bool attn_wide(const moy_attention_args* a, int heads, int rows) { return (int64_t)a->B * heads * ((rows + 127) / 128) >= 512; }
+
+template <typename T, int DP, int NQ>
+static int attn_fwd_tiles(const moy_attention_args* a, AttnParams p, hipStream_t st) {
+  constexpr int BK = attn_bk<T, DP>();
   auto kern = attn_fwd_kernel<T, DP, NQ, BK>;
   static const int ready = attn_lds_opt_in(reinterpret_cast<const void*>(kern));
   if (ready != MOY_OK) return ready;
@@ -1065,44 +1048,69 @@ static int attn_fwd(const moy_attention_args* a, AttnParams p, hipStream_t st) {
 }
 
 template <typename T, int DP>
-struct AttnBwdGeom {
-  static constexpr int NQ = AttnGeom<T, DP>::NQ, BK = AttnGeom<T, DP>::BK;
-  static constexpr int NK = sizeof(T) == 2 && DP <= 64 ? 2 : 1, BQ = sizeof(T) * DP <= 128 ? 64 : 32;
-};
+static int attn_fwd(const moy_attention_args* a, AttnParams p, hipStream_t st) {
+  if (attn_uses_split(a)) {
+    attn_splits(a, &p.tiles, &p.splits, &p.split_keys);
+    p.part = a->ws;
+    hipLaunchKernelGGL((attn_split_kernel<T, DP>), dim3((unsigned)((int64_t)a->B * a->Hk * p.tiles * p.splits)), dim3(256), 0, st, p);
+    const int rc = launch_status();
+    if (rc != MOY_OK || p.splits == 1) return rc;
+    hipLaunchKernelGGL((attn_join_kernel<T>), dim3((unsigned)(((int64_t)a->B * a->H * a->Lq + 3) / 4)), dim3(256), 0, st, p);
+    return launch_status();
+  }
+  if constexpr (sizeof(T) == 2 && DP == 64) {
+    if (attn_wide(a, a->H, a->Lq)) return attn_fwd_tiles<T, DP, 2>(a, p, st);
+  }
+  return attn_fwd_tiles<T, DP, 1>(a, p, st);
+}
+
+template <typename T, int DP, int NQ>
+static int attn_dq(const moy_attention_args* a, AttnParams p, hipStream_t st) {
+  constexpr int BK = attn_bk<T, DP>();
+  auto kern = attn_dq_kernel<T, DP, NQ, BK>;
+  static const int ready = attn_lds_opt_in(reinterpret_cast<const void*>(kern));
+  if (ready != MOY_OK) return ready;
+  const size_t bias = attn_bias_bytes(a), lds = 4 * Tile<T, DP, BK, 256>::BYTES + bias + (p.part ? 4 * 4 * (16 * 68 + 2 * (size_t)a->max_distance + 1) : 0);
+  p.tiles = (a->Lq + 64 * NQ - 1) / (64 * NQ);
+  hipLaunchKernelGGL(kern, dim3((unsigned)(a->B * a->H * p.tiles)), dim3(256), lds, st, p);
+  return launch_status();
+}
+
+template <typename T, int DP, int NK>
+static int attn_dkv(const moy_attention_args* a, AttnParams p, hipStream_t st) {
+  constexpr int BQ = attn_bk<T, DP>();
+  auto kern = attn_dkv_kernel<T, DP, NK, BQ>;
+  static const int ready = attn_lds_opt_in(reinterpret_cast<const void*>(kern));
+  if (ready != MOY_OK) return ready;
+  const size_t lds = 4 * Tile<T, DP, BQ, 256>::BYTES + 16 * BQ + attn_bias_bytes(a);
+  p.tiles = (a->Lk + 64 * NK - 1) / (64 * NK);
+  hipLaunchKernelGGL(kern, dim3((unsigned)(a->B * a->Hk * p.tiles)), dim3(256), lds, st, p);
+  return launch_status();
+}
 
 static int attn_dq_tiles(const moy_attention_args* a) {
-  const int rows = a->dtype != MOY_F32 && a->D <= 64 ? 128 : 64;
+  const int rows = a->dtype != MOY_F32 && a->D > 32 && a->D <= 64 && attn_wide(a, a->H, a->Lq) ? 128 : 64;
   return (a->Lq + rows - 1) / rows;
 }
 
 template <typename T, int DP>
 static int attn_bwd(const moy_attention_args* a, AttnParams p, hipStream_t st) {
-  using G = AttnBwdGeom<T, DP>;
-  const size_t bias = attn_bias_bytes(a);
-  {
-    auto kern = attn_dq_kernel<T, DP, G::NQ, G::BK>;
-    static const int ready = attn_lds_opt_in(reinterpret_cast<const void*>(kern));
-    if (ready != MOY_OK) return ready;
-    p.tiles = attn_dq_tiles(a);
-    const size_t lds = 4 * Tile<T, DP, G::BK, 256>::BYTES + bias + (p.part ? bias + 4 * 64 * 4 * (size_t)a->num_buckets : 0);
-    hipLaunchKernelGGL(kern, dim3((unsigned)(a->B * a->H * p.tiles)), dim3(256), lds, st, p);
-    const int rc = launch_status();
-    if (rc != MOY_OK) return rc;
+  int rc = MOY_ENOSYS;
+  if constexpr (sizeof(T) == 2 && DP == 64) {
+    if (attn_wide(a, a->H, a->Lq)) rc = attn_dq<T, DP, 2>(a, p, st);
   }
+  if (rc == MOY_ENOSYS) rc = attn_dq<T, DP, 1>(a, p, st);
+  if (rc != MOY_OK) return rc;
   if (a->dtable) {
-    hipLaunchKernelGGL((attn_dtable_kernel<T>), dim3((a->num_buckets * a->H + 3) / 4), dim3(256), 0, st, p.part, a->num_buckets, a->H, a->B * p.tiles,
-                       static_cast<T*>(a->dtable));
-    const int rc = launch_status();
-    if (rc != MOY_OK) return rc;
+    hipLaunchKernelGGL((attn_dtable_kernel<T>), dim3((a->num_buckets * a->H + 3) / 4), dim3(256), 0, st, p.part, a->num_buckets, a->H,
+                       a->B * attn_dq_tiles(a), static_cast<T*>(a->dtable));
+    if ((rc = launch_status()) != MOY_OK) return rc;
   }
   if (!a->dk && !a->dv) return MOY_OK;
-  auto kern = attn_dkv_kernel<T, DP, G::NK, G::BQ>;
-  static const int ready = attn_lds_opt_in(reinterpret_cast<const void*>(kern));
-  if (ready != MOY_OK) return ready;
-  p.tiles = (a->Lk + 64 * G::NK - 1) / (64 * G::NK);
-  const size_t lds = 4 * Tile<T, DP, G::BQ, 256>::BYTES + 16 * G::BQ + bias;
-  hipLaunchKernelGGL(kern, dim3((unsigned)(a->B * a->Hk * p.tiles)), dim3(256), lds, st, p);
-  return launch_status();
+  if constexpr (sizeof(T) == 2 && DP == 64) {
+    if (attn_wide(a, a->Hk, a->Lk)) return attn_dkv<T, DP, 2>(a, p, st);
+  }
+  return attn_dkv<T, DP, 1>(a, p, st);
 }
 
 #define MOY_ATTN_DISPATCH(FN, ...)                                                                                            \
