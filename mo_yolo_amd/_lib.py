@@ -221,3 +221,23 @@ def check(rc: int, what: str = ""):
     if rc != 0:
         msg = lib().moy_strerror(rc).decode()
         raise MoyoloError(f"{what or 'libmoyolo'} failed: {msg} (code {rc})")
+
+
+# what csrc/host.cpp calls
+_HOST_ENTRIES = ("moy_strerror", "moy_layer_norm", "moy_layer_norm_bwd", "moy_layer_norm_bwd_ws", "moy_linear", "moy_linear_ws", "moy_linear_bwd",
+                 "moy_linear_bwd_ws", "moy_attention", "moy_attention_ws", "moy_attention_bwd", "moy_attention_bwd_ws")
+_host_module = None
+
+
+def host():
+    """The host side of the transformer-layer operators (_host.so, csrc/host.cpp), bound to the library that lib() loads.  Raises if it has not been built."""
+    global _host_module
+    if _host_module is None:
+        l = lib()
+        try:
+            from . import _host
+        except ImportError as e:
+            raise MoyoloError(f"{os.path.join(HERE, '_host.so')} cannot be loaded ({e}): build it with `python -m mo_yolo_amd.build`") from e
+        _host.bind({n: C.cast(getattr(l, n), C.c_void_p).value for n in _HOST_ENTRIES}, MoyoloError)
+        _host_module = _host
+    return _host_module

@@ -4,6 +4,8 @@
     python -m mo_yolo_amd.build --diag     # libmoyolo_diag.so  -- the LAB: same sources with -DMOY_DIAG=1 (A/B knobs `MOY_*`, stamped /
                                            #                       ablated template instances); selected with MOYOLO_LIB=<path>
     python -m mo_yolo_amd.build --all [--force]
+                                           # each also builds _host.so   -- the host side of the transformer-layer operators (csrc/host.cpp: a torch
+                                           #                              extension, g++; it calls whichever of the two libraries is loaded)
 
 Every translation unit is compiled with -Rpass-analysis=kernel-resource-usage and the remarks are checked: a kernel of an
 LDS-DMA ring family (`gemm_wreg_kernel`, `conv_ws_kernel`, `conv_s2_kernel`, `gemm_dma_kernel`, ...) that needs scratch FAILS the build --
@@ -37,6 +39,28 @@ def _hipcc():
         if c and os.path.exists(c):
             return c
     raise RuntimeError("hipcc not found: libmoyolo.so cannot be built (ROCm toolchain required)")
+
+
+HOST_SRC = os.path.join(CSRC, "host.cpp")
+HOST = os.path.join(HERE, "_host.so")
+
+
+def _host_stale():
+    deps = [HOST_SRC, os.path.join(os.path.dirname(HERE), "include", "moyolo.h")]
+    return not os.path.exists(HOST) or any(os.path.getmtime(d) > os.path.getmtime(HOST) for d in deps)
+
+
+def _host_command():
+    import sysconfig
+
+    from torch.utils import cpp_extension as ext
+    cxx = shutil.which("g++") or shutil.which("c++")
+    if not cxx:
+        raise RuntimeError("g++ not found: _host.so cannot be built")
+    inc = [*ext.include_paths(), os.path.join(os.path.dirname(os.path.dirname(_hipcc())), "include"), "/opt/rocm/include", sysconfig.get_paths()["include"]]
+    return [cxx, "-O2", "-std=c++20", "-fPIC", "-shared", "-Wall", "-D__HIP_PLATFORM_AMD__=1", "-DTORCH_EXTENSION_NAME=_host",
+            *[a for d in inc for a in ("-isystem", d)], HOST_SRC, "-o", HOST + ".tmp", *["-L" + d for d in ext.library_paths()],
+            "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_hip"]
 
 
 def lib_path(diag=False):
@@ -92,6 +116,22 @@ def check_resources(src: str, remarks: str):
 
 def build(force=False, verbose=True, diag=False):
     lib = lib_path(diag)
+    host = None
+    if force or _host_stale():             # beside the kernels: it takes as long as they do
+        cmd = _host_command()
+        if verbose:
+            print(" ".join(cmd), flush=True)
+        host = (cmd, subprocess.Popen(cmd))
+    try:
+        return _build_library(lib, force, verbose, diag)
+    finally:
+        if host:
+            if host[1].wait() != 0:
+                raise subprocess.CalledProcessError(host[1].returncode, host[0])
+            os.replace(HOST + ".tmp", HOST)
+
+
+def _build_library(lib, force, verbose, diag):
     if not force and not needs_build(diag):
         return lib
     hipcc = _hipcc()

@@ -305,103 +305,25 @@ class MSDeformAttnFunction(torch.autograd.Function):
         return gv, None, None, gl, ga, None
 
 
-def _differentiable_once(backward):
-    """once_differentiable, whose guard is needed only where a graph of the backward is asked for (create_graph), and costs as much as a launch."""
-    guarded = torch.autograd.function.once_differentiable(backward)
-
-    def run(ctx, grad):
-        return guarded(ctx, grad) if torch.is_grad_enabled() else backward(ctx, grad)
-    return run
-
-
-def _wants_grad(*ts):
-    if torch.is_grad_enabled():
-        for t in ts:
-            if t is not None and t.requires_grad:
-                return True
-    return False
-
-
-class LayerNormFunction(torch.autograd.Function):
-    """Autograd of ops.layer_norm_forward: gradients for x, weight, bias and the residual (x and the residual share theirs)."""
-
-    @staticmethod
-    def forward(ctx, x, weight, bias, eps, residual):
-        y, stat = ops.layer_norm_forward(x, weight, bias, eps, residual, True)
-        ctx.save_for_backward(x, weight, residual, stat)
-        ctx.types = next((t.dtype for t in (weight, bias) if t is not None), torch.float32)
-        return y
-
-    @staticmethod
-    @_differentiable_once
-    def backward(ctx, dy):
-        x, weight, residual, stat = ctx.saved_tensors
-        nx, nw, nb, _, nr = ctx.needs_input_grad
-        wdt = ctx.types
-        dx, dw, db = ops._norm_backward(dy, x, weight, stat, residual, (nx or nr, nw, nb), ops._CODES[x.dtype], ops._CODES[wdt], wdt)
-        return dx if nx else None, dw, db, None, dx if nr else None
-
-
 def layer_norm(x, weight=None, bias=None, eps=1e-5, residual=None):
-    """Layer norm of x (+ residual) over the last axis (the post-norms of transformer.py:515-652, `norm(tgt + tgt2)`), differentiable; without a
-    gradient to compute, the forward alone.  weight / bias [C] in x's type or float32."""
-    if _wants_grad(x, weight, bias, residual):
-        return LayerNormFunction.apply(x, weight, bias, eps, residual)
-    return ops.layer_norm_forward(x, weight, bias, eps, residual)
-
-
-class LinearFunction(torch.autograd.Function):
-    """Autograd of ops.linear_forward: gradients for x, weight, bias and the residual (the last is dy itself)."""
-
-    @staticmethod
-    def forward(ctx, x, weight, bias, act, residual):
-        y, z = ops.linear_forward(x, weight, bias, act, residual, True)
-        ctx.save_for_backward(x, weight, z)
-        ctx.how = act, torch.float32 if bias is None else bias.dtype
-        return y
-
-    @staticmethod
-    @_differentiable_once
-    def backward(ctx, dy):
-        x, weight, z = ctx.saved_tensors
-        nx, nw, nb, _, nr = ctx.needs_input_grad
-        act, bias_dtype = ctx.how
-        dx, dw, db = ops._linear_backward(dy, x, weight, z, act, (nx, nw, nb), bias_dtype)
-        return dx, dw, db, None, dy if nr else None
+    """Layer norm of x (+ residual) over the last axis (the post-norms of transformer.py:515-652, `norm(tgt + tgt2)`), differentiable in x, weight,
+    bias and residual (once); without a gradient to compute, the forward alone.  Arguments as ops.layer_norm_forward."""
+    ops._norm_check(x, weight, bias, eps, residual)
+    return L.host().layer_norm(x, weight, bias, eps, residual)
 
 
 def linear(x, weight, bias=None, act=L.ACT_NONE, residual=None):
-    """act(x weight^T + bias) + residual, differentiable (arguments as ops.linear_forward); without a gradient to compute, the forward alone."""
-    if _wants_grad(x, weight, bias, residual):
-        return LinearFunction.apply(x, weight, bias, act, residual)
-    return ops.linear_forward(x, weight, bias, act, residual)
-
-
-class BiasedAttentionFunction(torch.autograd.Function):
-    """Autograd of ops.attention_forward: gradients for q, k, v and the bias table."""
-
-    @staticmethod
-    def forward(ctx, q, k, v, table, lut, causal, q_start, k_len, attn_mask, scale):
-        o, lse, rest = ops.attention_forward(q, k, v, table, lut, causal=causal, q_start=q_start, k_len=k_len, attn_mask=attn_mask, scale=scale, stats=True)
-        ctx.save_for_backward(q, k, v, o, lse, rest, table, lut, k_len, attn_mask)
-        ctx.how = causal, q_start, scale
-        return o
-
-    @staticmethod
-    @_differentiable_once
-    def backward(ctx, dout):
-        q, k, v, o, lse, rest, table, lut, k_len, attn_mask = ctx.saved_tensors
-        causal, q_start, scale = ctx.how
-        dq, dk, dv, dtable = ops._attention_backward(dout, q, k, v, o, lse, rest, table, lut, causal, q_start, k_len, attn_mask, scale, ctx.needs_input_grad)
-        return dq, dk, dv, dtable, None, None, None, None, None, None
+    """act(x weight^T + bias) + residual, differentiable in x, weight, bias and residual (once); without a gradient to compute, the forward alone.
+    Arguments as ops.linear_forward."""
+    ops._linear_check(x, weight, bias, act, residual)
+    return L.host().linear(x, weight, bias, act, residual)
 
 
 def biased_attention(q, k, v, table=None, lut=None, *, causal=False, q_start=None, k_len=None, attn_mask=None, scale=None):
-    """Attention with a learned relative position bias by buckets, differentiable in q, k, v and table; arguments as ops.attention_forward.  Without a
-    gradient to compute, the forward alone (a single new token over a long cache among it: the keys are split over the chip)."""
-    if _wants_grad(q, k, v, table):
-        return BiasedAttentionFunction.apply(q, k, v, table, lut, causal, q_start, k_len, attn_mask, scale)
-    return ops.attention_forward(q, k, v, table, lut, causal=causal, q_start=q_start, k_len=k_len, attn_mask=attn_mask, scale=scale)
+    """Attention with a learned relative position bias by buckets, differentiable in q, k, v and table (once); arguments as ops.attention_forward.
+    Without a gradient to compute, the forward alone (a single new token over a long cache among it: the keys are split over the chip)."""
+    ops._attention_check(q, k, v, table, lut, q_start, k_len, attn_mask, scale)
+    return L.host().attention(q, k, v, table, lut, k_len, attn_mask, *ops._attention_how(q, causal, q_start, scale))
 
 
 class MSDeformAttn(nn.Module):

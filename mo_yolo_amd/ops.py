@@ -514,36 +514,8 @@ def sigmoid_f32(x):
 
 
 # ----------------------------------------------------------------------------- operators of a trained transformer layer
-# Their host side is on the path of every training step, much of it in autograd's own thread: checks are made once a call (the backward of a Function repeats
-# none of the forward's), and what a launch needs is read without building objects.
+# Arguments are checked here; layouts, outputs, workspaces, launches and autograd's nodes are csrc/host.cpp.
 _CODES = {torch.float32: L.F32, torch.bfloat16: L.BF16, torch.float16: L.F16}
-_current_device = torch.cuda.current_device
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
-
-
-class _On:
-    """`with _On(tensor) as stream`: the tensor's device as the current one for a launch, on its current stream (raw handle)."""
-
-    __slots__ = ("index", "back")
-
-    def __init__(self, t):
-        self.index = t.device.index
-
-    def __enter__(self):
-        now = _current_device()
-        self.back = None if now == self.index else now
-        if self.back is not None:
-            torch.cuda.set_device(self.index)
-        return _raw_stream(self.index)
-
-    def __exit__(self, *exc):
-        if self.back is not None:
-            torch.cuda.set_device(self.back)
-        return False
-
-
-def _ptr(t):
-    return None if t is None else t.data_ptr()
 
 
 def _one_device(x, *others):
@@ -557,21 +529,14 @@ def _one_device(x, *others):
 
 
 def _type_code(x):
-    code = _CODES.get(x.dtype)
-    return _code(x) if code is None else code          # (raises)
+    if x.dtype not in _CODES:
+        _code(x)                                       # (raises)
 
 
-def _as_rows(t):
-    """[..., C] -> a 2-D view [rows, C] with unit column stride (a copy where the strides allow none)."""
-    if t.dim() != 2:
-        t = t.reshape(t.numel() // t.shape[-1], t.shape[-1])
-    return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
-
-
-def _norm_check(x, weight, bias, residual):
-    """-> (type code of x, of the weights, the weights' type)"""
+def _norm_check(x, weight, bias, eps, residual):
     _one_device(x, weight, bias, residual)
-    code, dt, shape = _type_code(x), x.dtype, x.shape
+    _type_code(x)
+    dt, shape = x.dtype, x.shape
     if not shape or shape[-1] == 0:
         raise ValueError("layer_norm: x must be [..., C] with C > 0")
     if residual is not None and (residual.shape != shape or residual.dtype != dt):
@@ -582,89 +547,30 @@ def _norm_check(x, weight, bias, residual):
             if t.shape != shape[-1:] or (t.dtype != dt and t.dtype != torch.float32) or (wdt is not None and t.dtype != wdt):
                 raise ValueError("layer_norm: weight and bias must be [C], both in x's type or both float32")
             wdt = t.dtype
-    return (code, L.F32, torch.float32) if wdt is None else (code, _CODES[wdt], wdt)
+    if not eps >= 0:
+        raise ValueError("layer_norm: eps must not be negative")
 
 
 def layer_norm_forward(x, weight=None, bias=None, eps=1e-5, residual=None, stats=False):
     """Layer norm of x (+ residual) over the last axis (moy_layer_norm); weight / bias [C] in x's type or float32.  float32 / bfloat16 /
     float16, any leading shape and row stride.  -> y, or with stats (y, stat) as layer_norm_backward takes it (fp32 [2, rows]: mean, 1 / deviation)."""
-    code, wcode, _ = _norm_check(x, weight, bias, residual)
-    if not eps >= 0:
-        raise ValueError("layer_norm: eps must not be negative")
-    x2 = _as_rows(x)
-    r2 = None if residual is None else _as_rows(residual)
-    w, b = None if weight is None else weight.contiguous(), None if bias is None else bias.contiguous()
-    rows, c = x2.shape
-    with _On(x) as stream:
-        y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
-        stat = torch.empty(2, rows, device=x.device, dtype=torch.float32) if stats else None
-        if rows:
-            at = None if stat is None else stat.data_ptr()
-            rc = L.lib().moy_layer_norm(x2.data_ptr(), x2.stride(0), _ptr(r2), 0 if r2 is None else r2.stride(0), _ptr(w), _ptr(b), wcode, rows, c, eps,
-                                        y.data_ptr(), c, at, None if at is None else at + 4 * rows, code, stream)
-            if rc:
-                L.check(rc, "moy_layer_norm")
+    _norm_check(x, weight, bias, eps, residual)
+    y, stat = L.host().layer_norm_forward(x, weight, bias, eps, residual, stats)
     return (y, stat) if stats else y
 
 
-def _norm_backward(dy, x, weight, stat, residual, need, code, wcode, wdt):
-    x2, g2 = _as_rows(x), _as_rows(dy)
-    r2 = None if residual is None else _as_rows(residual)
-    w = None if weight is None else weight.contiguous()
-    rows, c = x2.shape
-    with _On(x) as stream:
-        dev = x.device
-        dx = torch.empty(x.shape, device=dev, dtype=x.dtype) if need[0] else None
-        dw = torch.empty(c, device=dev, dtype=wdt) if need[1] else None
-        db = torch.empty(c, device=dev, dtype=wdt) if need[2] else None
-        if rows == 0:
-            for t in (dw, db):
-                if t is not None:
-                    t.zero_()
-        elif need[0] or need[1] or need[2]:
-            lib, n, ws = L.lib(), 0, None
-            if need[1] or need[2]:
-                n = lib.moy_layer_norm_bwd_ws(rows, c, code)
-                if n < 0:
-                    L.check(n, "moy_layer_norm_bwd_ws")
-                ws = torch.empty(n, device=dev, dtype=torch.float32)
-            at = stat.data_ptr()
-            rc = lib.moy_layer_norm_bwd(g2.data_ptr(), g2.stride(0), x2.data_ptr(), x2.stride(0), _ptr(r2), 0 if r2 is None else r2.stride(0), _ptr(w), wcode,
-                                        at, at + 4 * rows, rows, c, _ptr(dx), c, _ptr(dw), _ptr(db), _ptr(ws), n, code, stream)
-            if rc:
-                L.check(rc, "moy_layer_norm_bwd")
-    return dx, dw, db
-
-
-def layer_norm_backward(dy, x, weight, stat, residual=None, need=(True, True, True), weight_dtype=None):
+def layer_norm_backward(dy, x, weight, stat, residual=None, need=(True, True, True), weight_dtype=torch.float32):
     """Gradients of layer_norm_forward (moy_layer_norm_bwd): (dx, dweight, dbias); dx is the gradient of x and of the residual alike.  need: which of
-    the three are computed (None in the others' place); weight_dtype: the type of dweight / dbias where weight is None (float32)."""
-    code, wcode, wdt = _norm_check(x, weight, None, residual)
+    the three are computed (None in the others' place); weight_dtype: the type of dweight / dbias where weight is None."""
+    _norm_check(x, weight, None, 0.0, residual)
     _one_device(x, dy, stat)
-    if weight is None and weight_dtype is not None:
-        if weight_dtype not in (x.dtype, torch.float32):
-            raise ValueError("layer_norm_backward: weight_dtype is x's type or float32")
-        wcode, wdt = _CODES[weight_dtype], weight_dtype
+    if weight_dtype not in (x.dtype, torch.float32):
+        raise ValueError("layer_norm_backward: weight_dtype is x's type or float32")
     if dy.shape != x.shape or dy.dtype != x.dtype:
         raise ValueError("layer_norm_backward: dy must have x's shape and type")
     if stat.dtype != torch.float32 or tuple(stat.shape) != (2, x.numel() // x.shape[-1]) or not stat.is_contiguous():
         raise ValueError("layer_norm_backward: stat must be layer_norm_forward's")
-    return _norm_backward(dy, x, weight, stat, residual, need, code, wcode, wdt)
-
-
-def _linear_args(x, weight, bias, act, residual):
-    """The launch arguments of tensors that have been checked: (moy_linear_args, tensors to keep until the launch)."""
-    x2, w2, r2 = _as_rows(x), _as_rows(weight), None if residual is None else _as_rows(residual)
-    a = L.LinearArgs()
-    a.x, a.ldx, a.w, a.ldw, a.act, a.dtype = x2.data_ptr(), x2.stride(0), w2.data_ptr(), w2.stride(0), act, _CODES[x.dtype]
-    a.M = x2.shape[0]
-    a.N, a.K = w2.shape
-    if bias is not None:
-        bias = bias.contiguous()
-        a.b, a.b_dtype = bias.data_ptr(), _CODES[bias.dtype]
-    if r2 is not None:
-        a.r, a.ldr = r2.data_ptr(), r2.stride(0)
-    return a, (x2, w2, bias, r2)
+    return L.host().layer_norm_backward(dy, x, weight, stat, residual, *map(bool, need), weight_dtype if weight is None else weight.dtype)
 
 
 def _linear_check(x, weight, bias, act, residual):
@@ -685,53 +591,13 @@ def _linear_check(x, weight, bias, act, residual):
         raise ValueError("linear: more than 2^31 - 1 rows")
 
 
-def _linear_run(a, query, launch, what, dev, stream):
-    n = query(a)
-    if n < 0:
-        L.check(n, what)
-    if n:
-        ws = torch.empty(n, device=dev, dtype=torch.uint8)
-        a.ws, a.ws_len = ws.data_ptr(), n
-    rc = launch(a, stream)
-    if rc:
-        L.check(rc, what)
-
-
 def linear_forward(x, weight, bias=None, act=L.ACT_NONE, residual=None, keep_pre=False):
     """act(x weight^T + bias) + residual (moy_linear): x [..., K], weight [N, K] of one type (float32 / bfloat16 / float16), bias [N] in it or float32,
     residual [..., N]; any sizes, row strides and alignments (rows that are not whole 16-byte steps cost a copy).  -> y, or with keep_pre (y, z):
     z = what act was applied to, as linear_backward takes it (None for ACT_NONE)."""
     _linear_check(x, weight, bias, act, residual)
-    a, keep = _linear_args(x, weight, bias, act, residual)
-    with _On(x) as stream:
-        dev, n = x.device, a.N
-        y = torch.empty((*x.shape[:-1], n), device=dev, dtype=x.dtype)
-        z = torch.empty(a.M, n, device=dev, dtype=x.dtype) if keep_pre and act != L.ACT_NONE else None
-        if a.M:
-            a.y, a.ldy, a.z = y.data_ptr(), n, _ptr(z)
-            lib = L.lib()
-            _linear_run(a, lib.moy_linear_ws, lib.moy_linear, "moy_linear", dev, stream)
+    y, z = L.host().linear_forward(x, weight, bias, act, residual, keep_pre)
     return (y, z) if keep_pre else y
-
-
-def _linear_backward(dy, x, weight, z, act, need, bias_dtype):
-    a, keep = _linear_args(x, weight, None, act, None)
-    a.b_dtype = _CODES[bias_dtype]
-    with _On(x) as stream:
-        dev, dt = x.device, x.dtype
-        dx = torch.empty(x.shape, device=dev, dtype=dt) if need[0] else None
-        dw = torch.empty(weight.shape, device=dev, dtype=dt) if need[1] else None
-        db = torch.empty(a.N, device=dev, dtype=bias_dtype) if need[2] else None
-        if a.M == 0:
-            for t in (dw, db):
-                if t is not None:
-                    t.zero_()
-        elif need[0] or need[1] or need[2]:
-            g = _as_rows(dy)
-            a.dy, a.ldd, a.z, a.dx, a.dw, a.db = g.data_ptr(), g.stride(0), _ptr(z), _ptr(dx), _ptr(dw), _ptr(db)
-            lib = L.lib()
-            _linear_run(a, lib.moy_linear_bwd_ws, lib.moy_linear_bwd, "moy_linear_bwd", dev, stream)
-    return dx, dw, db
 
 
 def linear_backward(dy, x, weight, z=None, act=L.ACT_NONE, need=(True, True, True), bias_dtype=torch.float32):
@@ -746,7 +612,7 @@ def linear_backward(dy, x, weight, z=None, act=L.ACT_NONE, need=(True, True, Tru
         raise ValueError("linear_backward: dy must be [..., N] in x's type")
     if act != L.ACT_NONE and (z is None or tuple(z.shape) != (x.numel() // x.shape[-1], n) or z.dtype != x.dtype or not z.is_contiguous()):
         raise ValueError("linear_backward: z must be linear_forward's")
-    return _linear_backward(dy, x, weight, z, act, need, bias_dtype)
+    return L.host().linear_backward(dy, x, weight, z, act, *map(bool, need), bias_dtype)
 
 
 def relative_buckets(num_buckets, max_distance, bidirectional=True, device="cuda"):
@@ -766,20 +632,6 @@ def relative_buckets(num_buckets, max_distance, bidirectional=True, device="cuda
         side.append(n if n < near else near + t)
     after = [half + b for b in side[1:]] if bidirectional else [0] * max_distance
     return torch.tensor(side[:0:-1] + [0] + after, dtype=torch.uint8).to(device)
-
-
-def _strided(t):
-    """(a view that the attention kernels address: unit stride within a head, 16-byte steps and base; its strides of batch, token and head).  A copy where
-    the strides allow none."""
-    sb, sl, sh, sd = t.stride()
-    step = 16 // t.element_size()
-    n = t.shape
-    if sd != 1 or t.data_ptr() % 16 or (sb % step and n[0] > 1) or (sl % step and n[1] > 1) or (sh % step and n[2] > 1):
-        t = t.contiguous()
-        if t.data_ptr() % 16:
-            t = t.clone()
-        sb, sl, sh, sd = t.stride()
-    return t, 0 if n[0] == 1 else sb, 0 if n[1] == 1 else sl, 0 if n[2] == 1 else sh
 
 
 def _attention_check(q, k, v, table, lut, q_start, k_len, attn_mask, scale):
@@ -815,37 +667,8 @@ def _attention_check(q, k, v, table, lut, q_start, k_len, attn_mask, scale):
         raise ValueError("attention: scale must be finite and not negative")
 
 
-def _attention_args(q, k, v, table, lut, causal, q_start, k_len, attn_mask, scale):
-    """The launch arguments of tensors that have been checked: (moy_attention_args, tensors to keep until the launch)."""
-    a = L.AttentionArgs()
-    q, a.q_sb, a.q_sl, a.q_sh = _strided(q)
-    k, a.k_sb, a.k_sl, a.k_sh = _strided(k)
-    v, a.v_sb, a.v_sl, a.v_sh = _strided(v)
-    a.q, a.k, a.v, a.dtype = q.data_ptr(), k.data_ptr(), v.data_ptr(), _CODES[q.dtype]
-    a.B, a.Lq, a.H, a.D = q.shape
-    a.Lk, a.Hk = k.shape[1:3]
-    a.scale = a.D ** -0.5 if scale is None else scale
-    a.causal = 1 if causal else 0
-    if q_start is None:
-        a.q_from_end = 1
-    else:
-        a.q_start = int(q_start)
-    if table is not None:
-        table, lut = table.contiguous(), lut.contiguous()
-        a.table, a.lut, a.num_buckets, a.max_distance = table.data_ptr(), lut.data_ptr(), table.shape[0], lut.shape[0] // 2
-    if k_len is not None:
-        k_len = k_len.contiguous()
-        a.k_len = k_len.data_ptr()
-    m = attn_mask
-    if m is not None:
-        if m.stride(-1) != 1 and m.shape[-1] > 1:
-            m = m.contiguous()
-        a.mask = m.data_ptr()
-        sizes, strides = m.shape, m.stride()
-        a.m_sq = 0 if sizes[-2] == 1 else strides[-2]
-        if len(sizes) == 4:
-            a.m_sb, a.m_sh = 0 if sizes[0] == 1 else strides[0], 0 if sizes[1] == 1 else strides[1]
-    return a, (q, k, v, table, lut, k_len, m)
+def _attention_how(q, causal, q_start, scale):
+    return bool(causal), q_start is None, 0 if q_start is None else int(q_start), q.shape[3] ** -0.5 if scale is None else float(scale)
 
 
 def attention_forward(q, k, v, table=None, lut=None, *, causal=False, q_start=None, k_len=None, attn_mask=None, scale=None, stats=False):
@@ -858,62 +681,8 @@ def attention_forward(q, k, v, table=None, lut=None, *, causal=False, q_start=No
     neither by query nor by head.  scale: >= 0, D ** -0.5.  A query that sees no key gets zeros.
     -> o [B, Lq, H, D], or with stats (o, lse, rest) as attention_backward takes them (rest: what the rounding of a 16-bit o left out, else None)."""
     _attention_check(q, k, v, table, lut, q_start, k_len, attn_mask, scale)
-    a, keep = _attention_args(q, k, v, table, lut, causal, q_start, k_len, attn_mask, scale)
-    with _On(q) as stream:
-        dev = q.device
-        o = torch.empty(q.shape, device=dev, dtype=q.dtype)
-        lse = rest = None
-        if stats:
-            lse = torch.empty(a.B, a.H, a.Lq, device=dev, dtype=torch.float32)
-            rest = torch.empty(q.shape, device=dev, dtype=q.dtype) if a.dtype != L.F32 else None
-        if o.numel() and a.Lk == 0:
-            for t in (o, rest):
-                if t is not None:
-                    t.zero_()
-            if stats:
-                lse.fill_(float("-inf"))
-        elif o.numel():
-            lib = L.lib()
-            a.o, a.o_rest, a.lse = o.data_ptr(), _ptr(rest), _ptr(lse)
-            n = lib.moy_attention_ws(a)
-            if n < 0:
-                L.check(n, "moy_attention_ws")
-            if n:
-                ws = torch.empty(n, device=dev, dtype=torch.float32)
-                a.ws, a.ws_len = ws.data_ptr(), n
-            rc = lib.moy_attention(a, stream)
-            if rc:
-                L.check(rc, "moy_attention")
+    o, lse, rest = L.host().attention_forward(q, k, v, table, lut, k_len, attn_mask, *_attention_how(q, causal, q_start, scale), stats)
     return (o, lse, rest) if stats else o
-
-
-def _attention_backward(dout, q, k, v, o, lse, rest, table, lut, causal, q_start, k_len, attn_mask, scale, need):
-    with _On(q) as stream:
-        dev, dt = q.device, q.dtype
-        dq = torch.empty(q.shape, device=dev, dtype=dt) if need[0] else None
-        dk = torch.empty(k.shape, device=dev, dtype=dt) if need[1] else None
-        dv = torch.empty(k.shape, device=dev, dtype=dt) if need[2] else None
-        dtable = torch.empty(table.shape, device=dev, dtype=dt) if need[3] and table is not None else None
-        out = (dq, dk, dv, dtable)
-        if q.numel() == 0 or k.numel() == 0:
-            for t in out:
-                if t is not None:
-                    t.zero_()
-        elif any(t is not None for t in out):
-            a, keep = _attention_args(q, k, v, table, lut, causal, q_start, k_len, attn_mask, scale)
-            g, a.g_sb, a.g_sl, a.g_sh = _strided(dout)
-            a.dout, a.o, a.o_rest, a.lse = g.data_ptr(), o.data_ptr(), _ptr(rest), lse.data_ptr()
-            a.dq, a.dk, a.dv, a.dtable = _ptr(dq), _ptr(dk), _ptr(dv), _ptr(dtable)
-            lib = L.lib()
-            n = lib.moy_attention_bwd_ws(a)
-            if n < 0:
-                L.check(n, "moy_attention_bwd_ws")
-            ws = torch.empty(n, device=dev, dtype=torch.float32)
-            a.ws, a.ws_len = ws.data_ptr(), n
-            rc = lib.moy_attention_bwd(a, stream)
-            if rc:
-                L.check(rc, "moy_attention_bwd")
-    return out
 
 
 def attention_backward(dout, q, k, v, o, lse, rest=None, table=None, lut=None, *, causal=False, q_start=None, k_len=None, attn_mask=None, scale=None,
@@ -927,4 +696,4 @@ def attention_backward(dout, q, k, v, o, lse, rest=None, table=None, lut=None, *
             raise ValueError("attention_backward: dout, o and rest must have q's shape and type, o and rest as the forward gave them")
     if lse.dtype != torch.float32 or tuple(lse.shape) != (q.shape[0], q.shape[2], q.shape[1]) or not lse.is_contiguous():
         raise ValueError("attention_backward: lse must be the forward's")
-    return _attention_backward(dout, q, k, v, o, lse, rest, table, lut, causal, q_start, k_len, attn_mask, scale, need)
+    return L.host().attention_backward(dout, q, k, v, o, lse, rest, table, lut, k_len, attn_mask, *_attention_how(q, causal, q_start, scale), *map(bool, need))

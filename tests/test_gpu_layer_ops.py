@@ -192,6 +192,34 @@ def test_layer_norm_other_stream_and_graph():
         assert all(torch.equal(u, v) for u, v in zip(out, want)), k
 
 
+def test_gradients_that_are_not_asked_for_and_asked_for_twice():
+    gen = gen_of(40)
+    x, w, b, r, dy = rand(gen, 60, 64), rand(gen, 64), rand(gen, 64), rand(gen, 60, 64), rand(gen, 60, 64)
+    W, B, R = rand(gen, 48, 64), rand(gen, 48), rand(gen, 60, 48)
+    q, t, lut = rand(gen, 2, 30, 2, 32), rand(gen, 8, 2), ops.relative_buckets(8, 8)
+    calls = [(lambda *a: modules.layer_norm(a[0], a[1], a[2], residual=a[3]), (x, w, b, r)), (lambda *a: modules.linear(a[0], a[1], a[2], L.ACT_SILU, a[3]), (x, W, B, R)),
+             (lambda *a: modules.biased_attention(a[0], a[1], a[2], a[3], lut, q_start=0), (q, q.clone(), q.clone(), t)),
+             (lambda *a: modules.linear(a[0], a[1], None, L.ACT_NONE, a[2]), (x, W, R)), (lambda *a: modules.layer_norm(a[0], None, a[1]), (x, b))]
+    for f, args in calls:
+        every = [a.clone().requires_grad_(True) for a in args]
+        y = f(*every)
+        g = rand(gen, *y.shape)
+        want = torch.autograd.grad(y, every, g)
+        for only in range(len(args)):                                          # each leaf alone: the same gradient, nothing else computed
+            some = [a.clone().requires_grad_(i == only) for i, a in enumerate(args)]
+            assert torch.equal(torch.autograd.grad(f(*some), some[only], g)[0], want[only])
+        y = f(*every)
+        first = torch.autograd.grad(y, every[0], g.clone().requires_grad_(True), create_graph=True)[0]
+        assert torch.equal(first.detach(), want[0])
+        with pytest.raises(RuntimeError, match="cannot be differentiated again"):
+            torch.autograd.grad((first * first).sum() + f(*every).sum(), every[0])
+        y = f(*every)
+        with torch.no_grad():
+            every[0].add_(1.0)                                                 # a saved input that changed: autograd notices
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(y, every[0], g)
+
+
 # ------------------------------------------------------------------------------------------------------------------- attention
 def attention_reference(q, k, v, table=None, lut=None, causal=False, q_start=None, k_len=None, attn_mask=None, scale=None, dout=None):
     """({y, dq, dk, dv, dtable} in 64 bits, their tolerances)."""
@@ -575,9 +603,10 @@ def test_linear_strides_alignment_and_shapes():
     # C ABI: y in a wider buffer, its other columns left alone
     x, w = rand(gen, 70, 64, dtype=torch.bfloat16), rand(gen, 30, 64, dtype=torch.bfloat16)
     buf = torch.full((70, 48), 3.0, device="cuda", dtype=torch.bfloat16)
-    a, keep = ops._linear_args(x, w, None, L.ACT_NONE, None)
-    a.y, a.ldy = buf.data_ptr(), 48
-    ops._linear_run(a, L.lib().moy_linear_ws, L.lib().moy_linear, "moy_linear", x.device, ops._st())
+    a = L.LinearArgs()
+    a.x, a.ldx, a.w, a.ldw, a.M, a.N, a.K, a.dtype, a.y, a.ldy = x.data_ptr(), 64, w.data_ptr(), 64, 70, 30, 64, L.BF16, buf.data_ptr(), 48
+    assert L.lib().moy_linear_ws(a) == 0
+    L.check(L.lib().moy_linear(a, ops._st()))
     assert torch.equal(buf[:, :30], ops.linear_forward(x, w)) and bool((buf[:, 30:] == 3.0).all())
 
 

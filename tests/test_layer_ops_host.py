@@ -168,3 +168,25 @@ def test_linear_refuses_cpu_tensors():
         ops.linear_forward(x, w)
     with pytest.raises(RuntimeError, match="Not implemented on the CPU"):
         modules.linear(x, w.requires_grad_(True))
+
+
+def test_host_module_is_built_and_missing_fails_loudly(monkeypatch):
+    import builtins
+    import sys
+
+    from mo_yolo_amd import build
+    build.build(verbose=False)
+    h = _lib.host()
+    assert h is _lib.host() and callable(h.layer_norm) and callable(h.linear) and callable(h.attention)
+    monkeypatch.setattr(_lib, "_host_module", None)
+    monkeypatch.delitem(sys.modules, "mo_yolo_amd._host", raising=False)
+    monkeypatch.delattr(sys.modules["mo_yolo_amd"], "_host", raising=False)
+    real = builtins.__import__
+
+    def no_host(name, globals=None, locals=None, fromlist=(), level=0):
+        if fromlist and "_host" in fromlist:
+            raise ImportError("not there")
+        return real(name, globals, locals, fromlist, level)
+    monkeypatch.setattr(builtins, "__import__", no_host)
+    with pytest.raises(_lib.MoyoloError, match="_host.so"):
+        _lib.host()
