@@ -45,8 +45,8 @@ def _nchw(y2d: torch.Tensor, B, H, W):
 
 
 class _Prepared:
-    """Device-side re-layout of a module's parameters, rebuilt when dtype/device change or after
-    load_state_dict (cleared by the hook registered in _ParamModule)."""
+    """Device-side re-layout of a module's parameters, rebuilt when dtype/device change, after
+    load_state_dict (cleared by the hook registered in _ParamModule), or when a parameter was updated in place (an optimizer's step)."""
 
     def __init__(self):
         self.key = None
@@ -63,7 +63,7 @@ class _ParamModule(nn.Module):
         self._prep.key = None
 
     def _prepared(self, dev, dtype, build):
-        key = (str(dev), dtype)
+        key = (str(dev), dtype, *(0 if p.is_inference() else p._version for p in self.parameters()))
         if self._prep.key != key:
             with torch.no_grad():
                 self._prep.data = build(dev, dtype)
@@ -227,6 +227,10 @@ class _Linear(_ParamModule):
         pr = self._prepared(x2d.device, x2d.dtype, self._build)
         return ops.rowdot(x2d, pr["wf"], pr["b"], mode=mode, aux=aux, aux_rows=aux_rows)
 
+    def forward_train(self, x, act=L.ACT_NONE, residual=None):
+        """The differentiable form (any size): parameters in x's type, their gradients in their own."""
+        return linear(x, self.weight.to(x.dtype), self.bias, act, residual)
+
     def forward(self, x):
         shp = x.shape
         y = self.rows(x.reshape(-1, shp[-1]).contiguous()) if self.cout % 4 == 0 and self.cout > 8 else \
@@ -239,6 +243,9 @@ class _LayerNorm(nn.Module):
         super().__init__()
         self.weight = nn.Parameter(torch.ones(c))
         self.bias = nn.Parameter(torch.zeros(c))
+
+    def forward_train(self, x, residual=None):
+        return layer_norm(x, self.weight, self.bias, 1e-5, residual)
 
     def pair(self, dev):
         return (self.weight.detach().float().to(dev).contiguous(), self.bias.detach().float().to(dev).contiguous())
@@ -326,6 +333,19 @@ def biased_attention(q, k, v, table=None, lut=None, *, causal=False, q_start=Non
     return L.host().attention(q, k, v, table, lut, k_len, attn_mask, *ops._attention_how(q, causal, q_start, scale))
 
 
+class RelativePositionBias(nn.Module):
+    """The learned bias of biased_attention as a module: `weight` [num_buckets, n_heads] and the map of distances to buckets (ops.relative_buckets).
+    forward(q, k, v, **how) is biased_attention with them, the weight in q's type."""
+
+    def __init__(self, num_buckets=32, max_distance=128, n_heads=8, bidirectional=True):
+        super().__init__()
+        self.weight = nn.Parameter(torch.zeros(num_buckets, n_heads))
+        self.register_buffer("lut", ops.relative_buckets(num_buckets, max_distance, bidirectional, "cpu"), persistent=False)
+
+    def forward(self, q, k, v, **how):
+        return biased_attention(q, k, v, self.weight.to(q.dtype), self.lut, **how)
+
+
 class MSDeformAttn(nn.Module):
     """transformer.py:193-287 (d_model 256, 8 heads, 4 points, <= 4 levels, 4-d reference boxes)."""
 
@@ -347,6 +367,26 @@ class MSDeformAttn(nn.Module):
         self.attention_weights.rows(q2d, out_f32=True, out=offaw[:, no:])
         S = value2d.shape[0] // bs
         return ops.msda_fused(value2d, bs, S, shapes, offaw, ref2d, len_q)
+
+    def forward_train(self, query, refer_bbox, value, value_shapes, value_mask=None):
+        """The differentiable form of forward: gradients for query, value and every parameter (and refer_bbox [bs, len_q, 4], where it wants one).  The
+        sampling and the places it samples are fp32 whatever the query's type: its backward exists in fp32 / fp64, and a place's gradient jumps at every
+        cell's edge, so that the share p of places which a rounding moves over one costs sqrt(2 p) of that gradient, not p.  value_shapes: a list, which is copied to the device by every call, or an int64 tensor
+        [levels, 2] there (what a captured step needs)."""
+        bs, len_q = query.shape[:2]
+        M, Lv, P = self.n_heads, self.n_levels, self.n_points
+        v = self.value_proj.forward_train(value)
+        if value_mask is not None:
+            v = v.masked_fill(value_mask[..., None], 0.0)
+        wide = query.float()
+        off = self.sampling_offsets.forward_train(wide).view(bs, len_q, M, Lv, P, 2)
+        aw = self.attention_weights.forward_train(wide).view(bs, len_q, M, Lv * P).softmax(-1).view(bs, len_q, M, Lv, P)
+        box = refer_bbox.float()[:, :, None, None, None]
+        loc = box[..., :2] + off / P * box[..., 2:] * 0.5
+        shapes = value_shapes if torch.is_tensor(value_shapes) else torch.tensor([list(s) for s in value_shapes], dtype=torch.int64, device=query.device)
+        first = torch.cat((shapes.new_zeros(1), (shapes[:, 0] * shapes[:, 1]).cumsum(0)[:-1]))
+        samp = MSDeformAttnFunction.apply(v.float().view(bs, -1, M, self.d_model // M), shapes, first, loc.contiguous(), aw.contiguous(), bs)
+        return self.output_proj.forward_train(samp.to(query.dtype))
 
     def forward(self, query, refer_bbox, value, value_shapes, value_mask=None):
         bs, len_q = query.shape[:2]
@@ -382,6 +422,17 @@ class _MHA(_ParamModule):
         return dict(wqk=ops.pad_weight(W[:2 * E].to(dev), dtype), bqk=b[:2 * E].to(dev).contiguous(),
                     wv=ops.pad_weight(W[2 * E:].to(dev), dtype), bv=b[2 * E:].to(dev).contiguous())
 
+    def forward_train(self, x, pos, attn_mask=None, rel_bias=None):
+        """q = k = x + pos, v = x [bs, Lq, E], differentiable, without the residual: attn_mask bool (True: not attended) [Lq, Lq] or [bs or 1, heads or 1,
+        Lq, Lq]; rel_bias a RelativePositionBias over the order of the queries."""
+        bs, Lq, E = x.shape
+        W, b = self.in_proj_weight.to(x.dtype), self.in_proj_bias
+        heads = lambda t: t.unflatten(-1, (-1, E // self.nh))  # noqa: E731
+        q, k = heads(linear(x + pos, W[:2 * E], b[:2 * E])).split(self.nh, 2)
+        v = heads(linear(x, W[2 * E:], b[2 * E:]))
+        attend = biased_attention if rel_bias is None else rel_bias
+        return self.out_proj.forward_train(attend(q, k, v, q_start=0, attn_mask=attn_mask).flatten(2))
+
     def attend(self, x2d, pos2d, bs, Lq, R=None, ln=None):
         """q = k = x + pos, v = x (transformer.py:637-639); returns out_proj(attn) [+R, LN]."""
         pr = self._prepared(x2d.device, x2d.dtype, self._build)
@@ -394,7 +445,7 @@ class _MHA(_ParamModule):
 
 
 class MOTRDecoderLayer(nn.Module):
-    """transformer.py:515-652 (eval: dropouts are identity)."""
+    """transformer.py:515-652 (dropouts are identity).  forward: inference; forward_train: differentiable, with the masks of denoising training."""
 
     def __init__(self, d_model=256, n_heads=8, d_ffn=1024, dropout=0.1, act=None, n_levels=4, n_points=4, **_unused):
         super().__init__()
@@ -420,6 +471,16 @@ class MOTRDecoderLayer(nn.Module):
         e2 = ca.output_proj.rows(samp, R=e1, ln=self.norm2.pair(dev))
         h = self.linear1.rows(e2, act=L.ACT_RELU)
         return self.linear2.rows(h, R=e2, ln=self.norm3.pair(dev))
+
+    def forward_train(self, embed, refer_bbox, feats, shapes, padding_mask=None, attn_mask=None, track_query_pos=None, rel_bias=None):
+        """forward for training (transformer.py:627-652 with its masks): embed / track_query_pos [bs, Lq, C], refer_bbox [bs, Lq, 4] in (0, 1), feats [bs, S, C];
+        padding_mask bool [bs, S] (True: no feature there), attn_mask and rel_bias as _MHA.forward_train.  float32 / bfloat16 / float16 activations over
+        parameters of any of them; gradients for the inputs and every parameter.  (Planned modules -- MYDecoder and those around it -- copy the
+        weights when their engine is built: hand trained weights to them with load_state_dict.)"""
+        pos = track_query_pos.to(embed.dtype)
+        e1 = self.norm1.forward_train(self.self_attn.forward_train(embed, pos, attn_mask, rel_bias), residual=embed)
+        e2 = self.norm2.forward_train(self.cross_attn.forward_train(e1 + pos, refer_bbox, feats, shapes, padding_mask), residual=e1)
+        return self.norm3.forward_train(self.linear2.forward_train(self.linear1.forward_train(e2, act=L.ACT_RELU)), residual=e2)
 
     def forward(self, embed, refer_bbox, feats, shapes, padding_mask=None, attn_mask=None, track_query_pos=None):
         if padding_mask is not None or attn_mask is not None:
@@ -542,6 +603,17 @@ class QueryInteractionModule(nn.Module):
         track_instances.query_pos = qf
         track_instances.ref_pts = inverse_sigmoid(track_instances.pred_boxes[:, :4].detach().clone())
         return track_instances
+
+    def update_train(self, output_embedding, ref_pts, query_pos):
+        """The learned update of _update_track_embedding, differentiable: output_embedding / query_pos [n, C], ref_pts [n, 4] (no gradient: the reference
+        detaches them) -> the new query_pos [n, C]."""
+        if output_embedding.shape[0] == 0:
+            return query_pos
+        pos = ops.pos2posemb(ref_pts.detach().float().contiguous(), output_embedding.dtype)
+        tgt = self.norm1.forward_train(self.self_attn.forward_train(output_embedding[None], pos[None])[0], residual=output_embedding)
+        tgt = self.norm2.forward_train(self.linear2.forward_train(self.linear1.forward_train(tgt, act=L.ACT_RELU)), residual=tgt)
+        feat = self.linear_feat2.forward_train(self.linear_feat1.forward_train(tgt, act=L.ACT_RELU))
+        return self.norm_feat.forward_train(feat, residual=query_pos.to(feat.dtype))
 
     def forward(self, data: dict) -> Instances:
         return data["track_queries"]
