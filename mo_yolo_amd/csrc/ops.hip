@@ -3,6 +3,7 @@
 // self-attention core, deformable-attention sampling, ID assignment + predictor rows.
 // All HBM-side accesses are 8/16-byte vectors over channels-last rows; reductions and softmax use
 // wave shuffles; nothing here allocates or synchronises.
+#include <algorithm>
 #include "common.hpp"
 
 namespace moy {
@@ -2117,13 +2118,20 @@ extern "C" int moy_msda_fwd_f64(const double* value, const int64_t* spatial_shap
 }
 
 template <typename T>
+__global__ void clear_kernel(T* __restrict__ p, size_t n) {
+  for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) p[i] = T(0);
+}
+
+template <typename T>
 static int msda_bwd(const T* value, const int64_t* shapes, const int64_t* lstart, const T* loc, const T* aw, const T* gout, int N, int S,
                     int M, int D, int L, int Lq, int P, T* gvalue, T* gloc, T* gaw, void* stream) {
   if (!value || !shapes || !lstart || !loc || !aw || !gout || !gvalue || !gloc || !gaw) return MOY_EINVAL;
   if (N <= 0 || S <= 0 || M <= 0 || D <= 0 || L <= 0 || Lq <= 0 || P <= 0) return MOY_EINVAL;
   hipStream_t st = static_cast<hipStream_t>(stream);
   // grad_value accumulates: the reference allocates it with zeros_like (ms_deform_attn_cuda.cu:107); here the callee clears it
-  if (hipMemsetAsync(gvalue, 0, sizeof(T) * (size_t)N * S * M * D, st) != hipSuccess) return MOY_ELAUNCH;
+  // (by a kernel: a captured training step replays it, and a graph's fill nodes are not relied on here)
+  const size_t cells = (size_t)N * S * M * D;
+  hipLaunchKernelGGL((clear_kernel<T>), dim3((unsigned)std::min<size_t>((cells + 255) / 256, 2048)), dim3(256), 0, st, gvalue, cells);
   int G = 1;
   while (G < D && G < 64) G <<= 1;
   const long total = (long)N * Lq * M * L * P;
