@@ -14,6 +14,11 @@
 // 16 (query, head of a shared group) rows to a block, the keys split over waves and blocks, partial results joined in split order); attn_dq_kernel (dQ,
 // delta, sums of dtable); attn_dkv_kernel (dK, dV: a block owns keys and walks the queries of every head that shares them).  The two backward kernels
 // compute S twice instead of adding dQ atomically: results do not depend on the order in which blocks run.
+//
+// Measured: 2 x 4096 causal, 16 heads of 64, bf16: forward 121 us (570 TFLOP/s of the products that count), dQ 208, dK and dV 213; bound by what the vector units
+// do around the matrix cores (the exponential, its argument, maximum, sum and packing: some 140 instructions a wave for 64 keys x 32 queries, beside 32 matrix
+// instructions), at two or three waves to a SIMD.  16 x 300 with a mask by query, 8 heads of 32, fp16: 15.6, 26, 20: five tiles to a block, latency.
+// One query for each of 32 caches of up to 16384 keys, 16 heads over 4 key heads of 64: 77.6 us and 4.7 to join, 5.1 TB/s over the keys that count.
 #include "common.hpp"
 
 namespace moy {
@@ -239,19 +244,76 @@ __device__ __forceinline__ uint32_t mask4(const uint8_t* m, int j, int lk) {
   return w;
 }
 
+// A [ROWS queries][COLS keys] tile of mask bytes as bits in LDS (1: hidden), loaded ahead like the tiles it goes with: 256 threads take 8 or 16 bytes each.
+// Queries past the last repeat the last one's row, and bits past the last key are anything: neither is looked at.
+template <int ROWS, int COLS>
+struct MaskTile {
+  static constexpr int EACH = ROWS * COLS / 256, CB = EACH < 16 ? EACH : 16, N = EACH / CB, CH = COLS / CB, WORDS = COLS / 32, BYTES = ROWS * COLS / 8;
+  static_assert(CB >= 8 && N * CB == EACH, "whole chunks");
+  typedef uint32_t chunk __attribute__((ext_vector_type(CB / 4)));
+  chunk r[N];
+  __device__ __forceinline__ void load(const uint8_t* m, int64_t ld, int row0, int rows, int col0, int cols, int tid) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int c = tid + n * 256, col = col0 + c % CH * CB;
+      const uint8_t* row = m + (int64_t)min(row0 + c / CH, rows - 1) * ld;
+      if (cols >= CB) {
+        __builtin_memcpy(&r[n], row + min(col, cols - CB), CB);                // the last chunk ends with the row, and is shifted below
+      } else {
+#pragma unroll
+        for (int w = 0; w < CB / 4; ++w) {
+          uint32_t v = 0u;
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (col + 4 * w + e < cols) v |= (uint32_t)row[col + 4 * w + e] << (8 * e);
+          r[n][w] = v;
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ void store(uint32_t* lds, int col0, int cols, int tid) const {
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int c = tid + n * 256, col = col0 + c % CH * CB;
+      uint32_t bits = 0u;
+#pragma unroll
+      for (int w = 0; w < CB / 4; ++w) {
+        const uint32_t v = r[n][w], any = ((((v & 0x7f7f7f7fu) + 0x7f7f7f7fu) | v) >> 7) & 0x01010101u;   // a byte that is not 0: its lowest bit
+        bits |= (any * 0x01020408u >> 24 & 15u) << (4 * w);                    // the four gathered (no two products meet)
+      }
+      const int past = cols >= CB ? min(col - min(col, cols - CB), 31) : 0;
+      if constexpr (CB == 16) reinterpret_cast<uint16_t*>(lds)[c] = (uint16_t)(bits >> past);
+      else reinterpret_cast<uint8_t*>(lds)[c] = (uint8_t)(bits >> past);
+    }
+  }
+};
+// the bits of 32 keys from the one `left` short of the end on: those that do not count
+__device__ __forceinline__ uint32_t past_bits(int left) { return left >= 32 ? 0u : ~0u << max(left, 0); }
+// all ones where bit b is set (in assembly: the compiler makes a comparison and a selection of it, with a wait between them)
+__device__ __forceinline__ uint32_t bit_mask(uint32_t w, int b) {
+  uint32_t all;
+  asm("v_bfe_i32 %0, %1, %2, 1" : "=v"(all) : "v"(w), "n"(b));
+  return all;
+}
+__device__ __forceinline__ float pick(uint32_t all, float set, float v) {
+  return __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, set) & all) | (__builtin_bit_cast(uint32_t, v) & ~all));
+}
+
 // keys (backward of dK, dV: queries) of an LDS tile
 template <typename T, int DP>
 constexpr int attn_bk() { return sizeof(T) * DP <= 128 ? 64 : 32; }
 
 // ------------------------------------------------------------------------------------------------------------------------------ forward
-template <typename T, int DP, int NQ, int BK>
+template <typename T, int DP, int NQ, int BK, bool MASK>
 __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(const AttnParams p) {
   constexpr int KP = DP / 32, DT16 = DP / 16, NKT = BK / 16, BQ = 64 * NQ;
   using TL = Tile<T, DP, BK, 256>;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   T* kt_ = reinterpret_cast<T*>(smem);
   T* vt_ = reinterpret_cast<T*>(smem + 2 * TL::BYTES);
-  float* bias = reinterpret_cast<float*>(smem + 4 * TL::BYTES);
+  using ML = MaskTile<BQ, BK>;
+  uint32_t* mt_ = reinterpret_cast<uint32_t*>(smem + 4 * TL::BYTES);
+  float* bias = reinterpret_cast<float*>(smem + 4 * TL::BYTES + 2 * ML::BYTES);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
   const int id = xcd_order(blockIdx.x, gridDim.x);
   int bh, qt;
@@ -283,21 +345,26 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(const AttnParams p) {
     for (int d = 0; d < DT16; ++d) o[d][n] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
   TL kr, vr;
+  ML mr;
   if (nt > 0) {
-    kr.load(kb, p.k_sl, 0, sp.klen, p.D, sp.hide, tid);
-    vr.load(vb, p.v_sl, 0, sp.klen, p.D, sp.hide, tid);
+    kr.load(kb, p.k_sl, 0, sp.klen, p.D, MASK ? sp.hide : nullptr, tid);
+    vr.load(vb, p.v_sl, 0, sp.klen, p.D, MASK ? sp.hide : nullptr, tid);
+    if constexpr (MASK) mr.load(sp.mask, sp.m_sq, qt * BQ, p.Lq, 0, p.Lk, tid);
     if (p.table) load_bias<T>(p, h, bias, 256);
     kr.store(kt_, tid);
     vr.store(vt_, tid);
+    if constexpr (MASK) mr.store(mt_, 0, p.Lk, tid);
   }
   __syncthreads();
   for (int t = 0; t < nt; ++t) {
     const T* ks = kt_ + (t & 1) * (TL::BYTES / (int)sizeof(T));
     const T* vs = vt_ + (t & 1) * (TL::BYTES / (int)sizeof(T));
+    const uint32_t* ms = mt_ + (t & 1) * (ML::BYTES / 4);
     const int j0 = t * BK;
     if (t + 1 < nt) {
-      kr.load(kb, p.k_sl, j0 + BK, sp.klen, p.D, sp.hide, tid);
-      vr.load(vb, p.v_sl, j0 + BK, sp.klen, p.D, sp.hide, tid);
+      kr.load(kb, p.k_sl, j0 + BK, sp.klen, p.D, MASK ? sp.hide : nullptr, tid);
+      vr.load(vb, p.v_sl, j0 + BK, sp.klen, p.D, MASK ? sp.hide : nullptr, tid);
+      if constexpr (MASK) mr.load(sp.mask, sp.m_sq, qt * BQ, p.Lq, j0 + BK, p.Lk, tid);
     }
     f32x4 s[NKT][NQ];
 #pragma unroll
@@ -313,15 +380,15 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(const AttnParams p) {
     }
     const int p0 = q0 + sp.start, p1 = p0 + 16 * NQ - 1;                        // positions of the wave's queries
     const int far = p.table ? beyond(j0, BK, p0, p1, p.far) : -1;
-    const bool cut = sp.mask || j0 + BK > sp.klen || (p.causal && j0 + BK - 1 > p0);
+    const bool cut = MASK || j0 + BK > sp.klen || (p.causal && j0 + BK - 1 > p0);
     Frag<T> pf[BK / 32][NQ];
+    // One bias for the whole tile and every key counts: scale and bias wait for the exponential (scale >= 0: the largest product is the largest score).
+    const bool plain = far && !cut;
+    const float fixed = p.table && far ? bias[far < 0 ? 0 : 2 * p.far + 8] : 0.f;
+    if (!plain) {
 #pragma unroll
-    for (int n = 0; n < NQ; ++n) {
-      const int i = q0 + n * 16 + c, pos = i + sp.start;
-      const float fixed = p.table && far ? bias[far < 0 ? 0 : 2 * p.far + 8] : 0.f;
-      const bool plain = far && !cut;                                           // one bias for the tile, every key counts: scale and bias wait for the exponential
-      float top = -INFINITY;
-      if (!plain) {
+      for (int n = 0; n < NQ; ++n) {
+        const int pos = q0 + n * 16 + c + sp.start;
         if (far) {
 #pragma unroll
           for (int kt = 0; kt < NKT; ++kt) s[kt][n] = s[kt][n] * p.scale2 + fixed;
@@ -335,40 +402,55 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(const AttnParams p) {
         if (cut) {
           const int end = p.causal ? min(sp.klen, pos + 1) : sp.klen;
 #pragma unroll
-          for (int kt = 0; kt < NKT; ++kt) {
-            const int j = j0 + kt * 16 + 4 * g;
-            const uint32_t w = sp.mask && i < p.Lq ? mask4(sp.mask + (int64_t)i * sp.m_sq, j, p.Lk) : 0u;
+          for (int kc = 0; kc < BK / 32; ++kc) {
+            uint32_t off = past_bits(end - j0 - kc * 32);
+            if constexpr (MASK) off |= ms[(wave * 16 * NQ + n * 16 + c) * ML::WORDS + kc];
+            off >>= 4 * g;
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (j + e >= end || ((w >> (8 * e)) & 0xffu)) s[kt][n][e] = -INFINITY;
+            for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) s[2 * kc + kt][n][e] = pick(bit_mask(off, kt * 16 + e), -INFINITY, s[2 * kc + kt][n][e]);
           }
         }
       }
+    }
+    const float mul = plain ? p.scale2 : 1.f, plus = plain ? fixed : 0.f;
+    float top[NQ];
+    bool grown = false;
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+      top[n] = -INFINITY;
 #pragma unroll
       for (int kt = 0; kt < NKT; ++kt)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) top = fmaxf(top, s[kt][n][e]);
-      const float mul = plain ? p.scale2 : 1.f;                                 // (scale >= 0: the largest product is the largest score)
-      top = cols_max(plain ? top * mul + fixed : top);
-      // The reference of the exponentials follows the maximum only where that has grown by more than 2^8: weights stay below 256, which costs nothing of
-      // their precision, and the sums are seldom scaled.  (m = -inf at first: then the reference is the maximum, and a lone key weighs exactly 1.)
-      if (__any(top > m[n] + 8.f)) {
-        const float next = top > m[n] + 8.f ? top : m[n], f = next == m[n] ? 1.f : __builtin_amdgcn_exp2f(m[n] - next);
+        for (int e = 0; e < 4; ++e) top[n] = fmaxf(top[n], s[kt][n][e]);
+      top[n] = cols_max(__builtin_fmaf(top[n], mul, plus));
+      grown |= top[n] > m[n] + 8.f;
+    }
+    // The reference of the exponentials follows the maximum only where that has grown by more than 2^8: weights stay below 256, which costs nothing of
+    // their precision, and the sums are seldom scaled.  (m = -inf at first: then the reference is the maximum, and a lone key weighs exactly 1.)
+    if (__any(grown)) {
+#pragma unroll
+      for (int n = 0; n < NQ; ++n) {
+        const float next = top[n] > m[n] + 8.f ? top[n] : m[n], f = next == m[n] ? 1.f : __builtin_amdgcn_exp2f(m[n] - next);
         l[n] *= f;
 #pragma unroll
         for (int d = 0; d < DT16; ++d) o[d][n] *= f;
         m[n] = next;
       }
-      const float ref = (plain ? fixed : 0.f) - (m[n] == -INFINITY ? 0.f : m[n]);   // nothing counted yet: exp2(-inf) below, not NaN
-      float sum = 0.f;
+    }
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+      const float ref = plus - (m[n] == -INFINITY ? 0.f : m[n]);                // nothing counted yet: exp2(-inf) below, not NaN
+      f32x4 sum = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int kt = 0; kt < NKT; ++kt)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           s[kt][n][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][n][e], mul, ref));
-          sum += s[kt][n][e];
+          sum[e] += s[kt][n][e];
         }
-      l[n] += sum;
+      l[n] += (sum.x + sum.y) + (sum.z + sum.w);
 #pragma unroll
       for (int kc = 0; kc < BK / 32; ++kc) pf[kc][n] = frag_of<T>(s[2 * kc][n], s[2 * kc + 1][n]);
     }
@@ -383,6 +465,7 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(const AttnParams p) {
     if (t + 1 < nt) {
       kr.store(kt_ + ((t + 1) & 1) * (TL::BYTES / (int)sizeof(T)), tid);
       vr.store(vt_ + ((t + 1) & 1) * (TL::BYTES / (int)sizeof(T)), tid);
+      if constexpr (MASK) mr.store(mt_ + ((t + 1) & 1) * (ML::BYTES / 4), j0 + BK, p.Lk, tid);
     }
     __syncthreads();
   }
@@ -415,8 +498,9 @@ __global__ __launch_bounds__(256, 2) void attn_split_kernel(const AttnParams p) 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
   T* vs = reinterpret_cast<T*>(smem + wave * TL::BYTES);
   int id = blockIdx.x;
-  const int split = id % p.splits;
+  const int turn = id % p.splits;
   id /= p.splits;
+  const int split = (turn + id) % p.splits;                                    // (a block's number modulo 8 is its XCD: each takes early and late splits alike, since short sequences have no late ones)
   const int rt = id % p.tiles, bh = id / p.tiles, b = bh / p.Hk, hk = bh - b * p.Hk;
   const int share = p.H / p.Hk, rows = p.Lq * share, row = rt * 16 + c, i = row / share, h = hk * share + row - i * share;
   const bool live = row < rows;
@@ -555,32 +639,38 @@ __global__ __launch_bounds__(256, 2) void attn_split_kernel(const AttnParams p) 
   }
 }
 
-// a row's splits, joined in split order: 64 threads to a row, up to two columns each
+// A row's splits (64 at most), joined in a fixed order by a block: a lane holds a split's maximum and sum, then up to two columns of the result; the
+// waves take every fourth split, so that a row waits for memory twice (32 splits of 32 x 16 rows, heads of 64: one wave to a row took 13.8 us, this 4.7).
 template <typename T>
 __global__ __launch_bounds__(256) void attn_join_kernel(const AttnParams p) {
-  const int64_t n = (int64_t)p.B * p.H * p.Lq, at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (at >= n) return;
-  const int lane = threadIdx.x & 63;
-  float top = -INFINITY;
-  for (int s = 0; s < p.splits; ++s) top = fmaxf(top, p.part[2 * (s * n + at)]);
-  float sum = 0.f, val[2] = {0.f, 0.f};
-  for (int s = 0; s < p.splits; ++s) {
-    const int64_t slot = s * n + at;
-    const float m = p.part[2 * slot], f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top), l = p.part[2 * slot + 1];
-    if (m == -INFINITY && l == l) continue;
-    sum += l == l ? l * f : l;
-    const float* part = p.part + 2 * p.splits * n + slot * p.D;
-#pragma unroll
-    for (int k = 0; k < 2; ++k)
-      if (lane + 64 * k < p.D) val[k] += part[lane + 64 * k] * f;
+  __shared__ float vals[4][128], weight[64];
+  const int64_t n = (int64_t)p.B * p.H * p.Lq, at = blockIdx.x;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  float m = -INFINITY, l = 0.f;
+  if (lane < p.splits) {
+    m = p.part[2 * (lane * n + at)];
+    l = p.part[2 * (lane * n + at) + 1];
   }
-  const int i = at % p.Lq, h = at / p.Lq % p.H, b = at / p.Lq / p.H;
-#pragma unroll
-  for (int k = 0; k < 2; ++k)
-    if (lane + 64 * k < p.D)
-      store_o1(static_cast<T*>(p.o), static_cast<T*>(p.rest), (((int64_t)b * p.Lq + i) * p.H + h) * p.D + lane + 64 * k,
-               sum == 0.f ? 0.f : sum == sum ? val[k] / sum : NAN);
-  if (lane == 0 && p.lse) p.lse[at] = sum == 0.f ? -INFINITY : top + __builtin_amdgcn_logf(sum);
+  const float top = wave_max(m), f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top), sum = wave_sum(l * f);
+  if (wave == 0) weight[lane] = f;
+  __syncthreads();
+  const float* part = p.part + 2 * p.splits * n + at * p.D;
+  const int c0 = min(lane, p.D - 1), c1 = min(lane + 64, p.D - 1);             // (in bounds; not stored below)
+  float val[2] = {0.f, 0.f};
+#pragma unroll 8
+  for (int s = wave; s < p.splits; s += 4) {
+    const float w = weight[s], a = part[s * n * p.D + c0], b = p.D > 64 ? part[s * n * p.D + c1] : 0.f;
+    val[0] += w == 0.f ? 0.f : a * w;                                          // (a split without keys: its columns may hold NaN)
+    val[1] += w == 0.f ? 0.f : b * w;
+  }
+  vals[wave][lane] = val[0];
+  vals[wave][64 + lane] = val[1];
+  __syncthreads();
+  const int d = threadIdx.x, i = at % p.Lq, h = at / p.Lq % p.H, b = at / p.Lq / p.H;
+  if (d < p.D)
+    store_o1(static_cast<T*>(p.o), static_cast<T*>(p.rest), (((int64_t)b * p.Lq + i) * p.H + h) * p.D + d,
+             sum == 0.f ? 0.f : sum == sum ? (((vals[0][d] + vals[1][d]) + vals[2][d]) + vals[3][d]) / sum : NAN);
+  if (d == 0 && p.lse) p.lse[at] = sum == 0.f ? -INFINITY : top + __builtin_amdgcn_logf(sum);
 }
 
 // ----------------------------------------------------------------------------------------------------------------------------- backward
@@ -588,14 +678,16 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnParams p) {
 // The sums by bucket go by distance first, since a distance is a diagonal of dS: 16 queries by 32 keys of dS are laid into the wave's corner of LDS with zeros around
 // them, 47 lanes add a diagonal's 16 entries each and keep it in a table by distance (no two lanes share an entry, so results do not depend on any order); tiles
 // wholly beyond `far` add into two registers instead.  (One LDS addition for each element by bucket took 66 us of 104 on 16 x 300 queries, 8 heads of 32; this takes 10.)
-template <typename T, int DP, int NQ, int BK>
+template <typename T, int DP, int NQ, int BK, bool MASK>
 __global__ __launch_bounds__(256, 2) void attn_dq_kernel(const AttnParams p) {
   constexpr int KP = DP / 32, DT16 = DP / 16, BQ = 64 * NQ;
   using TL = Tile<T, DP, BK, 256>;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   T* kt_ = reinterpret_cast<T*>(smem);
   T* vt_ = reinterpret_cast<T*>(smem + 2 * TL::BYTES);
-  float* bias = reinterpret_cast<float*>(smem + 4 * TL::BYTES);
+  using ML = MaskTile<BQ, BK>;
+  uint32_t* mt_ = reinterpret_cast<uint32_t*>(smem + 4 * TL::BYTES);
+  float* bias = reinterpret_cast<float*>(smem + 4 * TL::BYTES + 2 * ML::BYTES);
   constexpr int DROW = 68, DIAG = 16 * DROW;                                   // the wave's corner: 16 zeros, 32 keys, 16 zeros and 4 to spread the banks
   const int entries = p.table ? (2 * p.far + 12) / 4 * 4 : 0, ends = 2 * p.far + 1;   // (whole 16 bytes)
   float* diag = bias + entries;                                                // [wave][16][DROW]
@@ -613,9 +705,11 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(const AttnParams p) {
   const int kend = p.causal ? min(sp.klen, last + 1) : sp.klen;
   const int nt = kend > 0 ? (kend + BK - 1) / BK : 0;
   TL kr, vr;
+  ML mr;
   if (nt > 0) {
-    kr.load(kb, p.k_sl, 0, sp.klen, p.D, sp.hide, tid);
-    vr.load(vb, p.v_sl, 0, sp.klen, p.D, sp.hide, tid);
+    kr.load(kb, p.k_sl, 0, sp.klen, p.D, MASK ? sp.hide : nullptr, tid);
+    vr.load(vb, p.v_sl, 0, sp.klen, p.D, MASK ? sp.hide : nullptr, tid);
+    if constexpr (MASK) mr.load(sp.mask, sp.m_sq, qt * BQ, p.Lq, 0, p.Lk, tid);
   }
   Frag<T> qf[NQ][KP], gf[NQ][KP];
   float lse[NQ], delta[NQ];
@@ -663,20 +757,24 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(const AttnParams p) {
   if (nt > 0) {
     kr.store(kt_, tid);
     vr.store(vt_, tid);
+    if constexpr (MASK) mr.store(mt_, 0, p.Lk, tid);
   }
   __syncthreads();
   for (int t = 0; t < nt; ++t) {
     const T* ks = kt_ + (t & 1) * (TL::BYTES / (int)sizeof(T));
     const T* vs = vt_ + (t & 1) * (TL::BYTES / (int)sizeof(T));
+    const uint32_t* ms = mt_ + (t & 1) * (ML::BYTES / 4);
     const int j0 = t * BK;
     if (t + 1 < nt) {
-      kr.load(kb, p.k_sl, j0 + BK, sp.klen, p.D, sp.hide, tid);
-      vr.load(vb, p.v_sl, j0 + BK, sp.klen, p.D, sp.hide, tid);
+      kr.load(kb, p.k_sl, j0 + BK, sp.klen, p.D, MASK ? sp.hide : nullptr, tid);
+      vr.load(vb, p.v_sl, j0 + BK, sp.klen, p.D, MASK ? sp.hide : nullptr, tid);
+      if constexpr (MASK) mr.load(sp.mask, sp.m_sq, qt * BQ, p.Lq, j0 + BK, p.Lk, tid);
     }
     const int p0 = q0 + sp.start, p1 = p0 + 16 * NQ - 1;
     const int far = p.table ? beyond(j0, BK, p0, p1, p.far) : -1;
-    const bool cut = sp.mask || j0 + BK > sp.klen || (p.causal && j0 + BK - 1 > p0);
+    const bool cut = MASK || j0 + BK > sp.klen || (p.causal && j0 + BK - 1 > p0);
     const float fixed = p.table && far ? bias[far < 0 ? 0 : 2 * p.far + 8] : 0.f;
+    float sum = 0.f;
 #pragma unroll
     for (int kc = 0; kc < BK / 32; ++kc) {                                     // 32 keys at a time: two score tiles make one operand
       f32x4 s[2][NQ], w[2][NQ];
@@ -700,29 +798,27 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(const AttnParams p) {
       for (int n = 0; n < NQ; ++n) {
         const int i = q0 + n * 16 + c, pos = i + sp.start;
         const int end = p.causal ? min(sp.klen, pos + 1) : sp.klen;
-        float sum = 0.f;
+        uint32_t off = 0u;
+        if (cut) {
+          off = past_bits(end - j0 - kc * 32);
+          if constexpr (MASK) off |= ms[(wave * 16 * NQ + n * 16 + c) * ML::WORDS + kc];
+          off >>= 4 * g;
+        }
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt) {
           const int j = j0 + kc * 32 + kt * 16 + 4 * g;
-          const int at = far ? 0 : bias_at(j - pos, p.far);
           f32x4 add = f32x4{fixed, fixed, fixed, fixed} - lse[n];
-          if (!far) add = bias4(bias + at) - lse[n];
-          uint32_t hid = 0u;
-          if (cut && sp.mask && i < p.Lq) hid = mask4(sp.mask + (int64_t)i * sp.m_sq, j, p.Lk);
+          if (!far) add = bias4(bias + bias_at(j - pos, p.far)) - lse[n];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            // scale, bias and the row's statistic in one multiply-add
-            float d = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][n][e], p.scale2, add[e])) * (w[kt][n][e] - delta[n]);
-            if (cut && (j + e >= end || ((hid >> (8 * e)) & 0xffu))) d = 0.f;
-            s[kt][n][e] = d;
+          for (int e = 0; e < 4; ++e)                                          // scale, bias and the row's statistic in one multiply-add
+            s[kt][n][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][n][e], p.scale2, add[e])) * (w[kt][n][e] - delta[n]);
+          if (cut) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[kt][n][e] = pick(bit_mask(off, kt * 16 + e), 0.f, s[kt][n][e]);
           }
-          if (p.part) {
-            if (far) sum += (s[kt][n].x + s[kt][n].y) + (s[kt][n].z + s[kt][n].w);
-            else *reinterpret_cast<f32x4*>(corner + c * DROW + 16 + kt * 16 + 4 * g) = s[kt][n];
-          }
+          if (far) sum += (s[kt][n].x + s[kt][n].y) + (s[kt][n].z + s[kt][n].w);
+          else if (p.part) *reinterpret_cast<f32x4*>(corner + c * DROW + 16 + kt * 16 + 4 * g) = s[kt][n];
         }
-        if (far < 0) before += sum;
-        if (far > 0) after += sum;
         if (p.part && !far) {
           __builtin_amdgcn_wave_barrier();
           float v = 0.f;
@@ -743,9 +839,12 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(const AttnParams p) {
         for (int n = 0; n < NQ; ++n) dq[d][n] = attn_mma(dq[d][n], a, df[n]);
       }
     }
+    before += far < 0 ? sum : 0.f;
+    after += far > 0 ? sum : 0.f;
     if (t + 1 < nt) {
       kr.store(kt_ + ((t + 1) & 1) * (TL::BYTES / (int)sizeof(T)), tid);
       vr.store(vt_ + ((t + 1) & 1) * (TL::BYTES / (int)sizeof(T)), tid);
+      if constexpr (MASK) mr.store(mt_ + ((t + 1) & 1) * (ML::BYTES / 4), j0 + BK, p.Lk, tid);
     }
     __syncthreads();
   }
@@ -799,14 +898,16 @@ __global__ __launch_bounds__(256) void attn_dtable_kernel(const float* __restric
 
 // dK and dV.  A lane owns a key's column (K and V of it in registers as operands), Q and dO tiles stream through LDS with their rows' lse and delta:
 // S = Q K^T, dP = dO V^T, then dV^T += dO^T P and dK^T += Q^T dS.  The heads that share the keys follow one another, so their sum needs no atomics.
-template <typename T, int DP, int NK, int BQ>
+template <typename T, int DP, int NK, int BQ, bool MASK>
 __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(const AttnParams p) {
   constexpr int KP = DP / 32, DT16 = DP / 16, BKB = 64 * NK;
   using TL = Tile<T, DP, BQ, 256>;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   T* qt_ = reinterpret_cast<T*>(smem);
   T* gt_ = reinterpret_cast<T*>(smem + 2 * TL::BYTES);
-  float* stat = reinterpret_cast<float*>(smem + 4 * TL::BYTES);                // [2][lse BQ | delta BQ]
+  using ML = MaskTile<BQ, BKB>;
+  uint32_t* mt_ = reinterpret_cast<uint32_t*>(smem + 4 * TL::BYTES);
+  float* stat = reinterpret_cast<float*>(smem + 4 * TL::BYTES + 2 * ML::BYTES);   // [2][lse BQ | delta BQ]
   float* bias = stat + 4 * BQ;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
   const int id = xcd_order(blockIdx.x, gridDim.x);
@@ -815,14 +916,14 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(const AttnParams p) {
   jt = p.tiles - 1 - jt;                                                       // (the first keys are seen by the most queries)
   const int b = bh / p.Hk, hk = bh - b * p.Hk, share = p.H / p.Hk;
   const int jb = jt * BKB, jw = jb + wave * 16 * NK;                           // the block's and the wave's first key
-  Span sp = span_of(p, b, hk * share);
+  const Span sp = span_of(p, b, hk * share);
   const T* kb = static_cast<const T*>(p.k) + b * p.k_sb + hk * p.k_sh;
   const T* vb = static_cast<const T*>(p.v) + b * p.v_sb + hk * p.v_sh;
   Frag<T> kf[NK][KP], vf[NK][KP];
 #pragma unroll
   for (int n = 0; n < NK; ++n) {
     const int j = jw + n * 16 + c;
-    const bool in = j < sp.klen && !(sp.hide && p.m_sh == 0 && sp.hide[j]);
+    const bool in = j < sp.klen && !(MASK && sp.hide && p.m_sh == 0 && sp.hide[j]);
 #pragma unroll
     for (int kp = 0; kp < KP; ++kp) {
       const bool on = in && kp * 32 + g * 8 < p.D;
@@ -839,11 +940,13 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(const AttnParams p) {
   const int i0 = p.causal ? max(0, jb - sp.start) / BQ * BQ : 0;
   const int nt = jb < sp.klen && i0 < p.Lq ? (p.Lq - i0 + BQ - 1) / BQ : 0, all = nt * share;
   TL qr, gr;
+  ML mr;
   float st = 0.f;
   auto load = [&](int t) {                                                     // tile t: head t / nt of the group, queries i0 + (t % nt) BQ ..
     const int h = hk * share + t / nt, i = i0 + (t % nt) * BQ;
     qr.load(static_cast<const T*>(p.q) + b * p.q_sb + h * p.q_sh, p.q_sl, i, p.Lq, p.D, nullptr, tid);
     gr.load(static_cast<const T*>(p.dout) + b * p.g_sb + h * p.g_sh, p.g_sl, i, p.Lq, p.D, nullptr, tid);
+    if constexpr (MASK) mr.load(sp.mask + t / nt * p.m_sh, sp.m_sq, i, p.Lq, jb, p.Lk, tid);
     if (tid < 2 * BQ) {
       const int ii = i + tid % BQ;
       const float* src = tid < BQ ? p.lse : p.delta;
@@ -854,6 +957,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(const AttnParams p) {
   auto keep = [&](int t) {
     qr.store(qt_ + (t & 1) * (TL::BYTES / (int)sizeof(T)), tid);
     gr.store(gt_ + (t & 1) * (TL::BYTES / (int)sizeof(T)), tid);
+    if constexpr (MASK) mr.store(mt_ + (t & 1) * (ML::BYTES / 4), jb, p.Lk, tid);
     if (tid < 2 * BQ) stat[(t & 1) * 2 * BQ + tid] = st;
   };
   if (all > 0) {
@@ -869,15 +973,15 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(const AttnParams p) {
         load_bias<T>(p, h, bias, 256);
         __syncthreads();
       }
-      if (sp.mask) sp.mask += p.m_sh;
     }
+    const uint32_t* ms = mt_ + (t & 1) * (ML::BYTES / 4) + wave * NK / 2;      // (the words of the wave's keys)
     const T* qs = qt_ + (t & 1) * (TL::BYTES / (int)sizeof(T));
     const T* gs = gt_ + (t & 1) * (TL::BYTES / (int)sizeof(T));
     const float* ls = stat + (t & 1) * 2 * BQ;
     if (t + 1 < all) load(t + 1);
     const int p0 = iq + sp.start, p1 = p0 + BQ - 1;
     const int far = p.table ? beyond(jw, 16 * NK, p0, p1, p.far) : -1;
-    const bool cut = sp.mask || jw + 16 * NK > sp.klen || (p.causal && jw + 16 * NK - 1 > p0);
+    const bool cut = MASK || jw + 16 * NK > sp.klen || (p.causal && jw + 16 * NK - 1 > p0);
     const float fixed = p.table && far ? bias[far < 0 ? 0 : 2 * p.far + 8] : 0.f;
 #pragma unroll
     for (int qc = 0; qc < BQ / 32; ++qc) {
@@ -902,6 +1006,11 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(const AttnParams p) {
       for (int qq = 0; qq < 2; ++qq) {
         const int i = qc * 32 + qq * 16 + 4 * g;                               // the lane's first of four queries in the tile
         const f32x4 ll = *reinterpret_cast<const f32x4*>(ls + i), dd = *reinterpret_cast<const f32x4*>(ls + BQ + i);
+        uint32_t hid[4] = {0u, 0u, 0u, 0u};
+        if constexpr (MASK) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) hid[e] = ms[(i + e) * ML::WORDS] >> ((wave * NK & 1) * 16 + c);
+        }
 #pragma unroll
         for (int n = 0; n < NK; ++n) {
           const int j = jw + n * 16 + c, pos = p0 + i;
@@ -912,15 +1021,17 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(const AttnParams p) {
           }
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(s[qq][n][e], p.scale2, add[e]));
-            if (cut) {
-              bool off = j >= sp.klen || (p.causal && j > pos + e);
-              if (sp.mask && j < p.Lk && iq + i + e < p.Lq) off |= sp.mask[(int64_t)(iq + i + e) * sp.m_sq + j] != 0;
-              if (off) pr = 0.f;
+            s[qq][n][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[qq][n][e], p.scale2, add[e]));
+            w[qq][n][e] = s[qq][n][e] * (w[qq][n][e] - dd[e]);
+          }
+          if (cut) {
+            const uint32_t off = j >= sp.klen ? 15u : p.causal ? ~past_bits(j - pos) : 0u;   // (bit e: the key lies behind query e)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const uint32_t none = bit_mask(off, e) | bit_mask(hid[e], n * 16);
+              s[qq][n][e] = pick(none, 0.f, s[qq][n][e]);
+              w[qq][n][e] = pick(none, 0.f, w[qq][n][e]);
             }
-            const float d = w[qq][n][e] - dd[e];
-            s[qq][n][e] = pr;
-            w[qq][n][e] = cut && pr == 0.f ? 0.f : pr * d;
           }
         }
       }
@@ -965,7 +1076,7 @@ static int attn_check(const moy_attention_args* a, bool bwd) {
   if (!a->q || !a->k || !a->v || !a->o || a->B <= 0 || a->H <= 0 || a->Hk <= 0 || a->Lq <= 0 || a->Lk <= 0 || a->D <= 0) return MOY_EINVAL;
   if (a->H % a->Hk || a->D % 8) return MOY_EINVAL;
   if (a->D > 128) return MOY_ENOSYS;
-  if (a->Lq > (1 << 30) || a->Lk > (1 << 30) || a->q_start > (1 << 30) || a->q_start < -(1 << 30)) return MOY_EINVAL;
+  if (a->Lq > (1 << 29) || a->Lk > (1 << 29) || a->q_start > (1 << 30) || a->q_start < -(1 << 30)) return MOY_EINVAL;
   if (!aligned16(a->q) || !aligned16(a->k) || !aligned16(a->v) || !aligned16(a->o)) return MOY_EINVAL;
   const int64_t st[] = {a->q_sb, a->q_sl, a->q_sh, a->k_sb, a->k_sl, a->k_sh, a->v_sb, a->v_sl, a->v_sh};
   for (int64_t s : st)
@@ -1011,12 +1122,13 @@ static bool attn_uses_split(const moy_attention_args* a) {
   return (int64_t)a->B * a->H * ((a->Lq + 63) / 64) < 128 && a->Lk >= 1024;
 }
 
-// Splits of at least 256 keys (two 32-key tiles to a wave), as many as give four blocks to a compute unit, 64 at most.
+// Splits of at least 256 keys (two 32-key tiles to a wave), as many as give sixteen blocks to a compute unit, of which four fit at a time: sequences differ in
+// length, and what follows fills in (32 caches of up to 16384 keys, 4 key heads of 64: 90.6 us with four blocks, 84.7 with eight, 77.6 with sixteen).  64 at most.
 static void attn_splits(const moy_attention_args* a, int* tiles, int* splits, int* keys) {
   const int rows = a->Lq * (a->H / a->Hk);
   *tiles = (rows + 15) / 16;
   const int64_t blocks = (int64_t)a->B * a->Hk * *tiles;
-  int64_t s = (1024 + blocks - 1) / blocks;
+  int64_t s = (4096 + blocks - 1) / blocks;
   const int64_t most = (a->Lk + 255) / 256;
   if (s > most) s = most;
   if (s > 64) s = 64;
@@ -1035,19 +1147,19 @@ static size_t attn_bias_bytes(const moy_attention_args* a) { return a->table ? (
 // the registers for twice the waves and are faster with 16 at any size (64 x 300 x 8: 33.9 against 31.4, 50.7 against 45.1).
 static bool attn_wide(const moy_attention_args* a, int heads, int rows) { return (int64_t)a->B * heads * ((rows + 127) / 128) >= 512; }
 
-template <typename T, int DP, int NQ>
+template <typename T, int DP, int NQ, bool MASK>
 static int attn_fwd_tiles(const moy_attention_args* a, AttnParams p, hipStream_t st) {
   constexpr int BK = attn_bk<T, DP>();
-  auto kern = attn_fwd_kernel<T, DP, NQ, BK>;
+  auto kern = attn_fwd_kernel<T, DP, NQ, BK, MASK>;
   static const int ready = attn_lds_opt_in(reinterpret_cast<const void*>(kern));
   if (ready != MOY_OK) return ready;
   p.tiles = (a->Lq + 64 * NQ - 1) / (64 * NQ);
-  const size_t lds = 4 * Tile<T, DP, BK, 256>::BYTES + attn_bias_bytes(a);
+  const size_t lds = 4 * Tile<T, DP, BK, 256>::BYTES + 2 * MaskTile<64 * NQ, BK>::BYTES + attn_bias_bytes(a);
   hipLaunchKernelGGL(kern, dim3((unsigned)(a->B * a->H * p.tiles)), dim3(256), lds, st, p);
   return launch_status();
 }
 
-template <typename T, int DP>
+template <typename T, int DP, bool MASK>
 static int attn_fwd(const moy_attention_args* a, AttnParams p, hipStream_t st) {
   if (attn_uses_split(a)) {
     attn_splits(a, &p.tiles, &p.splits, &p.split_keys);
@@ -1055,34 +1167,34 @@ static int attn_fwd(const moy_attention_args* a, AttnParams p, hipStream_t st) {
     hipLaunchKernelGGL((attn_split_kernel<T, DP>), dim3((unsigned)((int64_t)a->B * a->Hk * p.tiles * p.splits)), dim3(256), 0, st, p);
     const int rc = launch_status();
     if (rc != MOY_OK || p.splits == 1) return rc;
-    hipLaunchKernelGGL((attn_join_kernel<T>), dim3((unsigned)(((int64_t)a->B * a->H * a->Lq + 3) / 4)), dim3(256), 0, st, p);
+    hipLaunchKernelGGL((attn_join_kernel<T>), dim3((unsigned)((int64_t)a->B * a->H * a->Lq)), dim3(256), 0, st, p);
     return launch_status();
   }
   if constexpr (sizeof(T) == 2 && DP == 64) {
-    if (attn_wide(a, a->H, a->Lq)) return attn_fwd_tiles<T, DP, 2>(a, p, st);
+    if (attn_wide(a, a->H, a->Lq)) return attn_fwd_tiles<T, DP, 2, MASK>(a, p, st);
   }
-  return attn_fwd_tiles<T, DP, 1>(a, p, st);
+  return attn_fwd_tiles<T, DP, 1, MASK>(a, p, st);
 }
 
-template <typename T, int DP, int NQ>
+template <typename T, int DP, int NQ, bool MASK>
 static int attn_dq(const moy_attention_args* a, AttnParams p, hipStream_t st) {
   constexpr int BK = attn_bk<T, DP>();
-  auto kern = attn_dq_kernel<T, DP, NQ, BK>;
+  auto kern = attn_dq_kernel<T, DP, NQ, BK, MASK>;
   static const int ready = attn_lds_opt_in(reinterpret_cast<const void*>(kern));
   if (ready != MOY_OK) return ready;
-  const size_t bias = attn_bias_bytes(a), lds = 4 * Tile<T, DP, BK, 256>::BYTES + bias + (p.part ? 4 * 4 * (16 * 68 + 2 * (size_t)a->max_distance + 1) : 0);
+  const size_t bias = attn_bias_bytes(a), lds = 4 * Tile<T, DP, BK, 256>::BYTES + 2 * MaskTile<64 * NQ, BK>::BYTES + bias + (p.part ? 4 * 4 * (16 * 68 + 2 * (size_t)a->max_distance + 1) : 0);
   p.tiles = (a->Lq + 64 * NQ - 1) / (64 * NQ);
   hipLaunchKernelGGL(kern, dim3((unsigned)(a->B * a->H * p.tiles)), dim3(256), lds, st, p);
   return launch_status();
 }
 
-template <typename T, int DP, int NK>
+template <typename T, int DP, int NK, bool MASK>
 static int attn_dkv(const moy_attention_args* a, AttnParams p, hipStream_t st) {
   constexpr int BQ = attn_bk<T, DP>();
-  auto kern = attn_dkv_kernel<T, DP, NK, BQ>;
+  auto kern = attn_dkv_kernel<T, DP, NK, BQ, MASK>;
   static const int ready = attn_lds_opt_in(reinterpret_cast<const void*>(kern));
   if (ready != MOY_OK) return ready;
-  const size_t lds = 4 * Tile<T, DP, BQ, 256>::BYTES + 16 * BQ + attn_bias_bytes(a);
+  const size_t lds = 4 * Tile<T, DP, BQ, 256>::BYTES + 2 * MaskTile<BQ, 64 * NK>::BYTES + 16 * BQ + attn_bias_bytes(a);
   p.tiles = (a->Lk + 64 * NK - 1) / (64 * NK);
   hipLaunchKernelGGL(kern, dim3((unsigned)(a->B * a->Hk * p.tiles)), dim3(256), lds, st, p);
   return launch_status();
@@ -1093,13 +1205,13 @@ static int attn_dq_tiles(const moy_attention_args* a) {
   return (a->Lq + rows - 1) / rows;
 }
 
-template <typename T, int DP>
+template <typename T, int DP, bool MASK>
 static int attn_bwd(const moy_attention_args* a, AttnParams p, hipStream_t st) {
   int rc = MOY_ENOSYS;
   if constexpr (sizeof(T) == 2 && DP == 64) {
-    if (attn_wide(a, a->H, a->Lq)) rc = attn_dq<T, DP, 2>(a, p, st);
+    if (attn_wide(a, a->H, a->Lq)) rc = attn_dq<T, DP, 2, MASK>(a, p, st);
   }
-  if (rc == MOY_ENOSYS) rc = attn_dq<T, DP, 1>(a, p, st);
+  if (rc == MOY_ENOSYS) rc = attn_dq<T, DP, 1, MASK>(a, p, st);
   if (rc != MOY_OK) return rc;
   if (a->dtable) {
     hipLaunchKernelGGL((attn_dtable_kernel<T>), dim3((a->num_buckets * a->H + 3) / 4), dim3(256), 0, st, p.part, a->num_buckets, a->H,
@@ -1108,16 +1220,19 @@ static int attn_bwd(const moy_attention_args* a, AttnParams p, hipStream_t st) {
   }
   if (!a->dk && !a->dv) return MOY_OK;
   if constexpr (sizeof(T) == 2 && DP == 64) {
-    if (attn_wide(a, a->Hk, a->Lk)) return attn_dkv<T, DP, 2>(a, p, st);
+    if (attn_wide(a, a->Hk, a->Lk)) return attn_dkv<T, DP, 2, MASK>(a, p, st);
   }
-  return attn_dkv<T, DP, 1>(a, p, st);
+  return attn_dkv<T, DP, 1, MASK>(a, p, st);
 }
 
+#define MOY_ATTN_HEADS(FN, T, ...)                                                                                              \
+  (a->mask ? (a->D <= 32 ? FN<T, 32, true>(__VA_ARGS__) : a->D <= 64 ? FN<T, 64, true>(__VA_ARGS__) : FN<T, 128, true>(__VA_ARGS__))             \
+           : (a->D <= 32 ? FN<T, 32, false>(__VA_ARGS__) : a->D <= 64 ? FN<T, 64, false>(__VA_ARGS__) : FN<T, 128, false>(__VA_ARGS__)))
 #define MOY_ATTN_DISPATCH(FN, ...)                                                                                            \
   switch (a->dtype) {                                                                                                         \
-    case MOY_F32: return a->D <= 32 ? FN<float, 32>(__VA_ARGS__) : a->D <= 64 ? FN<float, 64>(__VA_ARGS__) : FN<float, 128>(__VA_ARGS__);       \
-    case MOY_BF16: return a->D <= 32 ? FN<bf16_t, 32>(__VA_ARGS__) : a->D <= 64 ? FN<bf16_t, 64>(__VA_ARGS__) : FN<bf16_t, 128>(__VA_ARGS__);   \
-    default: return a->D <= 32 ? FN<f16_t, 32>(__VA_ARGS__) : a->D <= 64 ? FN<f16_t, 64>(__VA_ARGS__) : FN<f16_t, 128>(__VA_ARGS__);            \
+    case MOY_F32: return MOY_ATTN_HEADS(FN, float, __VA_ARGS__);                                                              \
+    case MOY_BF16: return MOY_ATTN_HEADS(FN, bf16_t, __VA_ARGS__);                                                            \
+    default: return MOY_ATTN_HEADS(FN, f16_t, __VA_ARGS__);                                                                   \
   }
 
 }  // namespace moy
