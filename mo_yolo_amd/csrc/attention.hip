@@ -4,8 +4,11 @@
 //   P = softmax_j S over the keys that count     O = P V          empty rows: O = 0, no gradient
 //   dP = dO V^T    dS = P (dP - delta), delta_i = dO_i . O_i      dq = scale dS K    dK = scale dS^T Q    dV = P^T dO    dtable[b] = sum of dS in bucket b
 //
-// One pass over the keys with a running maximum and sum (fp32).  All products run on the matrix cores (16x16 tiles; 16-bit types: K = 32 at a time, P and
-// dS rounded to the type for the second products; fp32: exact fp32 products, K = 4 at a time in the same register layout), and are laid out so that
+// One pass over the keys with a running maximum and sum (fp32).  All products run on the matrix cores, in 16x16 tiles: 16-bit types take K = 32 at a time, fp32
+// exact products of K = 4 at a time in the same register layout.  In 16-bit types the forward's P enters its product as two operands, its rounded value and
+// what that leaves out: the backward takes dO . O for sum_j P_ij dP_ij, and what O missed of that would not cancel in dtable, where rows of dS add up
+// to 0 (a quarter of the forward's time at 2 x 4096; without it dtable was up to 2.4 times, o 1.4 times as far off as one rounding).  P and dS of the
+// backward are rounded once, like the results they go into.  The products are laid out so that
 // probabilities never leave registers: S^T = K Q^T puts a query in a lane's column and four consecutive keys in its accumulator, which is (keys permuted
 // alike on both sides) the operand that O^T = V^T P^T takes.  V^T, K^T, Q^T, dO^T operands come out of row-major LDS tiles through the transposing LDS
 // read (16-bit) or by single elements (fp32).  A row's maximum, sum, delta and position are one lane's scalars; only the maximum crosses lanes.
@@ -15,9 +18,9 @@
 // delta, sums of dtable); attn_dkv_kernel (dK, dV: a block owns keys and walks the queries of every head that shares them).  The two backward kernels
 // compute S twice instead of adding dQ atomically: results do not depend on the order in which blocks run.
 //
-// Measured: 2 x 4096 causal, 16 heads of 64, bf16: forward 121 us (570 TFLOP/s of the products that count), dQ 208, dK and dV 213; bound by what the vector units
-// do around the matrix cores (the exponential, its argument, maximum, sum and packing: some 140 instructions a wave for 64 keys x 32 queries, beside 32 matrix
-// instructions), at two or three waves to a SIMD.  16 x 300 with a mask by query, 8 heads of 32, fp16: 15.6, 26, 20: five tiles to a block, latency.
+// Measured: 2 x 4096 causal, 16 heads of 64, bf16: forward 148 us, dQ 205, dK and dV 213 (465, 500 and 645 TFLOP/s); bound by what the vector units
+// do around the matrix cores (the exponential, its argument, maximum, sum and packing: some 220 instructions a wave of the forward for 64 keys x 32 queries, beside 48
+// matrix instructions), at two or three waves to a SIMD.  16 x 300 with a mask by query, 8 heads of 32, fp16: 17, 25, 19: five tiles to a block, latency.
 // One query for each of 32 caches of up to 16384 keys, 16 heads over 4 key heads of 64: 77.6 us and 4.7 to join, 5.1 TB/s over the keys that count.
 #include "common.hpp"
 
@@ -80,6 +83,14 @@ template <typename T>
 __device__ __forceinline__ Frag<T> frag_of(const f32x4& a, const f32x4& b) {
   if constexpr (sizeof(T) == 4) return Frag<T>{a, b};
   else return Frag<T>{u32x4{pack_as<T>(a.x, a.y), pack_as<T>(a.z, a.w), pack_as<T>(b.x, b.y), pack_as<T>(b.z, b.w)}};
+}
+// what rounding to that operand left out, as another one
+template <typename T>
+__device__ __forceinline__ Frag<T> frag_rest(const f32x4& a, const f32x4& b, const Frag<T>& f) {
+  static_assert(sizeof(T) == 2, "nothing is rounded in fp32");
+  const uint32_t w[4] = {f.w.x, f.w.y, f.w.z, f.w.w};
+  return Frag<T>{u32x4{pack_as<T>(a.x - DT<T>::lo(w[0]), a.y - DT<T>::hi(w[0])), pack_as<T>(a.z - DT<T>::lo(w[1]), a.w - DT<T>::hi(w[1])),
+                       pack_as<T>(b.x - DT<T>::lo(w[2]), b.y - DT<T>::hi(w[2])), pack_as<T>(b.z - DT<T>::lo(w[3]), b.w - DT<T>::hi(w[3]))}};
 }
 // eight consecutive elements of a row, in memory or LDS (16-byte aligned)
 template <typename T>
@@ -307,6 +318,7 @@ constexpr int attn_bk() { return sizeof(T) * DP <= 128 ? 64 : 32; }
 template <typename T, int DP, int NQ, int BK, bool MASK>
 __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(const AttnParams p) {
   constexpr int KP = DP / 32, DT16 = DP / 16, NKT = BK / 16, BQ = 64 * NQ;
+  constexpr bool FINE = sizeof(T) == 2;                                        // P in two operands
   using TL = Tile<T, DP, BK, 256>;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   T* kt_ = reinterpret_cast<T*>(smem);
@@ -381,7 +393,7 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(const AttnParams p) {
     const int p0 = q0 + sp.start, p1 = p0 + 16 * NQ - 1;                        // positions of the wave's queries
     const int far = p.table ? beyond(j0, BK, p0, p1, p.far) : -1;
     const bool cut = MASK || j0 + BK > sp.klen || (p.causal && j0 + BK - 1 > p0);
-    Frag<T> pf[BK / 32][NQ];
+    Frag<T> pf[BK / 32][NQ], pr[FINE ? BK / 32 : 1][NQ];
     // One bias for the whole tile and every key counts: scale and bias wait for the exponential (scale >= 0: the largest product is the largest score).
     const bool plain = far && !cut;
     const float fixed = p.table && far ? bias[far < 0 ? 0 : 2 * p.far + 8] : 0.f;
@@ -452,7 +464,10 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(const AttnParams p) {
         }
       l[n] += (sum.x + sum.y) + (sum.z + sum.w);
 #pragma unroll
-      for (int kc = 0; kc < BK / 32; ++kc) pf[kc][n] = frag_of<T>(s[2 * kc][n], s[2 * kc + 1][n]);
+      for (int kc = 0; kc < BK / 32; ++kc) {
+        pf[kc][n] = frag_of<T>(s[2 * kc][n], s[2 * kc + 1][n]);
+        if constexpr (FINE) pr[kc][n] = frag_rest<T>(s[2 * kc][n], s[2 * kc + 1][n], pf[kc][n]);
+      }
     }
 #pragma unroll
     for (int d = 0; d < DT16; ++d)
@@ -460,7 +475,10 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(const AttnParams p) {
       for (int kc = 0; kc < BK / 32; ++kc) {
         const Frag<T> a = frag_cols<T, TL::PITCH>(vs, kc * 32, d * 16, lane);
 #pragma unroll
-        for (int n = 0; n < NQ; ++n) o[d][n] = attn_mma(o[d][n], a, pf[kc][n]);
+        for (int n = 0; n < NQ; ++n) {
+          o[d][n] = attn_mma(o[d][n], a, pf[kc][n]);
+          if constexpr (FINE) o[d][n] = attn_mma(o[d][n], a, pr[kc][n]);
+        }
       }
     if (t + 1 < nt) {
       kr.store(kt_ + ((t + 1) & 1) * (TL::BYTES / (int)sizeof(T)), tid);
@@ -591,7 +609,11 @@ __global__ __launch_bounds__(256, 2) void attn_split_kernel(const AttnParams p) 
     const Frag<T> pf = frag_of<T>(s[0], s[1]);
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
-    for (int d = 0; d < DT16; ++d) o[d] = attn_mma(o[d], frag_cols<T, TL::PITCH>(vs, 0, d * 16, lane), pf);
+    for (int d = 0; d < DT16; ++d) {
+      const Frag<T> a = frag_cols<T, TL::PITCH>(vs, 0, d * 16, lane);
+      o[d] = attn_mma(o[d], a, pf);
+      if constexpr (sizeof(T) == 2) o[d] = attn_mma(o[d], a, frag_rest<T>(s[0], s[1], pf));
+    }
     __builtin_amdgcn_wave_barrier();
   }
   // join the waves (in wave order)
