@@ -634,8 +634,8 @@ int64_t moy_layer_norm_bwd_ws(int64_t rows, int C, int dtype);    /* floats, or 
  * hide has to be finite wherever any query counts it or not (its weight 0 still multiplies it).
  * ws: fp32 workspace of moy_attention_ws / moy_attention_bwd_ws floats (0: none needed; negative: a MOY_E* code).
  * Backward: dout T [B, Lq, H, D] strided (g_*), the forward's o and lse; dq dense like o, dk / dv dense [B, Lk, Hk, D] (zeros from k_len on), dtable T
- * [num_buckets, H]; each optional, one at least given.  16-bit types: P and dS are rounded to T for the matrix cores, sums are fp32; nothing is
- * added in an order that depends on the launch. */
+ * [num_buckets, H]; each optional, one at least given.  16-bit types: the forward's P enters its product as two operands (its rounded value and the
+ * remainder), P and dS of the backward are rounded to T once; sums are fp32; nothing is added in an order that depends on the launch. */
 typedef struct moy_attention_args {
   const void* q; const void* k; const void* v;
   int64_t q_sb; int64_t q_sl; int64_t q_sh; int64_t k_sb; int64_t k_sl; int64_t k_sh; int64_t v_sb; int64_t v_sl; int64_t v_sh;

@@ -1,6 +1,6 @@
 // The host side of the transformer-layer operators (layer norm, linear, attention): layouts, outputs, workspaces and autograd nodes, in C++ because a training
 // step calls them from autograd's own thread, where each Python operation costs several times its usual price (forward and gradient of a small layer
-// norm: 118 us through Python functions, 70 us here, of which autograd itself takes 55).  Arguments have been checked by mo_yolo_amd.ops; the entry points of
+// norm: 118 us through Python functions, 67 us here, of which autograd itself takes 51).  Arguments have been checked by mo_yolo_amd.ops; the entry points of
 // the C ABI (include/moyolo.h) are handed over as addresses, so that whichever build of the library is loaded is the one that is called.
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>

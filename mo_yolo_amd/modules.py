@@ -328,7 +328,9 @@ def linear(x, weight, bias=None, act=L.ACT_NONE, residual=None):
 
 def biased_attention(q, k, v, table=None, lut=None, *, causal=False, q_start=None, k_len=None, attn_mask=None, scale=None):
     """Attention with a learned relative position bias by buckets, differentiable in q, k, v and table (once); arguments as ops.attention_forward.
-    Without a gradient to compute, the forward alone (a single new token over a long cache among it: the keys are split over the chip)."""
+    Without a gradient to compute, the forward alone (a single new token over a long cache among it: the keys are split over the chip).
+    (Of all three: a training step captured into a graph takes its gradients by torch.autograd.grad, or by backward() with no graph of the same
+    leaves from outside the capture alive: that one's accumulation would wait for a stream that is not captured.)"""
     ops._attention_check(q, k, v, table, lut, q_start, k_len, attn_mask, scale)
     return L.host().attention(q, k, v, table, lut, k_len, attn_mask, *ops._attention_how(q, causal, q_start, scale))
 

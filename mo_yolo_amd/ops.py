@@ -537,7 +537,7 @@ def _norm_check(x, weight, bias, eps, residual):
     _one_device(x, weight, bias, residual)
     _type_code(x)
     dt, shape = x.dtype, x.shape
-    if not shape or shape[-1] == 0:
+    if not shape or not 0 < shape[-1] <= 0x7fffffff:
         raise ValueError("layer_norm: x must be [..., C] with C > 0")
     if residual is not None and (residual.shape != shape or residual.dtype != dt):
         raise ValueError("layer_norm: residual must have x's shape and type")
@@ -587,13 +587,13 @@ def _linear_check(x, weight, bias, act, residual):
         raise ValueError("linear: bias must be [N] in x's type or float32")
     if residual is not None and (residual.shape != (*xs[:-1], ws[0]) or residual.dtype != dt):
         raise ValueError("linear: residual must be [..., N] in x's type")
-    if x.numel() // ws[1] > 0x7fffffff:
-        raise ValueError("linear: more than 2^31 - 1 rows")
+    if max(x.numel() // ws[1], *ws) > 0x7fffffff:
+        raise ValueError("linear: more than 2^31 - 1 rows or columns")
 
 
 def linear_forward(x, weight, bias=None, act=L.ACT_NONE, residual=None, keep_pre=False):
     """act(x weight^T + bias) + residual (moy_linear): x [..., K], weight [N, K] of one type (float32 / bfloat16 / float16), bias [N] in it or float32,
-    residual [..., N]; any sizes, row strides and alignments (rows that are not whole 16-byte steps cost a copy).  -> y, or with keep_pre (y, z):
+    residual [..., N]; any sizes, row strides and alignments (16-bit rows of odd length or at odd elements cost a copy).  -> y, or with keep_pre (y, z):
     z = what act was applied to, as linear_backward takes it (None for ACT_NONE)."""
     _linear_check(x, weight, bias, act, residual)
     y, z = L.host().linear_forward(x, weight, bias, act, residual, keep_pre)
@@ -644,6 +644,8 @@ def _attention_check(q, k, v, table, lut, q_start, k_len, attn_mask, scale):
         raise TypeError("attention: q, k and v must have one type")
     B, Lq, H, D = qs
     Lk, Hk = ks[1], ks[2]
+    if max(B, Lq, Lk, H) > 1 << 29:
+        raise ValueError("attention: more than 2^29 sequences, tokens or heads")
     if Hk == 0 or H == 0 or H % Hk or D == 0 or D % 8 or D > 128:
         raise ValueError("attention: H must be a multiple of Hk and D a multiple of 8 up to 128")
     if (table is None) != (lut is None):

@@ -190,3 +190,16 @@ def test_host_module_is_built_and_missing_fails_loudly(monkeypatch):
     monkeypatch.setattr(builtins, "__import__", no_host)
     with pytest.raises(_lib.MoyoloError, match="_host.so"):
         _lib.host()
+
+
+def test_sizes_that_do_not_fit_the_entry_points_are_refused(monkeypatch):
+    """Sizes are 32-bit behind the checks: a broadcast axis beyond that is an error, not a smaller size."""
+    monkeypatch.setattr(ops, "_one_device", lambda *t: None)
+    long = torch.zeros(1).expand(1, (1 << 32) + 8)
+    with pytest.raises(ValueError, match="layer_norm"):
+        ops._norm_check(long, None, None, 1e-5, None)
+    with pytest.raises(ValueError, match="linear"):
+        ops._linear_check(torch.zeros(2, 8), torch.zeros(1, 8).expand((1 << 32) + 8, 8), None, _lib.ACT_NONE, None)
+    q, k = torch.zeros(1, 4, 2, 8), torch.zeros(1, 1, 2, 8).expand(1, (1 << 32) + 8, 2, 8)
+    with pytest.raises(ValueError, match="attention"):
+        ops._attention_check(q, k, k, None, None, None, None, None, None)
