@@ -1137,11 +1137,12 @@ static AttnParams attn_params(const moy_attention_args* a) {
   return p;
 }
 
-// Few rows, or too few blocks of 64 queries to fill the chip: the keys are split.
+// The keys are split where there are few rows, or too few blocks of 64 queries to fill the chip, and keys enough to pay for the join (us, split against whole: bf16
+// heads of 64, 8 x 8 heads over 2, 4 queries, 4096 keys 13.0 / 72; 8 heads, 64 queries, 4096 keys 16.5 / 72, 1024 keys 11.8 / 20.6, 300 keys 11.5 / 9.2; 64 x 8 heads, 16 queries,
+// 1024 keys 46.5 / 43.4; 512 x 8 heads of 32, 8 queries, 300 keys 64 / 43; fp32, whose products take longer, 3 x 6 heads of 40, 77 queries, 401 keys 14.8 / 26).
 static bool attn_uses_split(const moy_attention_args* a) {
-  const int share = a->H / a->Hk;
-  if ((int64_t)a->Lq * share <= 16) return true;
-  return (int64_t)a->B * a->H * ((a->Lq + 63) / 64) < 128 && a->Lk >= 1024;
+  if (a->Lk < (a->dtype == MOY_F32 ? 256 : 512)) return false;
+  return (int64_t)a->Lq * (a->H / a->Hk) <= 16 || (int64_t)a->B * a->H * ((a->Lq + 63) / 64) < 128;
 }
 
 // Splits of at least 256 keys (two 32-key tiles to a wave), as many as give sixteen blocks to a compute unit, of which four fit at a time: sequences differ in

@@ -11,7 +11,7 @@
 // block order, so results do not depend on the order in which blocks run.  Sums and statistics are fp32; y / dx are rounded once.
 // Loads and stores are 16 bytes at any alignment (the hardware splits what crosses a line), so an odd width costs only its last chunk.
 // Measured: 108528 x 256 bf16 forward 20.3 us (5.5 TB/s), backward 29.1 (5.7) and 4 for the sums; 16384 x 4096 fp32 95 (5.6) and 158 (5.1), where a
-// large copy reaches 5.1; 4099 x 1283 fp16 with a residual 17 and 25; 300 x 256 4.3.
+// large copy reaches 5.1; 4099 x 1283 fp16 with a residual 14 and 26; 300 x 256 4.3.
 #include "chunk.hpp"
 
 namespace moy {
@@ -228,9 +228,12 @@ __global__ __launch_bounds__(LnGeom<TPR>::THREADS) void ln_bwd_kernel(const LnPa
     }
 }
 
-// Lanes and chunks for a row of `chunks` 16-byte pieces: the fewest lanes that hold it in one or two chunks each (registers), 2048 chunks at most
-// (16384 channels of 16 bits, 8192 of fp32).
-static int ln_lanes(int chunks) { return chunks <= 32 ? 16 : chunks <= 128 ? 64 : chunks <= 512 ? 256 : chunks <= 2048 ? 1024 : 0; }
+// Lanes and chunks for a row of `chunks` 16-byte pieces: the fewest lanes that hold it in one or two chunks each, 2048 chunks at most (16384 channels of 16
+// bits, 8192 of fp32).  The forward has the registers for three chunks in a wave's lanes, which save it the block's barriers; the backward has not (65536 x 1536
+// bf16 with three chunks against a block of 256 lanes: forward 74 us / 108, backward 171 / 149; with four, 65536 x 2048: 134 / 116).
+static int ln_lanes(int chunks, bool bwd) {
+  return chunks <= 32 ? 16 : chunks <= (bwd ? 128 : 192) ? 64 : chunks <= 512 ? 256 : chunks <= 2048 ? 1024 : 0;
+}
 
 static int ln_chunks(int C, int dtype) { return dtype == MOY_F32 ? (C + 3) / 4 : (C + 7) / 8; }
 
@@ -251,7 +254,11 @@ static int ln_launch(const LnParams& p, int lanes, int chunks, int blocks, hipSt
   const bool one = chunks <= lanes;
   switch (lanes) {
     case 16: if (one) MOY_LN(16, 1) else MOY_LN(16, 2)
-    case 64: if (one) MOY_LN(64, 1) else MOY_LN(64, 2)
+    case 64:
+      if constexpr (!BWD) {
+        if (chunks > 128) MOY_LN(64, 3)
+      }
+      if (one) MOY_LN(64, 1) else MOY_LN(64, 2)
     case 256: if (one) MOY_LN(256, 1) else MOY_LN(256, 2)
     default: if (one) MOY_LN(1024, 1) else MOY_LN(1024, 2)
   }
@@ -260,7 +267,7 @@ static int ln_launch(const LnParams& p, int lanes, int chunks, int blocks, hipSt
 
 template <bool BWD>
 static int ln_dispatch(const LnParams& p, int dtype, hipStream_t st) {
-  const int chunks = ln_chunks(p.C, dtype), lanes = ln_lanes(chunks);
+  const int chunks = ln_chunks(p.C, dtype), lanes = ln_lanes(chunks, BWD);
   const int blocks = ln_blocks(p.rows, lanes);
   switch (dtype) {
     case MOY_F32: return ln_launch<float, BWD>(p, lanes, chunks, blocks, st);
@@ -272,7 +279,7 @@ static int ln_dispatch(const LnParams& p, int dtype, hipStream_t st) {
 static int ln_check(int64_t rows, int C, int dtype, int w_dtype, bool weights) {
   if (rows <= 0 || C <= 0 || dtype < MOY_F32 || dtype > MOY_F16) return MOY_EINVAL;
   if (weights && w_dtype != MOY_F32 && w_dtype != dtype) return MOY_EINVAL;
-  return ln_lanes(ln_chunks(C, dtype)) ? MOY_OK : MOY_ENOSYS;
+  return ln_lanes(ln_chunks(C, dtype), true) ? MOY_OK : MOY_ENOSYS;
 }
 
 }  // namespace moy
@@ -295,7 +302,7 @@ extern "C" int moy_layer_norm(const void* x, int64_t ldx, const void* r, int64_t
 extern "C" int64_t moy_layer_norm_bwd_ws(int64_t rows, int C, int dtype) {
   const int rc = ln_check(rows, C, dtype, MOY_F32, false);
   if (rc != MOY_OK) return rc;
-  return (int64_t)ln_blocks(rows, ln_lanes(ln_chunks(C, dtype))) * 2 * C;
+  return (int64_t)ln_blocks(rows, ln_lanes(ln_chunks(C, dtype), true)) * 2 * C;
 }
 
 extern "C" int moy_layer_norm_bwd(const void* dy, int64_t ldd, const void* x, int64_t ldx, const void* r, int64_t ldr, const void* w, int w_dtype,
@@ -309,7 +316,7 @@ extern "C" int moy_layer_norm_bwd(const void* dy, int64_t ldd, const void* x, in
       !aligned_as(dw, w_dtype) || !aligned_as(db, w_dtype))
     return MOY_EINVAL;
   const bool sums = dw || db;
-  const int blocks = ln_blocks(rows, ln_lanes(ln_chunks(C, dtype)));
+  const int blocks = ln_blocks(rows, ln_lanes(ln_chunks(C, dtype), true));
   if (sums && (!ws || ws_len < (int64_t)blocks * 2 * C)) return MOY_EINVAL;
   LnParams p{};
   p.x = x; p.ldx = ldx; p.r = r; p.ldr = ldr; p.dy = dy; p.ldd = ldd; p.w = w; p.w_dtype = w_dtype;

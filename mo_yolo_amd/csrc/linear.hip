@@ -9,6 +9,8 @@
 // (128 bytes of k to a tile row, XOR-swizzled by way of the lanes' source addresses, what lies outside a matrix arrives as zeros), double-buffered
 // with one barrier per tile of k.  Products with too few tiles for the chip are split over k: fp32 partial results, joined in order by a second kernel that
 // also runs the epilogue.  Up to 32 rows (a new token of each sequence) take lin_few_kernel, which streams W once through registers.
+// Measured: 8192 x 4096 -> 4096 bf16 forward with z and a residual 240 to 260 us, dx 231, dW 227 (1.06 to 1.21 PFLOP/s, a large library product 1.22); 4800 x 256 -> 1024 14, 12,
+// 10 + 4; 1803 x 514 -> 770 fp32 35, 31 + 9, 28 + 6; one row of 1024 -> 4096 4.8: bound by the matrix cores' feeding, launches, the fp32 matrix rate, the trip to memory.
 // dz is its own pass (it feeds two products and the sums of db; in the products' prologues it would be recomputed for every column tile).
 // Loads are 16 bytes from any dword on; where a row ends inside one, the tail is cleared in LDS.  16-bit rows of odd length or at odd elements are
 // copied into padded rows first.
@@ -616,6 +618,8 @@ static bool lin_direct(const void* p, int64_t ld, int n, int es) {
 static int64_t lin_span(int64_t rows, int64_t ld, int64_t n, int es) { return ((rows - 1) * ld + n) * es; }
 static int64_t lin_pitch(int n, int es) { return ((int64_t)n * es + 15) / 16 * 16 / es; }
 
+// Few rows go through lin_few_kernel (us, against the tiled kernel, bf16: 1 row 256 -> 256 3.6 / 4.6, 1024 -> 4096 4.1 / 7.9, 4096 -> 4096 10.5 / 10.0; 16 rows 2.9 / 4.6, 4.4 / 7.9,
+// 10.0 / 10.8; 32 rows 3.3 / 4.7, 5.3 / 8.0, 14.1 / 12.4).
 static bool lin_few(int M) { return M <= 32; }
 
 template <typename T, bool ACOL, bool BCOL>
