@@ -44,6 +44,11 @@ def _nchw(y2d: torch.Tensor, B, H, W):
     return y2d.view(B, H, W, -1).permute(0, 3, 1, 2)
 
 
+def _fits(t, x):
+    """A vector parameter as the operators take it beside x: in float32 or x's own type."""
+    return t if t is None or t.dtype in (torch.float32, x.dtype) else t.to(x.dtype)
+
+
 class _Prepared:
     """Device-side re-layout of a module's parameters, rebuilt when dtype/device change, after
     load_state_dict (cleared by the hook registered in _ParamModule), or when a parameter was updated in place (an optimizer's step)."""
@@ -229,7 +234,7 @@ class _Linear(_ParamModule):
 
     def forward_train(self, x, act=L.ACT_NONE, residual=None):
         """The differentiable form (any size): parameters in x's type, their gradients in their own."""
-        return linear(x, self.weight.to(x.dtype), self.bias, act, residual)
+        return linear(x, self.weight.to(x.dtype), _fits(self.bias, x), act, residual)
 
     def forward(self, x):
         shp = x.shape
@@ -245,7 +250,7 @@ class _LayerNorm(nn.Module):
         self.bias = nn.Parameter(torch.zeros(c))
 
     def forward_train(self, x, residual=None):
-        return layer_norm(x, self.weight, self.bias, 1e-5, residual)
+        return layer_norm(x, _fits(self.weight, x), _fits(self.bias, x), 1e-5, residual)
 
     def pair(self, dev):
         return (self.weight.detach().float().to(dev).contiguous(), self.bias.detach().float().to(dev).contiguous())
@@ -428,7 +433,7 @@ class _MHA(_ParamModule):
         """q = k = x + pos, v = x [bs, Lq, E], differentiable, without the residual: attn_mask bool (True: not attended) [Lq, Lq] or [bs or 1, heads or 1,
         Lq, Lq]; rel_bias a RelativePositionBias over the order of the queries."""
         bs, Lq, E = x.shape
-        W, b = self.in_proj_weight.to(x.dtype), self.in_proj_bias
+        W, b = self.in_proj_weight.to(x.dtype), _fits(self.in_proj_bias, x)
         heads = lambda t: t.unflatten(-1, (-1, E // self.nh))  # noqa: E731
         q, k = heads(linear(x + pos, W[:2 * E], b[:2 * E])).split(self.nh, 2)
         v = heads(linear(x, W[2 * E:], b[2 * E:]))

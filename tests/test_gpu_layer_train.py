@@ -102,6 +102,21 @@ def test_decoder_layer_trains(dtype, masked, tol, gtol):
         assert off(rel.weight.grad, table.grad) < gtol * 2
 
 
+@pytest.mark.parametrize("held,dtype", [(torch.bfloat16, torch.bfloat16), (torch.float16, torch.float16), (torch.bfloat16, torch.float32), (torch.bfloat16, torch.float16)])
+def test_decoder_layer_with_16_bit_parameters(held, dtype):
+    """Parameters in 16 bits, activations in the same type or another: output as above, gradients in the parameters' type."""
+    layer = fill(M.MOTRDecoderLayer(256, 8, 512, 0.0, None, 3, 4), 13).to(DEV, held)
+    shapes, embed, pos, feats, box, dy = decoder_case(14)
+    rnd = lambda t: t.to(dtype).double()  # noqa: E731
+    out = layer.forward_train(embed.to(DEV, dtype), box.to(DEV), feats.to(DEV, dtype), shapes, track_query_pos=pos.to(DEV, dtype))
+    out.backward(dy.to(DEV, dtype))
+    sd, _ = double_of(layer, "l")
+    want = oracle_layer(shapes, rnd(embed), box.double(), rnd(feats), rnd(pos), sd)
+    assert out.dtype == dtype and off(out, want) < 4e-2
+    for n, p in layer.named_parameters():
+        assert p.grad is not None and p.grad.dtype == held and torch.isfinite(p.grad).all(), n
+
+
 def test_forward_train_agrees_with_forward_and_forward_sees_updates():
     layer = fill(M.MOTRDecoderLayer(256, 8, 512, 0.0, None, 3, 4), 5).to(DEV)
     shapes, embed, pos, feats, box, dy = (t if isinstance(t, list) else t.to(DEV) for t in decoder_case(6))
