@@ -646,3 +646,54 @@ def test_linear_repeats_on_any_stream_and_in_graphs():
         g.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, c) for a, c in zip(out, want))
+
+
+@pytest.mark.parametrize("Lq,Lk,dtype", [(3, 1, "f32"), (70, 5, "bf16"), (33, 15, "f16"), (130, 16, "bf16"), (65, 17, "f32"), (64, 63, "f16"), (200, 130, "bf16"), (5, 600, "f16"),
+                                         (129, 331, "f32")])
+@pytest.mark.parametrize("D", [32, 64, 128])
+def test_attention_masks_of_any_bytes_and_strides(Lq, Lk, dtype, D):
+    """A mask by batch, head and query as bytes of any value but 0, at odd addresses and row strides, hides what the dense boolean one does: bit for bit."""
+    B, H, Hk = 2, 4, 2
+    q, k, v, table, lut, dout = attention_inputs(Lq * 7 + Lk, B, Lq, Lk, H, Hk, D, dtype, 8, 20)
+    g = torch.Generator().manual_seed(Lq + Lk)
+    hidden = torch.rand(B, H, Lq, Lk, generator=g) < 0.4
+    hidden[0, 1, Lq // 2] = True                                               # a row without a key
+    wide = torch.zeros(B, H, Lq, Lk + 9, dtype=torch.uint8)
+    wide[..., 3:3 + Lk] = torch.where(hidden, torch.randint(1, 256, hidden.shape, generator=g), torch.zeros(1, dtype=torch.int64)).to(torch.uint8)
+    wide[..., :3] = wide[..., 3 + Lk:] = 255                                   # what stands beside the rows is not looked at
+    odd = wide.cuda()[..., 3:3 + Lk]
+    assert odd.stride(2) == Lk + 9 and odd.storage_offset() == 3
+    leaves = (q, k, v, table)
+    runs = []
+    for m in (hidden.cuda(), odd):
+        y = modules.biased_attention(q, k, v, table, lut, q_start=0, attn_mask=m)
+        runs.append((y, *torch.autograd.grad(y, leaves, dout)))
+    for a, b in zip(*runs):
+        assert torch.isfinite(a).all() and torch.equal(a, b)
+    assert not runs[0][0][0, Lq // 2, 1].any() and not runs[0][1][0, Lq // 2, 1].any()
+    out, tol = attention_reference(q.detach(), k.detach(), v.detach(), table.detach(), lut, dout=dout, q_start=0, attn_mask=hidden.cuda())
+    for name, got in zip(("y", "dq", "dk", "dv", "dtable"), runs[1]):
+        close(got, out[name], tol[name], name)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("Lk", [255, 256, 511, 512, 513, 5000])
+def test_attention_one_query_either_side_of_the_split(Lk, dtype):
+    """One query for each of three caches, one of them empty and one of a single key, where the keys are taken whole and where they are split."""
+    q, k, v, table, lut, _ = attention_inputs(Lk, 3, 1, Lk, 8, 2, 64, dtype, 32, 100, grad=False)
+    how = dict(causal=True, k_len=torch.tensor([0, 1, Lk - 1], dtype=torch.int32, device="cuda"))
+    y = modules.biased_attention(q, k, v, table, lut, **how)
+    out, tol = attention_reference(q, k, v, table, lut, **how)
+    close(y, out["y"], tol["y"], "y")
+    assert not y[0].any() and torch.equal(y[1, 0], v[1, 0].repeat_interleave(4, 0))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_attention_masked_with_two_tiles_to_a_wave(dtype):
+    """Heads enough that a wave takes 32 queries (keys): the mask's rows and words of both halves, with a ragged end."""
+    B, H, Lq, Lk = 64, 8, 75, 141
+    q, k, v, table, lut, dout = attention_inputs(3, B, Lq, Lk, H, H, 64, dtype, 16, 30)
+    hidden = torch.rand(B, 1, Lq, Lk, generator=torch.Generator().manual_seed(4)) < 0.3
+    kl = torch.full((B,), Lk, dtype=torch.int32)
+    kl[::3] = 100
+    check_attention(q, k, v, table, lut, dout, q_start=20, causal=True, k_len=kl.cuda(), attn_mask=hidden.cuda())
