@@ -50,12 +50,21 @@ def _fits(t, x):
 
 
 class _Prepared:
-    """Device-side re-layout of a module's parameters, rebuilt when dtype/device change, after
-    load_state_dict (cleared by the hook registered in _ParamModule), or when a parameter was updated in place (an optimizer's step)."""
+    """Device-side re-layout of a module's parameters, rebuilt when dtype / device change, after load_state_dict (cleared by the hook registered in _ParamModule), when a
+    parameter was updated in place (its version) or got other memory (its address; `held` keeps the old memory, so that no other can come to lie there), and by
+    forget_prepared.  A module whose differentiable form has run is being trained until its parameters are frozen (requires_grad_(False)): a replayed graph may change
+    them with no version to show for it, so they are laid out anew by every call -- inside the graph, where a call is captured."""
 
     def __init__(self):
-        self.key = None
-        self.data = None
+        self.key = self.data = self.held = None
+        self.trained = False
+        self.captured = []                     # what recorded graphs read
+
+    def __getstate__(self):                    # a copy of a module prepares its own
+        return _Prepared().__dict__
+
+    def __setstate__(self, _state):
+        self.__init__()
 
 
 class _ParamModule(nn.Module):
@@ -67,13 +76,33 @@ class _ParamModule(nn.Module):
     def _invalidate(self):
         self._prep.key = None
 
+    def _trains(self):
+        """Called by the differentiable forms."""
+        if torch.is_grad_enabled():
+            self._prep.trained = True
+
     def _prepared(self, dev, dtype, build):
-        key = (str(dev), dtype, *(0 if p.is_inference() else p._version for p in self.parameters()))
-        if self._prep.key != key:
+        prep, params = self._prep, list(self.parameters())
+        if prep.trained and any(p.requires_grad for p in params):
+            prep.key = prep.data = prep.held = None
             with torch.no_grad():
-                self._prep.data = build(dev, dtype)
-            self._prep.key = key
-        return self._prep.data
+                return build(dev, dtype)
+        key = (str(dev), dtype, *((p.data_ptr(), 0 if p.is_inference() else p._version) for p in params))
+        if prep.key != key:
+            with torch.no_grad():
+                prep.data, prep.held = build(dev, dtype), [p.detach() for p in params]
+            prep.key = key
+        if dev.type == "cuda" and torch.cuda.is_current_stream_capturing() and not any(prep.data is d for d in prep.captured):
+            prep.captured.append(prep.data)
+        return prep.data
+
+
+def forget_prepared(module):
+    """Has every submodule lay its parameters out anew at its next inference call: needed where parameters of a module that never ran forward_train / update_train were
+    written in a way that torch does not count (through `.data`, under inference_mode, by a kernel or a replayed graph of the caller's own)."""
+    for m in module.modules():
+        if isinstance(m, _ParamModule):
+            m._invalidate()
 
 
 def _bn_fold(bn: nn.BatchNorm2d, dev):
@@ -234,6 +263,7 @@ class _Linear(_ParamModule):
 
     def forward_train(self, x, act=L.ACT_NONE, residual=None):
         """The differentiable form (any size): parameters in x's type, their gradients in their own."""
+        self._trains()
         return linear(x, self.weight.to(x.dtype), _fits(self.bias, x), act, residual)
 
     def forward(self, x):
@@ -432,6 +462,7 @@ class _MHA(_ParamModule):
     def forward_train(self, x, pos, attn_mask=None, rel_bias=None):
         """q = k = x + pos, v = x [bs, Lq, E], differentiable, without the residual: attn_mask bool (True: not attended) [Lq, Lq] or [bs or 1, heads or 1,
         Lq, Lq]; rel_bias a RelativePositionBias over the order of the queries."""
+        self._trains()
         bs, Lq, E = x.shape
         W, b = self.in_proj_weight.to(x.dtype), _fits(self.in_proj_bias, x)
         heads = lambda t: t.unflatten(-1, (-1, E // self.nh))  # noqa: E731

@@ -1,0 +1,111 @@
+"""GPU: what the transformer-layer operators must refuse, must keep and must not round away, at the edges of their types, strides and weights.  Tolerances as in
+test_gpu_layer_ops: half a step of a type for each rounding, 2^-24 for each fp32 operation of the longest chain."""
+import pytest
+import torch
+
+from mo_yolo_amd import _lib as L
+from mo_yolo_amd import modules as M
+from mo_yolo_amd import ops
+
+pytestmark = pytest.mark.gpu
+DT = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+U32 = 2.0 ** -24
+
+
+def half_step(t):
+    return torch.finfo(t).eps / 2
+
+
+def tiny(t):
+    return torch.finfo(t).smallest_normal * torch.finfo(t).eps / 2
+
+
+def rand(gen, *shape, dtype=torch.float32, scale=1.0):
+    return (torch.randn(*shape, device="cuda", generator=gen) * scale).to(dtype)
+
+
+def gen_of(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+# ---------------------------------------------------------------------------------------------------------------- prepared weights
+def layer_case(gen, dtype=torch.float32):
+    shapes = [(9, 13), (5, 7), (3, 4)]
+    S = sum(h * w for h, w in shapes)
+    embed, pos, feats = rand(gen, 2, 30, 256, dtype=dtype), rand(gen, 2, 30, 256, dtype=dtype), rand(gen, 2, S, 256, dtype=dtype)
+    return shapes, embed, pos, feats, torch.rand(2, 30, 4, device="cuda", generator=gen) * 0.6 + 0.2
+
+
+def agree(layer, shapes, embed, pos, feats, box):
+    """forward against forward_train: two orders of the same fp32 sums, outputs of unit size."""
+    with torch.no_grad():
+        a = layer(embed, box, feats, [tuple(s) for s in shapes], track_query_pos=pos)
+        b = layer.forward_train(embed, box, feats, shapes, track_query_pos=pos)
+    return float((a - b).abs().max()) < 1e-4
+
+
+def test_forward_sees_what_a_replayed_training_step_changed():
+    """A replay changes the weights behind the back of their version counters."""
+    layer = M.MOTRDecoderLayer(256, 8, 512, 0.0, None, 3, 4).cuda()
+    case = layer_case(gen_of(5))
+    shapes, embed, pos, feats, box = case
+    sizes = torch.tensor(shapes, dtype=torch.int64, device="cuda")
+    dy = rand(gen_of(6), 2, 30, 256)
+    params = list(layer.parameters())
+    assert agree(layer, *case)                                                 # (prepared weights are there)
+
+    def step():
+        grads = torch.autograd.grad(layer.forward_train(embed, box, feats, sizes, track_query_pos=pos), params, dy)
+        with torch.no_grad():
+            for p, g in zip(params, grads):
+                p.sub_(g, alpha=1e-3)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            step()
+    torch.cuda.synchronize()
+    for _ in range(3):
+        before = [p.detach().clone() for p in params]
+        graph.replay()
+        torch.cuda.synchronize()
+        assert any(not torch.equal(a, p) for a, p in zip(before, params))
+        assert agree(layer, *case)
+    layer.requires_grad_(False)                                                # trained: kept again
+    assert agree(layer, *case) and agree(layer, *case)
+
+
+def test_a_captured_forward_follows_the_weights():
+    """The inference form of a layer that is being trained, in a graph: each replay uses the weights as they are then, also after eager forwards in between."""
+    layer = M.MOTRDecoderLayer(256, 8, 512, 0.0, None, 3, 4).cuda()
+    shapes, embed, pos, feats, box = layer_case(gen_of(7))
+    run = lambda: layer(embed, box, feats, shapes, track_query_pos=pos)  # noqa: E731
+    opt = torch.optim.SGD(layer.parameters(), lr=1e-3)
+
+    def train():
+        opt.zero_grad()
+        layer.forward_train(embed, box, feats, shapes, track_query_pos=pos).sum().backward()
+        opt.step()
+    train()
+    opt.zero_grad(set_to_none=True)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.no_grad():
+        with torch.cuda.stream(side):
+            run()
+            torch.cuda.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=side):
+                out = run()
+    torch.cuda.synchronize()
+    for _ in range(3):
+        train()
+        with torch.no_grad():
+            want = run()
+            graph.replay()
+            torch.cuda.synchronize()
+        assert torch.equal(out, want)
