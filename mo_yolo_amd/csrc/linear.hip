@@ -82,6 +82,23 @@ __device__ __forceinline__ float lin_act_grad(float v, int act) {
   }
 }
 
+// An argument of the activation as it is kept for the backward: what is finite stays finite and what is not 0 stays on its side of 0 when it is rounded to T.  (fp16
+// would hold 7e4 as infinity, where the derivative of SiLU is 0 * infinity, and 2^-26 as 0, where ReLU's gate is shut.)
+template <typename T>
+__device__ __forceinline__ float lin_kept(float v) {
+  if constexpr (sizeof(T) == 4) return v;
+  constexpr bool HALF = DT<T>::code == MOY_F16;
+  constexpr float MOST = HALF ? 65504.f : 0x1.fep127f;
+  if constexpr (HALF) v = fabsf(v) <= 0x1p-25f && v != 0.f ? copysignf(0x1p-24f, v) : v;   // half of the smallest number would still round to 0
+  return fabsf(v) < INFINITY ? __builtin_amdgcn_fmed3f(v, -MOST, MOST) : v;
+}
+template <typename T>
+__device__ __forceinline__ f32x4 lin_kept4(f32x4 v) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = lin_kept<T>(v[e]);
+  return v;
+}
+
 // the bias of columns n .. n + 3 (zeros without one)
 __device__ __forceinline__ f32x4 lin_bias(const LinParams& p, int n) {
   f32x4 b = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -96,7 +113,7 @@ __device__ __forceinline__ f32x4 lin_bias(const LinParams& p, int n) {
 // four outputs of row m from column n on, their bias added: z, activation, residual (r: loaded ahead where outputs are whole vectors)
 template <typename T>
 __device__ __forceinline__ void lin_finish_vec(const LinParams& p, int m, int n, f32x4 v, f32x4 r) {
-  if (p.z) DT<T>::store4(static_cast<T*>(p.z) + (int64_t)m * p.ldz + n, v);
+  if (p.z) DT<T>::store4(static_cast<T*>(p.z) + (int64_t)m * p.ldz + n, lin_kept4<T>(v));
   if (p.act != MOY_ACT_NONE) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] = lin_act<T>(v[e], p.act);
@@ -110,7 +127,7 @@ __device__ __forceinline__ void lin_finish_each(const LinParams& p, int m, int n
     if (n + e >= p.N) break;
     float u = e == 0 ? v.x : e == 1 ? v.y : e == 2 ? v.z : v.w;
     const int64_t at = (int64_t)m * p.ldy + n + e;
-    if (p.z) DT<T>::store1(static_cast<T*>(p.z) + (int64_t)m * p.ldz + n + e, u);
+    if (p.z) DT<T>::store1(static_cast<T*>(p.z) + (int64_t)m * p.ldz + n + e, lin_kept<T>(u));
     u = lin_act<T>(u, p.act);
     if (p.r) u += DT<T>::load1(static_cast<const T*>(p.r) + (int64_t)m * p.ldr + n + e);
     DT<T>::store1(static_cast<T*>(p.y) + at, u);
@@ -410,7 +427,7 @@ __global__ __launch_bounds__(WM * WN * 64) void lin_gemm_kernel(const LinParams 
         for (int k = 0; k < 4; ++k) {
           f32x4 v = value(x + k * ROWS);
           const bool in = there(x + k * ROWS);
-          if (p.z) oz.store4(down + x + k * ROWS, quad, in, v);
+          if (p.z) oz.store4(down + x + k * ROWS, quad, in, lin_kept4<T>(v));
           v = lin_act4<T>(v, p.act);
           if constexpr (RES) v += now[k];
           oy.store4(down + x + k * ROWS, quad, in, v);

@@ -109,3 +109,33 @@ def test_a_captured_forward_follows_the_weights():
             graph.replay()
             torch.cuda.synchronize()
         assert torch.equal(out, want)
+
+
+# ------------------------------------------------------------------------------------------------------------- what 16 bits cannot hold
+@pytest.mark.parametrize("rows", [2, 40, 700])
+@pytest.mark.parametrize("n", [64, 37])
+def test_linear_keeps_a_finite_argument_with_its_sign(rows, n):
+    """fp16: arguments of the activation past 65504 and below half of 2^-24.  The gradients are those of the activation's flat and straight ends and of ReLU's open side."""
+    K = 64
+    x, dy = torch.zeros(rows, K, device="cuda", dtype=torch.float16), torch.full((rows, n), 0.125, device="cuda", dtype=torch.float16)
+    w = torch.zeros(n, K, device="cuda", dtype=torch.float16)
+    x[:, 0], x[:, 1:3], w[:, 0], w[:, 1:3] = 60000.0, 100.0, 1.0, 100.0        # z = 60000 + 2e4 = 8e4, or -8e4
+    for sign, slope in ((1.0, 1.0), (-1.0, 0.0)):
+        leaves = [(x * sign).requires_grad_(True), w.clone().requires_grad_(True)]
+        for act, one in (("SILU", slope), ("RELU", slope), ("SIGMOID", 0.0)):
+            dx, dw = torch.autograd.grad(M.linear(*leaves, None, getattr(L, "ACT_" + act)), leaves, dy)
+            assert torch.isfinite(dx).all() and torch.isfinite(dw[:, 1:]).all(), (act, sign)            # (dw's first column: rows * 60000 / 8, past fp16's range from 9 rows on)
+            assert torch.equal(dx[:, 0], torch.full_like(dx[:, 0], one * n / 8)) and torch.equal(dw[:, 1], torch.full_like(dw[:, 1], one * sign * rows * 12.5)), (act, sign)
+    x = torch.full((rows, K), 2.0 ** -14, device="cuda", dtype=torch.float16)
+    w = torch.zeros(n, K, device="cuda", dtype=torch.float16)
+    w[:, 0] = 2.0 ** -12                                                       # z = 2^-26, which fp16 rounds to 0
+    for sign in (1.0, -1.0):
+        leaves = [(x * sign).requires_grad_(True), w.clone().requires_grad_(True)]
+        y, z = ops.linear_forward(leaves[0].detach(), w, None, L.ACT_RELU, None, True)
+        dx, _ = torch.autograd.grad(M.linear(*leaves, None, L.ACT_RELU), leaves, dy)
+        assert not y.any() and bool((z * sign > 0).all())
+        assert torch.equal(dx[:, 0], torch.full_like(dx[:, 0], n * 2.0 ** -15 if sign > 0 else 0.0))
+    x = x.clone()
+    x[0, 0], x[1, 0] = float("nan"), float("inf")                              # what is not finite stays so
+    z = ops.linear_forward(x, w, None, L.ACT_RELU, None, True)[1]
+    assert torch.isnan(z[0]).all() and torch.isposinf(z[1]).all()
