@@ -310,6 +310,13 @@ __device__ __forceinline__ float pick(uint32_t all, float set, float v) {
   return __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, set) & all) | (__builtin_bit_cast(uint32_t, v) & ~all));
 }
 
+// fp16 holds a probability with all its bits only from 2^-14 on, and rows of some ten thousand keys are below that: where P is an operand on its own (dV), it is carried
+// 2^15 times as large (at most 32768; in the exponent, the row's statistics and the result's scale, which costs nothing).
+template <typename T>
+constexpr float P_UP = DT<T>::code == MOY_F16 ? 32768.f : 1.f;
+template <typename T>
+constexpr float P_UP_LOG2 = DT<T>::code == MOY_F16 ? 15.f : 0.f;
+
 // keys (backward of dK, dV: queries) of an LDS tile
 template <typename T, int DP>
 constexpr int attn_bk() { return sizeof(T) * DP <= 128 ? 64 : 32; }
@@ -973,7 +980,8 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(const AttnParams p) {
       const int ii = i + tid % BQ;
       const float* src = tid < BQ ? p.lse : p.delta;
       st = ii < p.Lq ? src[((int64_t)b * p.H + h) * p.Lq + ii] : 0.f;
-      if (tid < BQ && (ii >= p.Lq || st == -INFINITY)) st = INFINITY;          // no such row, or an empty one: every probability 0
+      if (tid < BQ) st = ii >= p.Lq || st == -INFINITY ? INFINITY : st - P_UP_LOG2<T>;   // no such row, or an empty one: every probability 0
+      else st *= 1.f / P_UP<T>;
     }
   };
   auto keep = [&](int t) {
@@ -1044,7 +1052,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(const AttnParams p) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             s[qq][n][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[qq][n][e], p.scale2, add[e]));
-            w[qq][n][e] = s[qq][n][e] * (w[qq][n][e] - dd[e]);
+            w[qq][n][e] = s[qq][n][e] * __builtin_fmaf(w[qq][n][e], 1.f / P_UP<T>, -dd[e]);
           }
           if (cut) {
             const uint32_t off = j >= sp.klen ? 15u : p.causal ? ~past_bits(j - pos) : 0u;   // (bit e: the key lies behind query e)
@@ -1084,7 +1092,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(const AttnParams p) {
     for (int d = 0; d < DT16; ++d)
       if (d * 16 + g * 4 < p.D) {
         if (p.dk) DT<T>::store4(static_cast<T*>(p.dk) + at + d * 16, dk[d][n] * p.scale);
-        if (p.dv) DT<T>::store4(static_cast<T*>(p.dv) + at + d * 16, dv[d][n]);
+        if (p.dv) DT<T>::store4(static_cast<T*>(p.dv) + at + d * 16, dv[d][n] * (1.f / P_UP<T>));
       }
   }
 }

@@ -139,3 +139,23 @@ def test_linear_keeps_a_finite_argument_with_its_sign(rows, n):
     x[0, 0], x[1, 0] = float("nan"), float("inf")                              # what is not finite stays so
     z = ops.linear_forward(x, w, None, L.ACT_RELU, None, True)[1]
     assert torch.isnan(z[0]).all() and torch.isposinf(z[1]).all()
+
+
+def test_attention_gradient_of_values_under_small_weights():
+    """fp16, 40000 keys: weights of some 2^-15 and less keep all their bits on the way into dV (incoming gradients carry the usual loss scale)."""
+    gen = gen_of(8)
+    B, Lq, Lk, H, D = 1, 3, 40000, 2, 64
+    q, k, v, do = rand(gen, B, Lq, H, D, dtype=torch.float16), rand(gen, B, Lk, H, D, dtype=torch.float16), rand(gen, B, Lk, H, D, dtype=torch.float16), rand(
+        gen, B, Lq, H, D, dtype=torch.float16, scale=1024.0)
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    dv = torch.autograd.grad(M.biased_attention(*leaves, q_start=0), v, do)[0]
+    u = half_step(torch.float16)                                               # (a row's sum: 64 splits of four waves, 40 additions in a lane: chains below 128)
+    for h in range(H):
+        qd, kd, g = q[0, :, h].detach().double(), k[0, :, h].detach().double(), do[0, :, h].double()
+        s = qd @ kd.t() * D ** -0.5
+        p = torch.softmax(s, -1)
+        rel = U32 * (2 * (D + 8) * (qd.abs() @ kd.abs().t() * D ** -0.5).amax(-1, keepdim=True) + 2 * s.abs().amax(-1, keepdim=True) + 128)
+        want = p.t() @ g
+        tol = (p * (u + rel + Lq * U32)).t() @ g.abs() * (1 + u) + u * want.abs() + tiny(torch.float16)
+        bad = (dv[0, :, h].double() - want).abs() / tol
+        assert float(bad.max()) <= 1.0, float(bad.max())
