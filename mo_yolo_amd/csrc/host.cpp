@@ -2,6 +2,7 @@
 // step calls them from autograd's own thread, where each Python operation costs several times its usual price (forward and gradient of a small layer
 // norm: 118 us through Python functions, 67 us here, of which autograd itself takes 51).  Arguments have been checked by mo_yolo_amd.ops; the entry points of
 // the C ABI (include/moyolo.h) are handed over as addresses, so that whichever build of the library is loaded is the one that is called.
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -93,7 +94,15 @@ struct Wants {
   bool operator()(bool given) { return given && ctx->needs_input_grad(next++); }
 };
 
+// Forward-mode derivatives: no operator here has one, and a tangent that is dropped would be taken for zero by whatever comes after.
+void no_tangents(std::initializer_list<const Tensor*> ts) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  for (const Tensor* t : ts)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(/*level=*/0).defined(), "this operator has no forward-mode derivative (a tensor given to it has a tangent)");
+}
+
 bool wants_grad(std::initializer_list<const Tensor*> ts) {
+  no_tangents(ts);
   if (!at::GradMode::is_enabled()) return false;
   for (const Tensor* t : ts)
     if (t->defined() && t->requires_grad()) return true;
@@ -147,6 +156,7 @@ struct NormNode : torch::autograd::Function<NormNode> {
     return y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    no_tangents({&grads[0]});
     const auto s = ctx->get_saved_variables();
     const int64_t how = ctx->saved_data["how"].toInt();
     Wants wants{ctx};
@@ -214,6 +224,7 @@ struct LinearNode : torch::autograd::Function<LinearNode> {
     return y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    no_tangents({&grads[0]});
     const auto s = ctx->get_saved_variables();
     const int64_t how = ctx->saved_data["how"].toInt();
     Wants wants{ctx};
@@ -331,6 +342,7 @@ struct AttentionNode : torch::autograd::Function<AttentionNode> {
     return o;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    no_tangents({&grads[0]});
     const auto s = ctx->get_saved_variables();
     const int64_t how = ctx->saved_data["how"].toInt();
     Wants wants{ctx};

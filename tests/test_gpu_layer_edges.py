@@ -159,3 +159,30 @@ def test_attention_gradient_of_values_under_small_weights():
         tol = (p * (u + rel + Lq * U32)).t() @ g.abs() * (1 + u) + u * want.abs() + tiny(torch.float16)
         bad = (dv[0, :, h].double() - want).abs() / tol
         assert float(bad.max()) <= 1.0, float(bad.max())
+
+
+# ------------------------------------------------------------------------------------------------------ other ways to differentiate and to record
+def calls(gen, dtype=torch.float32):
+    """The three operators as functions of their leaves, and the leaves."""
+    x, w, b, W, B = (rand(gen, *s, dtype=dtype) for s in ((6, 64), (64,), (64,), (48, 64), (48,)))
+    q, k, v, t, lut = *(rand(gen, 2, 5, 2, 32, dtype=dtype) for _ in range(3)), rand(gen, 8, 2, dtype=dtype), ops.relative_buckets(8, 8)
+    return [(lambda x, w, b, r: M.layer_norm(x, w, b, residual=r), (x, w, b, x * 0.5)), (lambda x, w, b, r: M.linear(x, w, b, L.ACT_SILU, r), (x, W, B, x[:, :48] * 0.5)),
+            (lambda q, k, v, t: M.biased_attention(q, k, v, t, lut, q_start=0), (q, k, v, t))]
+
+
+def test_forward_mode_is_refused():
+    """A tangent on any argument, whether its primal wants a gradient or not, is an error and never dropped; so is one on the gradient that comes in."""
+    from torch.autograd import forward_ad as fw
+    for f, args in calls(gen_of(1)):
+        for n in range(len(args)):
+            for wants in (False, True):
+                with fw.dual_level():
+                    some = [fw.make_dual(a.clone().requires_grad_(wants), torch.ones_like(a)) if i == n else a for i, a in enumerate(args)]
+                    with pytest.raises(RuntimeError, match="forward-mode|jvp"):
+                        f(*some)
+                    with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode|jvp"):
+                        f(*some)
+        every = [a.clone().requires_grad_(True) for a in args]
+        y = f(*every)
+        with fw.dual_level(), pytest.raises(RuntimeError, match="forward-mode|jvp"):
+            torch.autograd.grad(y, every, fw.make_dual(torch.ones_like(y), torch.ones_like(y)))

@@ -1,9 +1,10 @@
 """CPU: host-side rules of the transformer-layer operators and modules at their edges (no launch)."""
 import copy
 
+import pytest
 import torch
 
-from mo_yolo_amd import modules
+from mo_yolo_amd import _lib, modules, ops
 
 
 # ---------------------------------------------------------------------------------------------------------------- prepared weights
@@ -68,3 +69,22 @@ def test_the_differentiable_forms_say_that_they_train():
         assert "self._trains()" in inspect.getsource(cls.forward_train)
     held = [m for top in (modules.MOTRDecoderLayer(), modules.QueryInteractionModule(None, 256, 256)) for m in top.modules() if isinstance(m, modules._ParamModule)]
     assert held and all(isinstance(m, (modules._Linear, modules._MHA)) for m in held)
+
+
+# ------------------------------------------------------------------------------------------------------ other ways to differentiate and to record
+def _host_calls():
+    """The differentiable entry points of the host side, past the checks that want a GPU: they refuse before they look at a device."""
+    h, x, w = _lib.host(), torch.ones(6, 8), torch.ones(8)
+    q, t, lut = torch.ones(2, 5, 2, 8), torch.ones(8, 2), ops.relative_buckets(8, 8, device="cpu")
+    return [(lambda x, w, b, r: h.layer_norm(x, w, b, 1e-5, r), (x, w, w.clone(), x.clone())), (lambda x, w, b, r: h.linear(x, w, b, _lib.ACT_SILU, r), (x, x.clone(), torch.ones(6), torch.ones(6, 6))),
+            (lambda q, k, v, t: h.attention(q, k, v, t, lut, None, None, False, False, 0, 1.0), (q, q.clone(), q.clone(), t))]
+
+
+def test_forward_mode_is_refused():
+    """A tangent is never dropped, on whichever argument it is and whether or not gradients are computed."""
+    from torch.autograd import forward_ad as fw
+    for f, args in _host_calls():
+        for n in range(len(args)):
+            for grad in (True, False):
+                with fw.dual_level(), torch.set_grad_enabled(grad), pytest.raises(NotImplementedError, match="forward-mode"):
+                    f(*[fw.make_dual(a, torch.ones_like(a)) if i == n else a for i, a in enumerate(args)])
