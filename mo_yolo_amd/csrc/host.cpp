@@ -4,8 +4,10 @@
 // the C ABI (include/moyolo.h) are handed over as addresses, so that whichever build of the library is loaded is the one that is called.
 #include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
 #include "../../include/moyolo.h"
@@ -43,8 +45,16 @@ int64_t check(int64_t rc, const char* what) {
 
 int code_of(at::ScalarType t) { return t == at::kFloat ? MOY_F32 : t == at::kBFloat16 ? MOY_BF16 : MOY_F16; }
 
+// What records torch's operations (torch.jit.trace, make_fx) sees the outputs made and not the launches that fill them: a replay would return memory that nothing wrote.
+bool not_recorded() {
+  TORCH_CHECK(!torch::jit::tracer::isTracing() && !c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value(),
+              "the transformer-layer operators launch kernels of their own and cannot be recorded by torch.jit.trace or make_fx");
+  return true;
+}
+
 // the tensor's device as the current one, and its current stream
 struct On {
+  bool live = not_recorded();
   at::AutoGradMode plain{false};           // (layout copies are no part of a graph)
   c10::OptionalDeviceGuard guard;
   void* stream;

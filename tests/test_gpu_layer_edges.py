@@ -186,3 +186,16 @@ def test_forward_mode_is_refused():
         y = f(*every)
         with fw.dual_level(), pytest.raises(RuntimeError, match="forward-mode|jvp"):
             torch.autograd.grad(y, every, fw.make_dual(torch.ones_like(y), torch.ones_like(y)))
+
+
+@pytest.mark.filterwarnings("ignore")
+def test_recording_a_trace_is_refused():
+    """A recorder that keeps torch's operations and not the launches would keep an output that nothing writes."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    for f, args in calls(gen_of(2)):
+        with pytest.raises(RuntimeError, match="recorded"):
+            torch.jit.trace(f, args, check_trace=False)
+        with pytest.raises(RuntimeError, match="recorded"):
+            make_fx(f)(*args)
+        y = f(*args)
+        assert torch.isfinite(y).all()

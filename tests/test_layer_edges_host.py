@@ -88,3 +88,13 @@ def test_forward_mode_is_refused():
             for grad in (True, False):
                 with fw.dual_level(), torch.set_grad_enabled(grad), pytest.raises(NotImplementedError, match="forward-mode"):
                     f(*[fw.make_dual(a, torch.ones_like(a)) if i == n else a for i, a in enumerate(args)])
+
+
+@pytest.mark.filterwarnings("ignore")
+def test_recording_a_trace_is_refused():
+    from torch.fx.experimental.proxy_tensor import make_fx
+    for f, args in _host_calls():
+        with pytest.raises(RuntimeError, match="recorded"):
+            torch.jit.trace(f, args, check_trace=False)
+        with pytest.raises(RuntimeError, match="recorded"):
+            make_fx(f)(*args)
