@@ -74,7 +74,7 @@ Tensor as_rows(const Tensor& t) {
   Tensor r = t.dim() == 2 ? t : t.reshape({t.numel() / t.size(-1), t.size(-1)});
   return r.stride(1) == 1 || r.size(1) == 1 ? r : r.contiguous();
 }
-int64_t row_stride(const Tensor& t) { return t.defined() ? t.stride(0) : 0; }
+int64_t row_stride(const Tensor& t) { return !t.defined() ? 0 : t.size(0) == 1 ? t.size(1) : t.stride(0); }   // (of a single row: its length, whatever it says)
 Tensor dense(const Tensor& t) { return t.defined() ? t.contiguous() : t; }
 
 // The gradients of a node whose backward has none of its own: where a graph of them is asked for (create_graph), they hang by a node that raises on what they
@@ -128,7 +128,7 @@ std::tuple<Tensor, Tensor> norm_forward(const Tensor& x, const Tensor& w, const 
   if (rows) {
     float* at = stats ? stat.data_ptr<float>() : nullptr;
     const int wcode = wc.defined() ? code_of(wc.scalar_type()) : bc.defined() ? code_of(bc.scalar_type()) : MOY_F32;
-    check(lib.norm(x2.data_ptr(), x2.stride(0), ptr(r2), row_stride(r2), ptr(wc), ptr(bc), wcode, rows, (int)c, (float)eps, y.data_ptr(), c, at,
+    check(lib.norm(x2.data_ptr(), row_stride(x2), ptr(r2), row_stride(r2), ptr(wc), ptr(bc), wcode, rows, (int)c, (float)eps, y.data_ptr(), c, at,
                    at ? at + rows : nullptr, code_of(x.scalar_type()), on.stream),
           "moy_layer_norm");
   }
@@ -149,7 +149,7 @@ std::tuple<Tensor, Tensor, Tensor> norm_backward(const Tensor& dy, const Tensor&
     const int64_t n = need_w || need_b ? check(lib.norm_bwd_ws(rows, (int)c, code), "moy_layer_norm_bwd_ws") : 0;
     Tensor ws = floats(n, x);
     float* at = stat.data_ptr<float>();
-    check(lib.norm_bwd(g2.data_ptr(), g2.stride(0), x2.data_ptr(), x2.stride(0), ptr(r2), row_stride(r2), ptr(wc), code_of(wtype), at, at + rows, rows, (int)c,
+    check(lib.norm_bwd(g2.data_ptr(), row_stride(g2), x2.data_ptr(), row_stride(x2), ptr(r2), row_stride(r2), ptr(wc), code_of(wtype), at, at + rows, rows, (int)c,
                        ptr(dx), c, ptr(dw), ptr(db), (float*)ptr(ws), n, code, on.stream),
           "moy_layer_norm_bwd");
   }
@@ -177,18 +177,37 @@ struct NormNode : torch::autograd::Function<NormNode> {
 };
 
 // ---------------------------------------------------------------------------------------------------------------------- linear
+// The rows of x, w, r and dy may lie at any distance.  The entry points take the strides of a view where their kernels' offsets reach (4 MiB from row to row, and any
+// stride of a single row or of a few rows going forward) and refuse others as MOY_ENOSYS: those operands are copied to dense rows, and the call is made again.
 struct LinearCall {
   moy_linear_args a{};
-  Tensor x, w, b, r;
-  LinearCall(const Tensor& x_, const Tensor& w_, const Tensor& b_, int64_t act, const Tensor& r_) : x(as_rows(x_)), w(as_rows(w_)), b(dense(b_)), r(as_rows(r_)) {
-    a.x = x.data_ptr(); a.ldx = x.stride(0); a.w = w.data_ptr(); a.ldw = w.stride(0); a.act = (int)act; a.dtype = code_of(x.scalar_type());
+  Tensor x, w, b, r, dy;
+  LinearCall(const Tensor& x_, const Tensor& w_, const Tensor& b_, int64_t act, const Tensor& r_, const Tensor& dy_ = Tensor())
+      : x(as_rows(x_)), w(as_rows(w_)), b(dense(b_)), r(as_rows(r_)), dy(as_rows(dy_)) {
+    a.act = (int)act; a.dtype = code_of(x.scalar_type());
     a.M = (int)x.size(0); a.N = (int)w.size(0); a.K = (int)w.size(1);
     a.b = ptr(b); a.b_dtype = b.defined() ? code_of(b.scalar_type()) : MOY_F32;
-    a.r = ptr(r); a.ldr = row_stride(r);
+    place();
+  }
+  void place() {
+    a.x = x.data_ptr(); a.ldx = row_stride(x); a.w = w.data_ptr(); a.ldw = row_stride(w);
+    a.r = ptr(r); a.ldr = row_stride(r); a.dy = ptr(dy); a.ldd = row_stride(dy);
+  }
+  bool compact() {
+    bool any = false;
+    for (Tensor* t : {&x, &w, &r, &dy})
+      if (t->defined() && !t->is_contiguous()) {
+        *t = t->contiguous();
+        any = true;
+      }
+    place();
+    return any;
   }
   template <typename Query, typename Launch>
   void run(Query query, Launch launch, const char* what, void* stream) {
-    const int64_t n = check(query(&a), what);
+    int64_t n = query(&a);
+    if (n == MOY_ENOSYS && compact()) n = query(&a);
+    check(n, what);
     Tensor ws = n ? at::empty({n}, x.options().dtype(at::kByte)) : Tensor();
     a.ws = ptr(ws); a.ws_len = n;
     check(launch(&a, stream), what);
@@ -211,15 +230,14 @@ std::tuple<Tensor, Tensor> linear_forward(const Tensor& x, const Tensor& w, cons
 std::tuple<Tensor, Tensor, Tensor> linear_backward(const Tensor& dy, const Tensor& x, const Tensor& w, const Tensor& z, int64_t act, bool need_x, bool need_w,
                                                    bool need_b, at::ScalarType btype) {
   const On on(x);
-  LinearCall c(x, w, Tensor(), act, Tensor());
+  LinearCall c(x, w, Tensor(), act, Tensor(), dy);
   c.a.b_dtype = code_of(btype);
   Tensor dx = made(need_x, x.sizes(), x, x.scalar_type()), dw = made(need_w, w.sizes(), x, x.scalar_type()), db = made(need_b, {c.a.N}, x, btype);
   if (c.a.M == 0) {
     if (need_w) dw.zero_();
     if (need_b) db.zero_();
   } else if (need_x || need_w || need_b) {
-    const Tensor g = as_rows(dy);
-    c.a.dy = g.data_ptr(); c.a.ldd = g.stride(0); c.a.z = ptr(z); c.a.dx = ptr(dx); c.a.dw = ptr(dw); c.a.db = ptr(db);
+    c.a.z = ptr(z); c.a.dx = ptr(dx); c.a.dw = ptr(dw); c.a.db = ptr(db);
     c.run(lib.linear_bwd_ws, lib.linear_bwd, "moy_linear_bwd", on.stream);
   }
   return {dx, dw, db};

@@ -689,17 +689,20 @@ static int lin_check(const moy_linear_args* a, bool bwd) {
   if (a->act < MOY_ACT_NONE || a->act > MOY_ACT_SIGMOID || (a->b_dtype != MOY_F32 && a->b_dtype != a->dtype)) return MOY_EINVAL;
   const int d = a->dtype;
   if (!a->x || !a->w || !aligned_as(a->x, d) || !aligned_as(a->w, d) || (a->M > 1 && a->ldx < 0) || (a->N > 1 && a->ldw < 0)) return MOY_EINVAL;
-  if (a->ldx * lin_es(d) > (1 << 22) || a->ldw * lin_es(d) > (1 << 22) || (int64_t)a->K * lin_es(d) > (1 << 22) || (int64_t)a->N * lin_es(d) > (1 << 22)) return MOY_ENOSYS;
+  // rows up to 4 MiB long, and no further apart where the tiled kernel addresses them (by 32-bit offsets within a tile); lin_few_kernel takes any distance
+  const bool few = !bwd && lin_few(a->M);
+  auto apart = [&](int64_t ld, int rows) { return !few && rows > 1 && ld > (1 << 22) / lin_es(d); };
+  if ((int64_t)a->K * lin_es(d) > (1 << 22) || (int64_t)a->N * lin_es(d) > (1 << 22) || apart(a->ldx, a->M) || apart(a->ldw, a->N)) return MOY_ENOSYS;
   if ((int64_t)((a->M + 63) / 64) * ((a->N + 63) / 64) * 16 > 0x7fffffffLL || (int64_t)((a->M + 63) / 64) * ((a->K + 63) / 64) * 16 > 0x7fffffffLL) return MOY_ENOSYS;
   if ((int64_t)a->M * (a->N > a->K ? a->N : a->K) / 4 / 256 > 0x3fffffffLL) return MOY_ENOSYS;
   if (!bwd) {
-    if (a->ldy * lin_es(d) > (1 << 22) || a->ldr * lin_es(d) > (1 << 22)) return MOY_ENOSYS;
+    if (apart(a->ldy, a->M) || (a->r && apart(a->ldr, a->M))) return MOY_ENOSYS;
     if (!a->y || !aligned_as(a->y, d) || (a->M > 1 && a->ldy < a->N) || !aligned_as(a->b, a->b_dtype)) return MOY_EINVAL;
     if (!aligned_as(a->r, d) || (a->r && a->M > 1 && a->ldr < 0) || !aligned_as(a->z, d)) return MOY_EINVAL;
   } else {
     if (!a->dy || !aligned_as(a->dy, d) || (a->M > 1 && a->ldd < 0) || (!a->dx && !a->dw && !a->db)) return MOY_EINVAL;
     if ((a->act != MOY_ACT_NONE && !a->z) || !aligned_as(a->z, d) || !aligned_as(a->dx, d) || !aligned_as(a->dw, d) || !aligned_as(a->db, a->b_dtype)) return MOY_EINVAL;
-    if (a->ldd * lin_es(d) > (1 << 22)) return MOY_ENOSYS;
+    if (apart(a->ldd, a->M)) return MOY_ENOSYS;
   }
   return MOY_OK;
 }

@@ -199,3 +199,32 @@ def test_recording_a_trace_is_refused():
             make_fx(f)(*args)
         y = f(*args)
         assert torch.isfinite(y).all()
+
+
+# ------------------------------------------------------------------------------------------------------------------------ strides
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_linear_takes_rows_that_lie_far_apart(dtype):
+    """The last token of each sequence (rows over 4 MiB apart) as x, residual, incoming gradient and weight: as from dense copies, bit for bit."""
+    dt, gen = DT[dtype], gen_of(3)
+    K, N = 256, 192
+    step = (1 << 22) // (K * torch.finfo(dt).bits // 8) + 3                    # rows to a sequence
+    for rows in (1, 2, 40):
+        h = torch.empty(rows, step, K, device="cuda", dtype=dt)
+        h[:, -1] = rand(gen, rows, K, dtype=dt)
+        x, w, b = h[:, -1], rand(gen, N, K, dtype=dt, scale=K ** -0.5), rand(gen, N, dtype=dt)
+        rr, gg = (torch.empty(rows, step + 99, N + 64, device="cuda", dtype=dt) for _ in range(2))
+        rr[:, -1], gg[:, -1] = rand(gen, rows, N + 64, dtype=dt), rand(gen, rows, N + 64, dtype=dt)
+        r, dy = rr[:, -1, 64:], gg[:, -1, 64:]
+        assert rows == 1 or min(x.stride(0), r.stride(0), dy.stride(0)) * x.element_size() > 1 << 22
+        runs = []
+        for xs, rs, ds in ((x, r, dy), (x.clone(), r.clone(), dy.clone())):
+            leaves = [t.detach().requires_grad_(True) for t in (xs, w, b, rs)]
+            y = M.linear(leaves[0], *leaves[1:3], L.ACT_SILU, leaves[3])
+            runs.append((y, ops.linear_forward(xs, w, b, L.ACT_SILU, rs), *torch.autograd.grad(y, leaves, ds)))
+        for a, c in zip(*runs):
+            assert torch.isfinite(a).all() and torch.equal(a, c)
+        assert torch.equal(ops.linear_forward(w, x), ops.linear_forward(w, x.clone()))                # ... as the weight
+        g = rand(gen, N, rows, dtype=dt)
+        for a, c in zip(ops.linear_backward(g, w, x, need=(True, True, False)), ops.linear_backward(g, w, x.clone(), need=(True, True, False))):
+            assert a is c is None or torch.equal(a, c)
+        assert torch.equal(ops.layer_norm_forward(x), ops.layer_norm_forward(x.clone()))

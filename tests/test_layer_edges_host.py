@@ -1,5 +1,6 @@
 """CPU: host-side rules of the transformer-layer operators and modules at their edges (no launch)."""
 import copy
+import ctypes as C
 
 import pytest
 import torch
@@ -98,3 +99,28 @@ def test_recording_a_trace_is_refused():
             torch.jit.trace(f, args, check_trace=False)
         with pytest.raises(RuntimeError, match="recorded"):
             make_fx(f)(*args)
+
+
+# ------------------------------------------------------------------------------------------------------------------------ strides
+def test_linear_strides_that_the_entry_points_take():
+    """Rows over 4 MiB apart: where there is one, or few going forward; the workspace queries answer as the calls do."""
+    def query(bwd=False, **kw):
+        a = _lib.LinearArgs()
+        a.x = a.w = a.y = 0x10000
+        a.M, a.N, a.K, a.ldx, a.ldw, a.ldy, a.dtype = 1, 64, 4096, 4096, 4096, 64, _lib.BF16
+        if bwd:
+            a.dy = a.dx = a.dw = 0x10000
+            a.ldd = 64
+        for n, x in kw.items():
+            setattr(a, n, x)
+        return (_lib.lib().moy_linear_bwd_ws if bwd else _lib.lib().moy_linear_ws)(C.byref(a))
+    far = 513 * 4096                                                           # elements of 16 bits: 4 KiB over the limit
+    for kw in (dict(ldx=far), dict(ldx=1 << 40, ldy=1 << 40, r=0x10000, ldr=1 << 40), dict(M=2, ldx=far), dict(M=32, ldx=1 << 33, ldw=1 << 33), dict(M=40, N=1, ldw=1 << 40)):
+        assert query(**kw) >= 0, kw
+    assert query(True, ldx=1 << 40, ldd=1 << 40) >= 0 and query(True, M=40, N=1, ldw=1 << 40) >= 0
+    for kw in (dict(ldx=far), dict(ldw=far), dict(ldy=far), dict(r=0x10000, ldr=far)):
+        assert query(M=33, **kw) == _lib.ENOSYS, kw
+    for kw in (dict(ldx=far), dict(ldw=far), dict(ldd=far)):
+        assert query(True, M=2, **kw) == _lib.ENOSYS, kw
+    assert query(M=33, ldr=far) >= 0                                           # (no residual)
+    assert query(M=33, ldx=512 * 4096) >= 0 and query(K=1 << 22, ldx=1 << 22, ldw=1 << 22) == _lib.ENOSYS
