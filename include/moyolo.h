@@ -630,8 +630,9 @@ int64_t moy_layer_norm_bwd_ws(int64_t rows, int C, int dtype);    /* floats, or 
  * table T [num_buckets <= 64, H] with lut uint8 [2 max_distance + 1] (device; entries past num_buckets count as the last), max_distance <= 1024; both NULL: no
  * bias.  Key j counts iff j < k_len[b] (int32 [B], device, clamped to [0, Lk]; NULL: Lk), and j <= i + start if causal, and mask (uint8, strides m_sb,
  * m_sh, m_sq, key stride 1; NULL: none) is 0 there.  start = q_start, or with q_from_end k_len[b] - Lq (the queries are the last tokens of the cache).
- * Rows of k / v from k_len on are not read, nor those that a mask without query and head strides (m_sq == m_sh == 0) hides; a key that such a rule does not
- * hide has to be finite wherever any query counts it or not (its weight 0 still multiplies it).
+ * Rows of k / v from k_len on are not read, nor those that a mask without query and head strides (m_sq == m_sh == 0) hides; with causal, rows behind the last
+ * query's position are not read either.  A key that such a rule does not hide has to be finite wherever any query counts it or not (its weight 0 still
+ * multiplies it).
  * ws: fp32 workspace of moy_attention_ws / moy_attention_bwd_ws floats (0: none needed; negative: a MOY_E* code).
  * Backward: dout T [B, Lq, H, D] strided (g_*), the forward's o and lse; dq dense like o, dk / dv dense [B, Lk, Hk, D] (zeros from k_len on), dtable T
  * [num_buckets, H]; each optional, one at least given.  16-bit types: the forward's P enters its product as two operands (its rounded value and the

@@ -343,7 +343,7 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(const AttnParams p) {
   const T* vb = static_cast<const T*>(p.v) + b * p.v_sb + hk * p.v_sh;
   const int q0 = qt * BQ + wave * 16 * NQ;                                      // the wave's first query
   const int last = min(qt * BQ + BQ, p.Lq) - 1 + sp.start;                      // position of the block's last query
-  const int kend = p.causal ? min(sp.klen, last + 1) : sp.klen;
+  const int kend = p.causal ? min(sp.klen, last + 1) : sp.klen;                // (no query of the block sees a key from here on: not read)
   const int nt = kend > 0 ? (kend + BK - 1) / BK : 0;
 
   Frag<T> qf[NQ][KP];
@@ -366,8 +366,8 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(const AttnParams p) {
   TL kr, vr;
   ML mr;
   if (nt > 0) {
-    kr.load(kb, p.k_sl, 0, sp.klen, p.D, MASK ? sp.hide : nullptr, tid);
-    vr.load(vb, p.v_sl, 0, sp.klen, p.D, MASK ? sp.hide : nullptr, tid);
+    kr.load(kb, p.k_sl, 0, kend, p.D, MASK ? sp.hide : nullptr, tid);
+    vr.load(vb, p.v_sl, 0, kend, p.D, MASK ? sp.hide : nullptr, tid);
     if constexpr (MASK) mr.load(sp.mask, sp.m_sq, qt * BQ, p.Lq, 0, p.Lk, tid);
     if (p.table) load_bias<T>(p, h, bias, 256);
     kr.store(kt_, tid);
@@ -381,8 +381,8 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(const AttnParams p) {
     const uint32_t* ms = mt_ + (t & 1) * (ML::BYTES / 4);
     const int j0 = t * BK;
     if (t + 1 < nt) {
-      kr.load(kb, p.k_sl, j0 + BK, sp.klen, p.D, MASK ? sp.hide : nullptr, tid);
-      vr.load(vb, p.v_sl, j0 + BK, sp.klen, p.D, MASK ? sp.hide : nullptr, tid);
+      kr.load(kb, p.k_sl, j0 + BK, kend, p.D, MASK ? sp.hide : nullptr, tid);
+      vr.load(vb, p.v_sl, j0 + BK, kend, p.D, MASK ? sp.hide : nullptr, tid);
       if constexpr (MASK) mr.load(sp.mask, sp.m_sq, qt * BQ, p.Lq, j0 + BK, p.Lk, tid);
     }
     f32x4 s[NKT][NQ];
@@ -557,12 +557,12 @@ __global__ __launch_bounds__(256, 2) void attn_split_kernel(const AttnParams p) 
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt) {
       const int j = j0 + kt * 16 + c;
-      const bool in = j < sp.klen && !(hide && hide[j]);
+      const bool in = j < kall && !(hide && hide[j]);
       const T* kp_ = kb + (int64_t)j * p.k_sl + g * 8;
 #pragma unroll
       for (int kp = 0; kp < KP; ++kp) kf[kt][kp] = in && kp * 32 + g * 8 < p.D ? frag_row(kp_ + kp * 32) : frag_zero<T>();
     }
-    vr.load(vb, p.v_sl, j0, sp.klen, p.D, hide, lane);
+    vr.load(vb, p.v_sl, j0, kall, p.D, hide, lane);
   };
   int j0 = k0 + wave * 32;
   if (j0 < k1) load(j0);
@@ -736,8 +736,8 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(const AttnParams p) {
   TL kr, vr;
   ML mr;
   if (nt > 0) {
-    kr.load(kb, p.k_sl, 0, sp.klen, p.D, MASK ? sp.hide : nullptr, tid);
-    vr.load(vb, p.v_sl, 0, sp.klen, p.D, MASK ? sp.hide : nullptr, tid);
+    kr.load(kb, p.k_sl, 0, kend, p.D, MASK ? sp.hide : nullptr, tid);
+    vr.load(vb, p.v_sl, 0, kend, p.D, MASK ? sp.hide : nullptr, tid);
     if constexpr (MASK) mr.load(sp.mask, sp.m_sq, qt * BQ, p.Lq, 0, p.Lk, tid);
   }
   Frag<T> qf[NQ][KP], gf[NQ][KP];
@@ -795,8 +795,8 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(const AttnParams p) {
     const uint32_t* ms = mt_ + (t & 1) * (ML::BYTES / 4);
     const int j0 = t * BK;
     if (t + 1 < nt) {
-      kr.load(kb, p.k_sl, j0 + BK, sp.klen, p.D, MASK ? sp.hide : nullptr, tid);
-      vr.load(vb, p.v_sl, j0 + BK, sp.klen, p.D, MASK ? sp.hide : nullptr, tid);
+      kr.load(kb, p.k_sl, j0 + BK, kend, p.D, MASK ? sp.hide : nullptr, tid);
+      vr.load(vb, p.v_sl, j0 + BK, kend, p.D, MASK ? sp.hide : nullptr, tid);
       if constexpr (MASK) mr.load(sp.mask, sp.m_sq, qt * BQ, p.Lq, j0 + BK, p.Lk, tid);
     }
     const int p0 = q0 + sp.start, p1 = p0 + 16 * NQ - 1;
@@ -946,13 +946,14 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(const AttnParams p) {
   const int b = bh / p.Hk, hk = bh - b * p.Hk, share = p.H / p.Hk;
   const int jb = jt * BKB, jw = jb + wave * 16 * NK;                           // the block's and the wave's first key
   const Span sp = span_of(p, b, hk * share);
+  const int kall = p.causal ? min(sp.klen, p.Lq + sp.start) : sp.klen;         // (no query sees a key from here on)
   const T* kb = static_cast<const T*>(p.k) + b * p.k_sb + hk * p.k_sh;
   const T* vb = static_cast<const T*>(p.v) + b * p.v_sb + hk * p.v_sh;
   Frag<T> kf[NK][KP], vf[NK][KP];
 #pragma unroll
   for (int n = 0; n < NK; ++n) {
     const int j = jw + n * 16 + c;
-    const bool in = j < sp.klen && !(MASK && sp.hide && p.m_sh == 0 && sp.hide[j]);
+    const bool in = j < kall && !(MASK && sp.hide && p.m_sh == 0 && sp.hide[j]);
 #pragma unroll
     for (int kp = 0; kp < KP; ++kp) {
       const bool on = in && kp * 32 + g * 8 < p.D;

@@ -679,7 +679,8 @@ def attention_forward(q, k, v, table=None, lut=None, *, causal=False, q_start=No
     strides; H a multiple of Hk: shared key heads), D a multiple of 8 up to 128; float32 / bfloat16 / float16.
     table [num_buckets, H] in q's type with lut = relative_buckets(...), or any uint8 map of clamped distances to buckets; none: no bias.
     q_start: position of the first query (keys count from 0); None: the queries are the last of the k_len[b] (or Lk) keys, as with a cache.
-    causal: a query sees keys up to its own position.  k_len int32 [B]: keys that count (rows behind them are not read).  attn_mask bool, True = hidden,
+    causal: a query sees keys up to its own position (rows behind the last query's are not read).  k_len int32 [B]: keys that
+    count (nor are rows behind them).  attn_mask bool, True = hidden,
     [Lq, Lk] or [B, H, Lq, Lk] with axes of 1 where it does not differ; hidden rows of k / v must still be finite, unless the mask differs
     neither by query nor by head.  scale: >= 0, D ** -0.5.  A query that sees no key gets zeros.
     -> o [B, Lq, H, D], or with stats (o, lse, rest) as attention_backward takes them (rest: what the rounding of a 16-bit o left out, else None)."""

@@ -228,3 +228,27 @@ def test_linear_takes_rows_that_lie_far_apart(dtype):
         for a, c in zip(ops.linear_backward(g, w, x, need=(True, True, False)), ops.linear_backward(g, w, x.clone(), need=(True, True, False))):
             assert a is c is None or torch.equal(a, c)
         assert torch.equal(ops.layer_norm_forward(x), ops.layer_norm_forward(x.clone()))
+
+
+# ------------------------------------------------------------------------------------------------------------------------ keys ahead
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("Lq,Lk,D,start", [(20, 200, 64, 10), (1, 3000, 32, 40), (130, 700, 128, 0), (4, 900, 40, 505), (300, 330, 64, 7), (64, 64, 32, -20)])
+def test_keys_ahead_of_every_query_are_not_looked_at(Lq, Lk, D, start, dtype):
+    """Causal attention over a cache that is allocated ahead: what stands behind the last query's position (NaN, infinities) changes nothing and gets zeros."""
+    gen, dt = gen_of(Lq * 7 + Lk), DT[dtype]
+    q, k, v, do = (rand(gen, 2, n, h, D, dtype=dt) for n, h in ((Lq, 4), (Lk, 2), (Lk, 2), (Lq, 4)))
+    table, lut = rand(gen, 16, 4, dtype=dt), ops.relative_buckets(16, 30)
+    how = dict(causal=True, q_start=start)
+    runs = []
+    for fill in (0.0, float("nan"), float("inf")):
+        k2, v2 = k.clone(), v.clone()
+        k2[:, max(0, start + Lq):], v2[:, max(0, start + Lq):] = fill, -fill
+        leaves = [t.clone().requires_grad_(True) for t in (q, k2, v2, table)]
+        y = M.biased_attention(*leaves, lut, **how)
+        with torch.no_grad():
+            assert torch.equal(y, M.biased_attention(*leaves, lut, **how))
+        runs.append((y, *torch.autograd.grad(y, leaves, do)))
+        assert not runs[-1][2][:, max(0, start + Lq):].any() and not runs[-1][3][:, max(0, start + Lq):].any()
+    for got in runs[1:]:
+        for a, b in zip(got, runs[0]):
+            assert torch.isfinite(a).all() and torch.equal(a, b)
