@@ -252,3 +252,123 @@ def test_keys_ahead_of_every_query_are_not_looked_at(Lq, Lk, D, start, dtype):
     for got in runs[1:]:
         for a, b in zip(got, runs[0]):
             assert torch.isfinite(a).all() and torch.equal(a, b)
+
+
+def test_linear_and_norm_offsets_past_32_bits():
+    """Operands and results whose last rows lie past 2^31 elements."""
+    n, pitch, gen = 70000, 40000, gen_of(4)
+    big = torch.empty(n, pitch, device="cuda", dtype=torch.bfloat16)
+    big[:, :192] = rand(gen, n, 192, dtype=torch.bfloat16)
+    x, dy, w = big[:, :64], big[:, 64:192], rand(gen, 128, 64, dtype=torch.bfloat16)
+    y, z = ops.linear_forward(x, w, act=L.ACT_SILU, residual=dy, keep_pre=True)
+    yc, zc = ops.linear_forward(x.clone(), w, act=L.ACT_SILU, residual=dy.clone(), keep_pre=True)
+    assert torch.equal(y, yc) and torch.equal(z, zc)
+    for a, b in zip(ops.linear_backward(dy, x, w, z, L.ACT_SILU), ops.linear_backward(dy.clone(), x.clone(), w, z, L.ACT_SILU)):
+        assert torch.equal(a, b)
+    assert torch.equal(ops.linear_forward(x[-20:], w), ops.linear_forward(x[-20:].clone(), w))
+    y, stat = ops.layer_norm_forward(x, residual=dy[:, :64], stats=True)
+    yc, sc = ops.layer_norm_forward(x.clone(), residual=dy[:, :64].clone(), stats=True)
+    assert torch.equal(y, yc) and torch.equal(stat, sc)
+    for a, b in zip(ops.layer_norm_backward(dy[:, :64], x, None, stat), ops.layer_norm_backward(dy[:, :64].clone(), x.clone(), None, stat)):
+        assert torch.equal(a, b)
+    del big, x, dy, y, z, yc, zc
+    rows = (1 << 21) + 1000                                                    # dense ones of 2^31 elements and more: x, y, z, dy and dx
+    x, w, b = rand(gen, rows, 8, dtype=torch.bfloat16), rand(gen, 1024, 8, dtype=torch.bfloat16), rand(gen, 1024, dtype=torch.bfloat16)
+    y, z = ops.linear_forward(x, w, b, L.ACT_SILU, keep_pre=True)
+    part = torch.cat((torch.arange(500), torch.arange(rows - 1500, rows))).cuda()
+    yc, zc = ops.linear_forward(x[part], w, b, L.ACT_SILU, keep_pre=True)
+    assert y.numel() > 1 << 31 and torch.equal(y[part], yc) and torch.equal(z[part], zc)
+    dx = ops.linear_backward(y, x, w, z, L.ACT_SILU, need=(True, False, False))[0]
+    a, b = dx[part].float(), ops.linear_backward(yc, x[part], w, zc, L.ACT_SILU, need=(True, False, False))[0].float()
+    # (few rows split their sums: a bf16 step, and 1024 fp32 additions of terms that add up to less than 1100 in size)
+    assert bool(((a - b).abs() <= 2.0 ** -7 * b.abs() + 1024 * U32 * 1100).all())
+    s, stat = ops.layer_norm_forward(y, stats=True)
+    sc, tc = ops.layer_norm_forward(yc, stats=True)
+    assert torch.equal(s[part], sc)
+    assert torch.equal(ops.layer_norm_backward(z, y, None, stat, need=(True, False, False))[0][part], ops.layer_norm_backward(zc, yc, None, tc, need=(True, False, False))[0])
+
+
+# ---------------------------------------------------------------------------------------------------- what is not rounded on the way
+def forward_tolerance(y, p, v, rel, n, dt):
+    """Of o and of o + rest where P enters its product as two operands: P errs by its fp32 statistics (rel, n additions) and by the square of a half step (the
+    remainder's own rounding; fp16: no less than half of 2^-24, the reference of the exponentials at most 2^8 below the largest weight); o is rounded once, o + rest by the square of a half step."""
+    u, ya = half_step(dt), p @ v.abs()
+    wide = dt == torch.float32
+    inner = ((0 if wide else u * u) + rel + n * U32) * ya + (tiny(dt) * (p > 0).double() @ v.abs() if dt == torch.float16 else 0)
+    return inner + u * y.abs() + tiny(dt), inner + (u if wide else u * u) * y.abs() + tiny(dt)
+
+
+def tight_reference(q, k, v, do, table, lut, start):
+    """One head in 64 bits: y, dtable, and the tolerances of y and of dtable where nothing but a result is rounded to 16 bits."""
+    dt, (Lq, D), Lk, far = q.dtype, q.shape, k.shape[0], lut.shape[0] // 2
+    qd, kd, vd, g, td = (t.double() for t in (q, k, v, do, table))
+    at = lut.to(q.device).long()[(torch.arange(Lk, device=q.device)[None] - torch.arange(Lq, device=q.device)[:, None] - start).clamp(-far, far) + far]
+    s = qd @ kd.t() * D ** -0.5 + td[at]
+    size = qd.abs() @ kd.abs().t() * D ** -0.5 + td[at].abs()
+    p = torch.softmax(s, -1)
+    rel = U32 * (2 * (D + 8) * size.amax(-1, keepdim=True) + 2 * s.abs().amax(-1, keepdim=True) + Lk + 16)
+    y = p @ vd
+    ty, to = forward_tolerance(y, p, vd, rel, Lk, dt)
+    dp, dpa = g @ vd.t(), g.abs() @ vd.abs().t()
+    delta = (g * y).sum(-1, keepdim=True)
+    ds = p * (dp - delta)
+    off = (g.abs() * to).sum(-1, keepdim=True) + 2 * U32 * (D + 8) * (g.abs() * y.abs()).sum(-1, keepdim=True)
+    te = p * (rel * (dp - delta).abs() + U32 * (D + 8) * dpa + off + 2 * U32 * (dp.abs() + delta.abs())) + (Lk + 64 + Lq) * U32 * ds.abs()
+    add = lambda t: torch.zeros(td.shape[0], dtype=torch.float64, device=q.device).index_add_(0, at.reshape(-1), t.reshape(-1))  # noqa: E731
+    dtable = add(ds)
+    return dict(y=y, dtable=dtable), dict(y=ty, dtable=add(te) * (1 + half_step(dt)) + half_step(dt) * dtable.abs() + tiny(dt))
+
+
+TIGHT = [(300, 300, 32, 3, 2), (70, 400, 64, 3, 2), (33, 200, 128, 3, 2), (5, 2000, 64, 3, 2), (1, 9, 8, 100, 64)]   # (the last: one bucket, so dtable is 0)
+
+
+def tight_inputs(gen, Lq, Lk, D, H, dt):
+    r = lambda *s: torch.randn(*s, device=gen.device, generator=gen).to(dt)  # noqa: E731
+    return r(Lq, H, D), r(Lk, H, D), r(Lk, H, D), r(Lq, H, D), r(16, H)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("Lq,Lk,D,start,H", TIGHT)
+def test_attention_rounds_its_results_alone(Lq, Lk, D, start, H, dtype):
+    """o and dtable within one rounding of their own: the forward's weights are not rounded to 16 bits, nor is what delta is taken from."""
+    dt, lut = DT[dtype], ops.relative_buckets(16, 30)
+    ins = tight_inputs(gen_of(Lq + Lk), Lq, Lk, D, H, dt)
+    leaves = [t[None].requires_grad_(True) for t in ins[:3]] + [ins[4].requires_grad_(True)]
+    y = M.biased_attention(*leaves, lut, q_start=start)
+    dtable = torch.autograd.grad(y, leaves[3], ins[3][None])[0]
+    for h in range(H):
+        want, tol = tight_reference(*(t.detach()[:, h] for t in ins), lut, start)
+        for name, got in (("y", y[0, :, h]), ("dtable", dtable[:, h])):
+            far = (got.detach().double() - want[name]).abs() / tol[name]
+            assert float(far.max()) <= 1.0, (name, h, float(far.max()))
+
+
+# -------------------------------------------------------------------------------------------------------------- whole layers, closer
+@pytest.mark.parametrize("held,dtype,gtol", [(torch.float32, torch.bfloat16, 8.5e-2), (torch.float32, torch.float16, 3e-2), (torch.bfloat16, torch.bfloat16, 8.5e-2),
+                                             (torch.float16, torch.float16, 3e-2), (torch.bfloat16, torch.float32, 3e-5), (torch.bfloat16, torch.float16, 3e-2)])
+def test_decoder_layer_gradients(held, dtype, gtol, monkeypatch):
+    """Every gradient of the layer, parameters held in any type, against 64 bits (relative 2-norms).  The bounds are those that test_gpu_layer_train derives for the
+    ReLU's sqrt(2 p), twice that for a parameter, and half a step of its type.  The gradient of a place that is sampled jumps at a cell's edge, and a few of 26880 places lie
+    over one for a rounding of their arguments (one that did carried 84 % of the error of embed's gradient here); so the formulas take the places that the layer took,
+    which leaves no such step, and the sampling's parameters are held to the same bounds (fp32 activations: ten times those, the offsets' terms over their sums)."""
+    from oracle import track_oracle as O
+    from test_gpu_layer_train import decoder_case, double_of, fill, off, oracle_layer
+    layer = fill(M.MOTRDecoderLayer(256, 8, 512, 0.0, None, 3, 4), 23).to("cuda", held)
+    shapes, embed, pos, feats, box, dy = decoder_case(24)
+    rnd = lambda t: t.to(dtype).double()  # noqa: E731
+    dev = [t.to("cuda", dtype).requires_grad_(True) for t in (embed, pos, feats)]
+    places, sample, core = [], M.MSDeformAttnFunction.apply, O.msda_core
+    monkeypatch.setattr(M.MSDeformAttnFunction, "apply", lambda v, sizes, first, loc, aw, step: (places.append(loc.detach().cpu().double()), sample(v, sizes, first, loc, aw, step))[1])
+    out = layer.forward_train(dev[0], box.cuda(), dev[2], shapes, track_query_pos=dev[1])
+    out.backward(dy.to("cuda", dtype))
+    monkeypatch.setattr(O, "msda_core", lambda v, sizes, loc, aw: core(v, sizes, loc + (places[0] - loc).detach(), aw))
+    sd, by = double_of(layer, "l")
+    ref = [rnd(t).requires_grad_(True) for t in (embed, pos, feats)]
+    want = oracle_layer(shapes, ref[0], box.double(), ref[2], ref[1], sd)
+    want.backward(rnd(dy))
+    assert len(places) == 1 and off(out, want) < {torch.float32: 3e-5, torch.float16: 6e-3, torch.bfloat16: 4e-2}[dtype]
+    for name, a, b in zip(("embed", "pos", "feats"), dev, ref):
+        assert off(a.grad, b.grad) < gtol + half_step(dtype), (name, off(a.grad, b.grad))
+    for n, p in layer.named_parameters():
+        bound = gtol * (10 if dtype == torch.float32 and ("sampling_offsets" in n or "attention_weights" in n) else 2)
+        assert p.grad.dtype == held and off(p.grad, by[n].grad) < bound + half_step(held), (n, off(p.grad, by[n].grad))

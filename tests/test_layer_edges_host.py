@@ -124,3 +124,33 @@ def test_linear_strides_that_the_entry_points_take():
         assert query(True, M=2, **kw) == _lib.ENOSYS, kw
     assert query(M=33, ldr=far) >= 0                                           # (no residual)
     assert query(M=33, ldx=512 * 4096) >= 0 and query(K=1 << 22, ldx=1 << 22, ldw=1 << 22) == _lib.ENOSYS
+
+
+
+def test_the_tight_bounds_see_a_rounded_weight_and_a_rounded_output():
+    """The bounds of test_gpu_layer_edges.test_attention_rounds_its_results_alone, on the CPU with the roundings planted: weights rounded to 16 bits miss them for y, and
+    a delta from the rounded output misses them for dtable; weights as two operands and a delta with what the rounding left out do not."""
+    import test_gpu_layer_edges as E
+    lut = ops.relative_buckets(16, 30, device="cpu")
+    for dt in (torch.bfloat16, torch.float16):
+        seen = dict(y=False, dtable=False)
+        for Lq, Lk, D, start, H in E.TIGHT:
+            ins = E.tight_inputs(torch.Generator().manual_seed(Lq + Lk), Lq, Lk, D, H, dt)
+            at = lut.long()[(torch.arange(Lk)[None] - torch.arange(Lq)[:, None] - start).clamp(-30, 30) + 30]
+            for h in range(H):
+                q, k, v, do, table = (t[:, h] for t in ins)
+                want, tol = E.tight_reference(q, k, v, do, table, lut, start)
+                qd, kd, vd, g = (t.double() for t in (q, k, v, do))
+                p = torch.softmax(qd @ kd.t() * D ** -0.5 + table.double()[at], -1)
+                r = lambda t: t.to(dt).double()  # noqa: E731
+                top = p.amax(-1, keepdim=True)
+                w = p / top                                                        # as the kernel holds them: the largest 1
+                two = (r(w) + r(w - r(w))) @ vd * top
+                by = lambda delta: torch.zeros(16, dtype=torch.float64).index_add_(0, at.reshape(-1), (p * (g @ vd.t() - delta)).reshape(-1))  # noqa: E731
+                o, one = r(two), r(r(w) @ vd * top)
+                good = dict(y=o, dtable=r(by((g * (o + r(two - o))).sum(-1, keepdim=True))))
+                bad = dict(y=one, dtable=r(by((g * o).sum(-1, keepdim=True))))
+                for name in want:
+                    assert bool(((good[name] - want[name]).abs() <= tol[name]).all()), (name, dt, Lq)
+                    seen[name] |= bool(((bad[name] - want[name]).abs() > tol[name]).any())
+        assert all(seen.values()), (dt, seen)
