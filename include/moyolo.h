@@ -659,7 +659,7 @@ int64_t moy_attention_bwd_ws(const moy_attention_args* args);
  * x T [M, K] (ldx), w T [N, K] (ldw), any sizes and alignments of T, strides >= 0; b [N] fp32 or T (b_dtype), r T [M, N] (ldr) optional; act MOY_ACT_*.
  * y T [M, N] (ldy); z T [M, N] dense: written if given, read by the backward where act is not MOY_ACT_NONE.  dx / dw T dense, db b_dtype: each optional,
  * one at least given.  Rows up to 4 MiB long, and no further
- * apart unless there is one or (forward) at most 32 rows of x (else MOY_ENOSYS).  ws: moy_linear_ws / moy_linear_bwd_ws BYTES, 16-byte aligned (0: none needed;
+ * apart unless there is one, or the forward has at most 32 rows of x of up to 2048 elements, or at most 16 in fp32 (else MOY_ENOSYS).  ws: moy_linear_ws / moy_linear_bwd_ws BYTES, 16-byte aligned (0: none needed;
  * negative: a MOY_E* code).  Sums are fp32 in an order that the sizes fix; 16-bit types round dz (and the z of the backward) to T;
  * a finite z stays finite there, and one that is not 0 keeps its sign. */
 typedef struct moy_linear_args {

@@ -8,7 +8,7 @@
 // nothing is transposed in memory.  fp32 products are exact (16x16x4); 16-bit ones run 16x16x32.  Both operands go from memory straight into LDS
 // (128 bytes of k to a tile row, XOR-swizzled by way of the lanes' source addresses, what lies outside a matrix arrives as zeros), double-buffered
 // with one barrier per tile of k.  Products with too few tiles for the chip are split over k: fp32 partial results, joined in order by a second kernel that
-// also runs the epilogue.  Up to 32 rows (a new token of each sequence) take lin_few_kernel, which streams W once through registers.
+// also runs the epilogue.  Few rows (a new token of each sequence) take lin_few_kernel, which streams W once through registers.
 // Measured: 8192 x 4096 -> 4096 bf16 forward with z and a residual 240 to 260 us, dx 231, dW 227 (1.06 to 1.21 PFLOP/s, a large library product 1.22); 4800 x 256 -> 1024 14, 12,
 // 10 + 4; 1803 x 514 -> 770 fp32 35, 31 + 9, 28 + 6; one row of 1024 -> 4096 4.8: bound by the matrix cores' feeding, launches, the fp32 matrix rate, the trip to memory.
 // dz is its own pass (it feeds two products and the sums of db; in the products' prologues it would be recomputed for every column tile).
@@ -635,9 +635,12 @@ static bool lin_direct(const void* p, int64_t ld, int n, int es) {
 static int64_t lin_span(int64_t rows, int64_t ld, int64_t n, int es) { return ((rows - 1) * ld + n) * es; }
 static int64_t lin_pitch(int n, int es) { return ((int64_t)n * es + 15) / 16 * 16 / es; }
 
-// Few rows go through lin_few_kernel (us, against the tiled kernel, bf16: 1 row 256 -> 256 3.6 / 4.6, 1024 -> 4096 4.1 / 7.9, 4096 -> 4096 10.5 / 10.0; 16 rows 2.9 / 4.6, 4.4 / 7.9,
-// 10.0 / 10.8; 32 rows 3.3 / 4.7, 5.3 / 8.0, 14.1 / 12.4).
-static bool lin_few(int M) { return M <= 32; }
+// Few rows go through lin_few_kernel, which asks for W in one wave of loads after another: up to 32 rows of up to 2048 elements, up to 16 of any length in fp32, whose tiled
+// kernel pays four times as much for the rows that are not there (us, against the tiled kernel; 1, 16, 32 rows.  bf16: 256 -> 256 3.6 / 4.5, 2.9 / 4.6, 3.3 / 4.7;
+// 1024 -> 4096 4.2 / 7.9, 4.4 / 8.0, 5.5 / 8.0; 2048 -> 4096 6.3 / 7.5, 6.4 / 8.1, 8.4 / 8.8; 4096 -> 1024 8.0 / 7.3, 9.5 / 8.4, 13.0 / 8.6; 4096 -> 4096 10.5 / 9.8, 9.9 / 10.6,
+// 14.1 / 12.4; 8192 -> 8192 31.7 / 24.3, 31.9 / 24.9, 45.7 / 25.3.  fp32: 1024 -> 4096 6.1 / 11.5, 7.0 / 12.1, 9.4 / 13.2; 2048 -> 2048 8.7 / 12.0, 11.1 / 12.6, 15.5 / 13.5;
+// 4096 -> 1024 14.8 / 12.2, 17.8 / 12.7, 26.9 / 13.2; 4096 -> 4096 19.3 / 25.6, 19.3 / 25.8, 28.1 / 26.1; 8192 -> 8192 55 / 80, 65 / 80, 102 / 81).
+static bool lin_few(int M, int K, int es) { return M <= (K <= 2048 ? 32 : es == 4 ? 16 : 0); }
 
 template <typename T, bool ACOL, bool BCOL>
 static int lin_gemm(LinParams p, float* part, hipStream_t st) {
@@ -690,7 +693,7 @@ static int lin_check(const moy_linear_args* a, bool bwd) {
   const int d = a->dtype;
   if (!a->x || !a->w || !aligned_as(a->x, d) || !aligned_as(a->w, d) || (a->M > 1 && a->ldx < 0) || (a->N > 1 && a->ldw < 0)) return MOY_EINVAL;
   // rows up to 4 MiB long, and no further apart where the tiled kernel addresses them (by 32-bit offsets within a tile); lin_few_kernel takes any distance
-  const bool few = !bwd && lin_few(a->M);
+  const bool few = !bwd && lin_few(a->M, a->K, lin_es(d));
   auto apart = [&](int64_t ld, int rows) { return !few && rows > 1 && ld > (1 << 22) / lin_es(d); };
   if ((int64_t)a->K * lin_es(d) > (1 << 22) || (int64_t)a->N * lin_es(d) > (1 << 22) || apart(a->ldx, a->M) || apart(a->ldw, a->N)) return MOY_ENOSYS;
   if ((int64_t)((a->M + 63) / 64) * ((a->N + 63) / 64) * 16 > 0x7fffffffLL || (int64_t)((a->M + 63) / 64) * ((a->K + 63) / 64) * 16 > 0x7fffffffLL) return MOY_ENOSYS;
@@ -717,7 +720,7 @@ struct LinPlan {
 static LinPlan lin_plan(const moy_linear_args* a, bool bwd) {
   const int es = lin_es(a->dtype);
   LinPlan p{};
-  const bool few = !bwd && lin_few(a->M);                                       // (takes any rows)
+  const bool few = !bwd && lin_few(a->M, a->K, es);                            // (takes any rows)
   p.pad_x = !few && (!bwd || a->dw) && !lin_direct(a->x, a->ldx, a->K, es);
   p.pad_w = !few && (!bwd || a->dx) && !lin_direct(a->w, a->ldw, a->K, es);
   int64_t at = 0;
@@ -741,7 +744,7 @@ static LinPlan lin_plan(const moy_linear_args* a, bool bwd) {
     if (a->db) at += lin_round((int64_t)p.sum_rows * a->N * 4);
   } else {
     p.part = at;
-    if (!lin_few(a->M)) at += lin_part_bytes(a->M, a->N, a->K, es);
+    if (!few) at += lin_part_bytes(a->M, a->N, a->K, es);
   }
   p.total = at;
   return p;
@@ -764,7 +767,7 @@ static int lin_fwd(const moy_linear_args* a, const LinPlan& plan, hipStream_t st
   p.M = a->M; p.N = a->N; p.K = a->K;
   p.bias = a->b; p.bias_dtype = a->b_dtype; p.act = a->act;
   p.r = a->r; p.ldr = a->ldr; p.y = a->y; p.ldy = a->ldy; p.z = a->z; p.ldz = a->N;
-  if (lin_few(a->M)) {
+  if (lin_few(a->M, a->K, sizeof(T))) {
     p.vec = p.N % 4 == 0 && p.ldy % 4 == 0 && reinterpret_cast<uintptr_t>(p.y) % (4 * sizeof(T)) == 0 &&
             (!p.z || reinterpret_cast<uintptr_t>(p.z) % (4 * sizeof(T)) == 0) && (!p.r || (p.ldr % 4 == 0 && reinterpret_cast<uintptr_t>(p.r) % (4 * sizeof(T)) == 0));
     const dim3 grid((unsigned)((a->N + 15) / 16));

@@ -593,8 +593,8 @@ def _linear_check(x, weight, bias, act, residual):
 
 def linear_forward(x, weight, bias=None, act=L.ACT_NONE, residual=None, keep_pre=False):
     """act(x weight^T + bias) + residual (moy_linear): x [..., K], weight [N, K] of one type (float32 / bfloat16 / float16), bias [N] in it or float32,
-    residual [..., N]; rows of up to 4 MiB at any strides and alignments (16-bit rows of odd length or at odd elements, and more than
-    32 rows that lie over 4 MiB apart, cost a copy).  -> y, or with keep_pre (y, z):
+    residual [..., N]; rows of up to 4 MiB at any strides and alignments (16-bit rows of odd length or at odd elements, and rows that lie
+    over 4 MiB apart, unless they are few, cost a copy).  -> y, or with keep_pre (y, z):
     z = what act was applied to, as linear_backward takes it (None for ACT_NONE)."""
     _linear_check(x, weight, bias, act, residual)
     y, z = L.host().linear_forward(x, weight, bias, act, residual, keep_pre)

@@ -372,3 +372,13 @@ def test_decoder_layer_gradients(held, dtype, gtol, monkeypatch):
     for n, p in layer.named_parameters():
         bound = gtol * (10 if dtype == torch.float32 and ("sampling_offsets" in n or "attention_weights" in n) else 2)
         assert p.grad.dtype == held and off(p.grad, by[n].grad) < bound + half_step(held), (n, off(p.grad, by[n].grad))
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("M", [1, 16, 17, 32, 33])
+@pytest.mark.parametrize("K", [2048, 2049, 4096])
+def test_linear_either_side_of_the_kernel_for_few_rows(M, K, dtype):
+    from test_gpu_layer_ops import check_linear
+    dt, gen = DT[dtype], gen_of(M + K)
+    N = 200
+    check_linear(rand(gen, M, K, dtype=dt), rand(gen, N, K, dtype=dt, scale=K ** -0.5), rand(gen, N, dtype=dt), rand(gen, M, N, dtype=dt), "silu", rand(gen, M, N, dtype=dt))

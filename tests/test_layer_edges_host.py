@@ -115,9 +115,11 @@ def test_linear_strides_that_the_entry_points_take():
             setattr(a, n, x)
         return (_lib.lib().moy_linear_bwd_ws if bwd else _lib.lib().moy_linear_ws)(C.byref(a))
     far = 513 * 4096                                                           # elements of 16 bits: 4 KiB over the limit
-    for kw in (dict(ldx=far), dict(ldx=1 << 40, ldy=1 << 40, r=0x10000, ldr=1 << 40), dict(M=2, ldx=far), dict(M=32, ldx=1 << 33, ldw=1 << 33), dict(M=40, N=1, ldw=1 << 40)):
+    for kw in (dict(ldx=far), dict(ldx=1 << 40, ldy=1 << 40, r=0x10000, ldr=1 << 40), dict(M=16, ldx=far, dtype=_lib.F32), dict(M=32, K=2048, ldx=1 << 33, ldw=1 << 33), dict(M=40, N=1, ldw=1 << 40)):
         assert query(**kw) >= 0, kw
     assert query(True, ldx=1 << 40, ldd=1 << 40) >= 0 and query(True, M=40, N=1, ldw=1 << 40) >= 0
+    for kw in (dict(M=2, ldx=far), dict(M=17, ldx=far, dtype=_lib.F32)):
+        assert query(**kw) == _lib.ENOSYS, kw
     for kw in (dict(ldx=far), dict(ldw=far), dict(ldy=far), dict(r=0x10000, ldr=far)):
         assert query(M=33, **kw) == _lib.ENOSYS, kw
     for kw in (dict(ldx=far), dict(ldw=far), dict(ldd=far)):
