@@ -1168,10 +1168,6 @@ static void attn_splits(const moy_attention_args* a, int* tiles, int* splits, in
   *splits = (a->Lk + *keys - 1) / *keys;
 }
 
-static int attn_lds_opt_in(const void* kern) {
-  return hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024) == hipSuccess ? MOY_OK : MOY_ELAUNCH;
-}
-
 static size_t attn_bias_bytes(const moy_attention_args* a) { return a->table ? (2 * (size_t)a->max_distance + 12) / 4 * 16 : 0; }
 
 // 16-bit heads of 40 to 64: 32 queries (keys) to a wave where that leaves two blocks to a compute unit (8 x 1024 x 8 heads of 64: forward 43 us against 48, dQ
@@ -1183,8 +1179,9 @@ template <typename T, int DP, int NQ, bool MASK>
 static int attn_fwd_tiles(const moy_attention_args* a, AttnParams p, hipStream_t st) {
   constexpr int BK = attn_bk<T, DP>();
   auto kern = attn_fwd_kernel<T, DP, NQ, BK, MASK>;
-  static const int ready = attn_lds_opt_in(reinterpret_cast<const void*>(kern));
-  if (ready != MOY_OK) return ready;
+  static std::atomic<uint64_t> ready{0};
+  const int rc = lds_opt_in(reinterpret_cast<const void*>(kern), ready);
+  if (rc != MOY_OK) return rc;
   p.tiles = (a->Lq + 64 * NQ - 1) / (64 * NQ);
   const size_t lds = 4 * Tile<T, DP, BK, 256>::BYTES + 2 * MaskTile<64 * NQ, BK>::BYTES + attn_bias_bytes(a);
   hipLaunchKernelGGL(kern, dim3((unsigned)(a->B * a->H * p.tiles)), dim3(256), lds, st, p);
@@ -1212,8 +1209,9 @@ template <typename T, int DP, int NQ, bool MASK>
 static int attn_dq(const moy_attention_args* a, AttnParams p, hipStream_t st) {
   constexpr int BK = attn_bk<T, DP>();
   auto kern = attn_dq_kernel<T, DP, NQ, BK, MASK>;
-  static const int ready = attn_lds_opt_in(reinterpret_cast<const void*>(kern));
-  if (ready != MOY_OK) return ready;
+  static std::atomic<uint64_t> ready{0};
+  const int rc = lds_opt_in(reinterpret_cast<const void*>(kern), ready);
+  if (rc != MOY_OK) return rc;
   const size_t bias = attn_bias_bytes(a), lds = 4 * Tile<T, DP, BK, 256>::BYTES + 2 * MaskTile<64 * NQ, BK>::BYTES + bias + (p.part ? 4 * 4 * (16 * 68 + 2 * (size_t)a->max_distance + 1) : 0);
   p.tiles = (a->Lq + 64 * NQ - 1) / (64 * NQ);
   hipLaunchKernelGGL(kern, dim3((unsigned)(a->B * a->H * p.tiles)), dim3(256), lds, st, p);
@@ -1224,8 +1222,9 @@ template <typename T, int DP, int NK, bool MASK>
 static int attn_dkv(const moy_attention_args* a, AttnParams p, hipStream_t st) {
   constexpr int BQ = attn_bk<T, DP>();
   auto kern = attn_dkv_kernel<T, DP, NK, BQ, MASK>;
-  static const int ready = attn_lds_opt_in(reinterpret_cast<const void*>(kern));
-  if (ready != MOY_OK) return ready;
+  static std::atomic<uint64_t> ready{0};
+  const int rc = lds_opt_in(reinterpret_cast<const void*>(kern), ready);
+  if (rc != MOY_OK) return rc;
   const size_t lds = 4 * Tile<T, DP, BQ, 256>::BYTES + 2 * MaskTile<BQ, 64 * NK>::BYTES + 16 * BQ + attn_bias_bytes(a);
   p.tiles = (a->Lk + 64 * NK - 1) / (64 * NK);
   hipLaunchKernelGGL(kern, dim3((unsigned)(a->B * a->Hk * p.tiles)), dim3(256), lds, st, p);

@@ -1,5 +1,6 @@
 // Shared device helpers for the gfx950 kernels of libmoyolo.so (wave64 everywhere).
 #pragma once
+#include <atomic>
 #include <cstdio>
 #include <cstdlib>
 #include <hip/hip_runtime.h>
@@ -212,6 +213,17 @@ __device__ __forceinline__ uint32_t fdiv(uint32_t n, const FastDiv& f) {
 inline int launch_status() {
   hipError_t e = hipGetLastError();
   return e == hipSuccess ? MOY_OK : MOY_ELAUNCH;
+}
+
+// 160 KB of LDS for a kernel that asks for it at its launch.  The attribute is the current device's own: `done` (one for each kernel) has a bit for each device.
+inline int lds_opt_in(const void* kern, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess) return MOY_ELAUNCH;
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (done.load(std::memory_order_relaxed) & bit) return MOY_OK;
+  if (hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024) != hipSuccess) return MOY_ELAUNCH;
+  done.fetch_or(bit, std::memory_order_relaxed);
+  return MOY_OK;
 }
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }

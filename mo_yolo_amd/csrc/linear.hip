@@ -659,8 +659,9 @@ static int lin_gemm(LinParams p, float* part, hipStream_t st) {
 #define MOY_LIN(WM, WN, MI, NI, ST)                                                                                                     \
   {                                                                                                                                 \
     auto kern = lin_gemm_kernel<T, ACOL, BCOL, WM, WN, MI, NI, ST>;                                                                     \
-    static const bool ready = hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024) == hipSuccess; \
-    if (!ready) return MOY_ELAUNCH;                                                                                                 \
+    static std::atomic<uint64_t> ready{0};                                                                                              \
+    const int rc = lds_opt_in(reinterpret_cast<const void*>(kern), ready);                                                              \
+    if (rc != MOY_OK) return rc;                                                                                                    \
     hipLaunchKernelGGL(kern, grid, dim3(WM * WN * 64), ST * 128 * (WM * MI * 16 + WN * NI * 16), st, p);                               \
   }
   if (sizeof(T) == 2 && k.tile == 256) {

@@ -382,3 +382,16 @@ def test_linear_either_side_of_the_kernel_for_few_rows(M, K, dtype):
     dt, gen = DT[dtype], gen_of(M + K)
     N = 200
     check_linear(rand(gen, M, K, dtype=dt), rand(gen, N, K, dtype=dt, scale=K ** -0.5), rand(gen, N, dtype=dt), rand(gen, M, N, dtype=dt), "silu", rand(gen, M, N, dtype=dt))
+
+
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="wants two devices")
+def test_a_second_device():
+    """Each device is asked for its kernels' LDS; the current one stays as it is."""
+    for f, args in calls(gen_of(9)):
+        runs = []
+        for dev in ("cuda:0", "cuda:1"):
+            leaves = [a.detach().to(dev).requires_grad_(True) for a in args]
+            y = f(*leaves) if leaves[0].dim() == 2 else M.biased_attention(*leaves, ops.relative_buckets(8, 8, device=dev), q_start=0)
+            runs.append([t.cpu() for t in (y, *torch.autograd.grad(y, leaves, torch.ones_like(y)))])
+            assert torch.cuda.current_device() == 0
+        assert all(torch.equal(a, b) for a, b in zip(*runs))
