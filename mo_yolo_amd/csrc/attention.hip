@@ -8,7 +8,9 @@
 // exact products of K = 4 at a time in the same register layout.  In 16-bit types the forward's P enters its product as two operands, its rounded value and
 // what that leaves out: the backward takes dO . O for sum_j P_ij dP_ij, and what O missed of that would not cancel in dtable, where rows of dS add up
 // to 0 (a quarter of the forward's time at 2 x 4096; without it dtable was up to 2.4 times, o 1.4 times as far off as one rounding).  P and dS of the
-// backward are rounded once, like the results they go into.  The products are laid out so that
+// backward are rounded to 16 bits once: nothing there adds up to 0, and dq, dk and dv are 2.4e-3 off in norm (bf16, 2 x 4096) where the rounding of an exact result alone makes
+// 1.7e-3; both as two operands made it that, for 233 us of dQ instead of 206 and 281 of dK and dV instead of 215.  Who wants neither rounding computes in fp32.
+// The products are laid out so that
 // probabilities never leave registers: S^T = K Q^T puts a query in a lane's column and four consecutive keys in its accumulator, which is (keys permuted
 // alike on both sides) the operand that O^T = V^T P^T takes.  V^T, K^T, Q^T, dO^T operands come out of row-major LDS tiles through the transposing LDS
 // read (16-bit) or by single elements (fp32).  A row's maximum, sum, delta and position are one lane's scalars; only the maximum crosses lanes.
@@ -18,10 +20,13 @@
 // delta, sums of dtable); attn_dkv_kernel (dK, dV: a block owns keys and walks the queries of every head that shares them).  The two backward kernels
 // compute S twice instead of adding dQ atomically: results do not depend on the order in which blocks run.
 //
-// Measured: 2 x 4096 causal, 16 heads of 64, bf16: forward 148 us, dQ 205, dK and dV 213 (465, 500 and 645 TFLOP/s); bound by what the vector units
-// do around the matrix cores (the exponential, its argument, maximum, sum and packing: some 220 instructions a wave of the forward for 64 keys x 32 queries, beside 48
-// matrix instructions), at two or three waves to a SIMD.  16 x 300 with a mask by query, 8 heads of 32, fp16: 17, 25, 19: five tiles to a block, latency.
-// One query for each of 32 caches of up to 16384 keys, 16 heads over 4 key heads of 64: 77.6 us and 4.7 to join, 5.1 TB/s over the keys that count.
+// Measured: 2 x 4096 causal, 16 heads of 64, bf16: forward 152 us, dQ 208, dK and dV 217 (450, 495 and 635 TFLOP/s).  By its counters the forward is bound by the vector units: they
+// are busy 73 % of the time (320 instructions of a wave for 64 keys x 32 queries, 32 of them exponentials at four times the price), the matrix cores 35 % (48 instructions), at 2.7
+// waves to a SIMD.  dQ and dK / dV keep the vector units busy for 51 and 52 %, the matrix cores for 24 and 31 %, the LDS for 21 and 25 %: their registers leave 1.9 waves to a SIMD,
+// each of which waits a third of its time for data, with too little beside it to fill in.  Heads of 128 take 277, 394 and 523, heads of 96 as much (they are padded to 128), at 16
+// queries or keys to a wave.  fp32, 4 x 1024 causal, 16 heads of 64: 109, 171, 185.  16 x 300 with a mask by query, 8 heads of 32, fp16: 17, 26, 19: five tiles to a block, latency.
+// One query for each of 32 caches of up to 16384 keys, 16 heads over 4 key heads of 64: 78 us and 4.8 to join, 5.1 TB/s over the keys that count; full caches of 16384, heads of 64
+// in fp32 or of 128 in bf16 193 and 197 (5.5), of 128 in fp32 423 (5.1, with 20 bytes of a lane spilled).  The backward does not split the keys: 16 queries, 4096 keys, 8 heads of 64 are eight blocks and 86 us of dQ.
 #include "common.hpp"
 
 namespace moy {

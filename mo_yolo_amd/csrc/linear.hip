@@ -9,9 +9,14 @@
 // (128 bytes of k to a tile row, XOR-swizzled by way of the lanes' source addresses, what lies outside a matrix arrives as zeros), double-buffered
 // with one barrier per tile of k.  Products with too few tiles for the chip are split over k: fp32 partial results, joined in order by a second kernel that
 // also runs the epilogue.  Few rows (a new token of each sequence) take lin_few_kernel, which streams W once through registers.
-// Measured: 8192 x 4096 -> 4096 bf16 forward with z and a residual 240 to 260 us, dx 231, dW 227 (1.06 to 1.21 PFLOP/s, a large library product 1.22); 4800 x 256 -> 1024 14, 12,
-// 10 + 4; 1803 x 514 -> 770 fp32 35, 31 + 9, 28 + 6; one row of 1024 -> 4096 4.8: bound by the matrix cores' feeding, launches, the fp32 matrix rate, the trip to memory.
+// Measured (a trace's best and median): 8192 x 4096 -> 4096 bf16 forward with z and a residual 252 to 279 us, dx 231 to 258, dW 224 to 249 (1.09, 1.19 and 1.23 PFLOP/s at best, a
+// large library product 1.22); 4800 x 256 -> 1024 14.6, 12, 10 + 4; 1803 x 514 -> 770 fp32 35, 32 + 9, 28 + 5; 4096 x 2048 -> 2048 fp32 320, 334, 356 (0.11 PFLOP/s, the library 0.14);
+// one row of 1024 -> 4096 4.7, fp32 6.7: bound by the matrix cores' feeding, launches, the fp32 matrix rate, the trip to memory.
 // dz is its own pass (it feeds two products and the sums of db; in the products' prologues it would be recomputed for every column tile).
+// In 16-bit types z is kept, and dz enters its products, rounded to T once, which the matrix cores ask of an operand: gradients of SiLU at the large size are 2.4e-3 off in norm, where
+// the rounding of an exact result alone makes 1.7e-3; a second operand with what the rounding leaves out would make it that, for twice the matrix work of dx and dW (some 480 us of 721).
+// Without an activation, and for ReLU, nothing is rounded but the results.  A z off by half a step moves a derivative by up to that step's size relative to itself (SiLU and sigmoid at
+// 10 in bf16: 4 %, of a derivative of 5e-4 and less).  db is summed before dz is rounded.  Who wants neither rounding computes in fp32.
 // Loads are 16 bytes from any dword on; where a row ends inside one, the tail is cleared in LDS.  16-bit rows of odd length or at odd elements are
 // copied into padded rows first.
 #include <type_traits>

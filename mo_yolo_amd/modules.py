@@ -511,7 +511,7 @@ class MOTRDecoderLayer(nn.Module):
         return self.linear2.rows(h, R=e2, ln=self.norm3.pair(dev))
 
     def forward_train(self, embed, refer_bbox, feats, shapes, padding_mask=None, attn_mask=None, track_query_pos=None, rel_bias=None):
-        """forward for training (transformer.py:627-652 with its masks): embed / track_query_pos [bs, Lq, C], refer_bbox [bs, Lq, 4] in (0, 1), feats [bs, S, C];
+        """forward for training (transformer.py:627-652 with its masks; no dropout, whatever the layer was built with): embed / track_query_pos [bs, Lq, C], refer_bbox [bs, Lq, 4] in (0, 1), feats [bs, S, C];
         padding_mask bool [bs, S] (True: no feature there), attn_mask and rel_bias as _MHA.forward_train.  float32 / bfloat16 / float16 activations over
         parameters of any of them; gradients for the inputs and every parameter.  (Planned modules -- MYDecoder and those around it -- copy the
         weights when their engine is built: hand trained weights to them with load_state_dict.)"""
