@@ -4,6 +4,7 @@
 // the C ABI (include/moyolo.h) are handed over as addresses, so that whichever build of the library is loaded is the one that is called.
 #include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -47,7 +48,8 @@ int code_of(at::ScalarType t) { return t == at::kFloat ? MOY_F32 : t == at::kBFl
 
 // What records torch's operations (torch.jit.trace, make_fx) sees the outputs made and not the launches that fill them: a replay would return memory that nothing wrote.
 bool not_recorded() {
-  TORCH_CHECK(!torch::jit::tracer::isTracing() && !c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value(),
+  TORCH_CHECK(!torch::jit::tracer::isTracing() && !c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value() &&
+                  !c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::PreDispatch),
               "the transformer-layer operators launch kernels of their own and cannot be recorded by torch.jit.trace or make_fx");
   return true;
 }

@@ -97,8 +97,9 @@ def test_recording_a_trace_is_refused():
     for f, args in _host_calls():
         with pytest.raises(RuntimeError, match="recorded"):
             torch.jit.trace(f, args, check_trace=False)
-        with pytest.raises(RuntimeError, match="recorded"):
-            make_fx(f)(*args)
+        for before_dispatch in (False, True):
+            with pytest.raises(RuntimeError, match="recorded"):
+                make_fx(f, pre_dispatch=before_dispatch)(*args)
 
 
 # ------------------------------------------------------------------------------------------------------------------------ strides
