@@ -99,6 +99,19 @@ variable_list once(variable_list grads, std::initializer_list<const Tensor*> fro
   return all;
 }
 
+// What a backward pass is given comes out of autograd's hands: a saved tensor's hooks or a `.data` that was set in between may have made another type or size of it, and the
+// kernels would read past its end.
+bool like(const Tensor& t, const Tensor& x, at::IntArrayRef sizes) {
+  return t.defined() && t.scalar_type() == x.scalar_type() && t.device() == x.device() && t.sizes() == sizes;
+}
+bool maybe_like(const Tensor& t, const Tensor& x, at::IntArrayRef sizes) { return !t.defined() || like(t, x, sizes); }
+bool block_of(const Tensor& t, const Tensor& x, at::ScalarType type, int64_t n) {
+  return t.defined() && t.scalar_type() == type && t.device() == x.device() && t.numel() == n && t.is_contiguous();
+}
+void as_saved(bool ok, const char* what) {
+  TORCH_CHECK(ok, what, ": a saved tensor or the incoming gradient does not have the forward's size, type or device");
+}
+
 // Which inputs of a Function want a gradient: AutogradContext counts the tensors that were given, this counts all of them.
 struct Wants {
   AutogradContext* ctx;
@@ -139,6 +152,9 @@ std::tuple<Tensor, Tensor> norm_forward(const Tensor& x, const Tensor& w, const 
 
 std::tuple<Tensor, Tensor, Tensor> norm_backward(const Tensor& dy, const Tensor& x, const Tensor& w, const Tensor& stat, const Tensor& r, bool need_x, bool need_w,
                                                  bool need_b, at::ScalarType wtype) {
+  as_saved(x.dim() > 0 && x.size(-1) > 0 && like(dy, x, x.sizes()) && maybe_like(r, x, x.sizes()) && block_of(stat, x, at::kFloat, 2 * (x.numel() / x.size(-1))) &&
+               (!w.defined() || (w.scalar_type() == wtype && w.device() == x.device() && w.sizes() == x.sizes().slice(x.dim() - 1))) && (wtype == at::kFloat || wtype == x.scalar_type()),
+           "layer_norm");
   const On on(x);
   const Tensor x2 = as_rows(x), g2 = as_rows(dy), r2 = as_rows(r), wc = dense(w);
   const int64_t rows = x2.size(0), c = x2.size(1);
@@ -231,6 +247,13 @@ std::tuple<Tensor, Tensor> linear_forward(const Tensor& x, const Tensor& w, cons
 
 std::tuple<Tensor, Tensor, Tensor> linear_backward(const Tensor& dy, const Tensor& x, const Tensor& w, const Tensor& z, int64_t act, bool need_x, bool need_w,
                                                    bool need_b, at::ScalarType btype) {
+  bool ok = x.dim() > 0 && w.dim() == 2 && w.numel() > 0 && like(w, x, {w.size(0), x.size(-1)}) && (btype == at::kFloat || btype == x.scalar_type());
+  if (ok) {
+    auto shape = x.sizes().vec();
+    shape.back() = w.size(0);
+    ok = like(dy, x, shape) && (act == MOY_ACT_NONE || block_of(z, x, x.scalar_type(), x.numel() / x.size(-1) * w.size(0)));
+  }
+  as_saved(ok, "linear");
   const On on(x);
   LinearCall c(x, w, Tensor(), act, Tensor(), dy);
   c.a.b_dtype = code_of(btype);
@@ -340,6 +363,18 @@ std::tuple<Tensor, Tensor, Tensor> attention_forward(const Tensor& q, const Tens
 std::tuple<Tensor, Tensor, Tensor, Tensor> attention_backward(const Tensor& dout, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& o, const Tensor& lse,
                                                               const Tensor& rest, const Tensor& table, const Tensor& lut, const Tensor& k_len, const Tensor& mask,
                                                               const AttentionHow& how, bool nq, bool nk, bool nv, bool nt) {
+  bool ok = q.dim() == 4 && k.dim() == 4 && k.size(2) > 0 && q.size(2) % k.size(2) == 0 && like(k, q, {q.size(0), k.size(1), k.size(2), q.size(3)}) && like(v, q, k.sizes()) &&
+            like(dout, q, q.sizes()) && like(o, q, q.sizes()) && o.is_contiguous() && maybe_like(rest, q, q.sizes()) && (!rest.defined() || rest.is_contiguous()) &&
+            block_of(lse, q, at::kFloat, q.size(0) * q.size(1) * q.size(2)) && table.defined() == lut.defined();
+  if (ok && table.defined())
+    ok = table.dim() == 2 && like(table, q, {table.size(0), q.size(2)}) && lut.dim() == 1 && lut.size(0) % 2 == 1 && lut.scalar_type() == at::kByte && lut.device() == q.device();
+  if (ok && k_len.defined()) ok = k_len.dim() == 1 && k_len.size(0) == q.size(0) && k_len.scalar_type() == at::kInt && k_len.device() == q.device();
+  if (ok && mask.defined()) {
+    const int64_t d = mask.dim(), want[4] = {q.size(0), q.size(2), q.size(1), k.size(1)};
+    ok = (d == 2 || d == 4) && mask.element_size() == 1 && mask.device() == q.device() && mask.size(d - 1) == want[3];
+    for (int64_t i = 0; ok && i < d - 1; ++i) ok = mask.size(i) == 1 || mask.size(i) == want[4 - d + i];
+  }
+  as_saved(ok, "attention");
   const On on(q);
   const auto type = q.scalar_type();
   nt = nt && table.defined();

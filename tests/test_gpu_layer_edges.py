@@ -395,3 +395,20 @@ def test_a_second_device():
             runs.append([t.cpu() for t in (y, *torch.autograd.grad(y, leaves, torch.ones_like(y)))])
             assert torch.cuda.current_device() == 0
         assert all(torch.equal(a, b) for a, b in zip(*runs))
+
+
+# ------------------------------------------------------------------------------------------------------------------- saved tensors
+def test_saved_tensors_that_went_through_hooks():
+    """Kept on the host and brought back: the same gradients.  Brought back in another type or size: an error."""
+    for f, args in calls(gen_of(10), torch.bfloat16):
+        every = [a.clone().requires_grad_(True) for a in args]
+        y = f(*every)
+        want = torch.autograd.grad(y, every, torch.ones_like(y))
+        with torch.autograd.graph.save_on_cpu():
+            y = f(*every)
+        assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y, every, torch.ones_like(y)), want))
+        for change in (lambda t: t.float() if t.dtype == torch.bfloat16 else t, lambda t: t[:1] if t.dtype == torch.bfloat16 else t):
+            with torch.autograd.graph.saved_tensors_hooks(lambda t: t, change):
+                y = f(*every)
+            with pytest.raises(RuntimeError, match="forward's size"):
+                torch.autograd.grad(y, every, torch.ones_like(y))

@@ -157,3 +157,27 @@ def test_the_tight_bounds_see_a_rounded_weight_and_a_rounded_output():
                     assert bool(((good[name] - want[name]).abs() <= tol[name]).all()), (name, dt, Lq)
                     seen[name] |= bool(((bad[name] - want[name]).abs() > tol[name]).any())
         assert all(seen.values()), (dt, seen)
+
+
+# ------------------------------------------------------------------------------------------------------------------- saved tensors
+def test_backward_refuses_what_the_forward_did_not_save():
+    """Another type or size of any tensor that a backward pass is given is an error before a kernel could read past its end."""
+    h, code = _lib.host(), torch.float32
+    x, w = torch.ones(6, 8, dtype=torch.bfloat16), torch.ones(8)
+    W, z = torch.ones(5, 8, dtype=torch.bfloat16), torch.ones(6, 5, dtype=torch.bfloat16)
+    q, k, t = (torch.ones(*s, dtype=torch.bfloat16) for s in ((2, 5, 4, 8), (2, 7, 2, 8), (8, 4)))
+    lut, n, m, lse = ops.relative_buckets(8, 8, device="cpu"), torch.ones(2, dtype=torch.int32), torch.zeros(5, 7, dtype=torch.bool), torch.ones(2, 4, 5)
+    norm = (lambda dy, x, w, stat, r: h.layer_norm_backward(dy, x, w, stat, r, True, True, True, code), (x, x, w, torch.ones(2, 6), x))
+    linear = (lambda dy, x, w, z: h.linear_backward(dy, x, w, z, _lib.ACT_SILU, True, True, True, code), (z, x, W, z))
+    attention = (lambda *a: h.attention_backward(*a, False, False, 0, 1.0, True, True, True, True), (q, q, k, k, q, lse, q, t, lut, n, m))
+    for f, args in (norm, linear, attention):
+        with pytest.raises(RuntimeError) as e:                                 # as they were: only the missing GPU stops them
+            f(*args)
+        assert "forward's size" not in str(e.value)
+        for i, a in enumerate(args):
+            other = torch.float64 if a.dtype == torch.float32 else torch.float32
+            # (of the statistics and of z the count is what matters; a table of any length goes with a map that is clamped to it)
+            counted, table = a is lse or f is norm[0] and i == 3 or f is linear[0] and i == 3, a is t
+            for bad in (a.to(other), a[..., :-1], *([] if table else [torch.cat((a, a))]), *([] if counted else [a[None]])):
+                with pytest.raises(RuntimeError, match="forward's size"):
+                    f(*[bad if j == i else b for j, b in enumerate(args)])
