@@ -83,16 +83,19 @@ class _ParamModule(nn.Module):
 
     def _prepared(self, dev, dtype, build):
         prep, params = self._prep, list(self.parameters())
-        if prep.trained and any(p.requires_grad for p in params):
+        key = (str(dev), dtype, *((p.data_ptr(), 0 if p.is_inference() else p._version) for p in params))
+        capturing = dev.type == "cuda" and torch.cuda.is_current_stream_capturing()
+        trains = prep.trained and any(p.requires_grad for p in params)
+        if trains:
             prep.key = prep.data = prep.held = None
+        if trains or (capturing and prep.key != key):        # (what a capture lays out is written by its replays alone)
             with torch.no_grad():
                 return build(dev, dtype)
-        key = (str(dev), dtype, *((p.data_ptr(), 0 if p.is_inference() else p._version) for p in params))
         if prep.key != key:
             with torch.no_grad():
                 prep.data, prep.held = build(dev, dtype), [p.detach() for p in params]
             prep.key = key
-        if dev.type == "cuda" and torch.cuda.is_current_stream_capturing() and not any(prep.data is d for d in prep.captured):
+        if capturing and not any(prep.data is d for d in prep.captured):
             prep.captured.append(prep.data)
         return prep.data
 

@@ -111,6 +111,33 @@ def test_a_captured_forward_follows_the_weights():
         assert torch.equal(out, want)
 
 
+def test_weights_laid_out_in_a_capture_stay_in_its_graph():
+    """A layer whose first inference call is captured: an eager call before any replay lays out its own, and a replay after an update uses the new weights."""
+    warm, layer = (M.MOTRDecoderLayer(256, 8, 512, 0.0, None, 3, 4).cuda() for _ in range(2))
+    shapes, embed, pos, feats, box = layer_case(gen_of(12))
+    run = lambda layer: layer(embed, box, feats, shapes, track_query_pos=pos)  # noqa: E731
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.no_grad():
+        with torch.cuda.stream(side):
+            run(warm)
+            torch.cuda.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=side):
+                out = run(layer)
+        torch.cuda.synchronize()
+        want = run(layer)
+        warm.load_state_dict(layer.state_dict())
+        assert torch.equal(want, run(warm))
+        for _ in range(2):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want) and torch.equal(run(layer), want)
+            for p in layer.parameters():
+                p.mul_(0.9)
+            want = run(layer)
+
+
 # ------------------------------------------------------------------------------------------------------------- what 16 bits cannot hold
 @pytest.mark.parametrize("rows", [2, 40, 700])
 @pytest.mark.parametrize("n", [64, 37])
