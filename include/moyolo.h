@@ -633,6 +633,7 @@ int64_t moy_layer_norm_bwd_ws(int64_t rows, int C, int dtype);    /* floats, or 
  * Rows of k / v from k_len on are not read, nor those that a mask without query and head strides (m_sq == m_sh == 0) hides; with causal, rows behind the last
  * query's position are not read either.  A key that such a rule does not hide has to be finite wherever any query counts it or not (its weight 0 still
  * multiplies it).
+ * B * H * ceil(Lq / 64), and backwards B * Hk * ceil(Lk / 64), below 2^24 (else MOY_ENOSYS).
  * ws: fp32 workspace of moy_attention_ws / moy_attention_bwd_ws floats (0: none needed; negative: a MOY_E* code).
  * Backward: dout T [B, Lq, H, D] strided (g_*), the forward's o and lse; dq dense like o, dk / dv dense [B, Lk, Hk, D] (zeros from k_len on), dtable T
  * [num_buckets, H]; each optional, one at least given.  16-bit types: the forward's P enters its product as two operands (its rounded value and the
@@ -659,7 +660,8 @@ int64_t moy_attention_bwd_ws(const moy_attention_args* args);
  * x T [M, K] (ldx), w T [N, K] (ldw), any sizes and alignments of T, strides >= 0; b [N] fp32 or T (b_dtype), r T [M, N] (ldr) optional; act MOY_ACT_*.
  * y T [M, N] (ldy); z T [M, N] dense: written if given, read by the backward where act is not MOY_ACT_NONE.  dx / dw T dense, db b_dtype: each optional,
  * one at least given.  Rows up to 4 MiB long, and no further
- * apart unless there is one, or the forward has at most 32 rows of x of up to 2048 elements, or at most 16 in fp32 (else MOY_ENOSYS).  ws: moy_linear_ws / moy_linear_bwd_ws BYTES, 16-byte aligned (0: none needed;
+ * apart unless there is one, or the forward has at most 32 rows of x of up to 2048 elements, or at most 16 in fp32; M up to 2^31 - 512
+ * (else MOY_ENOSYS).  ws: moy_linear_ws / moy_linear_bwd_ws BYTES, 16-byte aligned (0: none needed;
  * negative: a MOY_E* code).  Sums are fp32 in an order that the sizes fix; 16-bit types round dz (and the z of the backward) to T;
  * a finite z stays finite there, and one that is not 0 keeps its sign. */
 typedef struct moy_linear_args {

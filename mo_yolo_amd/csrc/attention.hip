@@ -1106,6 +1106,28 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(const AttnParams p) {
 // -------------------------------------------------------------------------------------------------------------------------------- host
 static bool attn_stride_ok(int64_t s, int es) { return s >= 0 && s * es % 16 == 0; }
 
+// The keys are split where there are few rows, or too few blocks of 64 queries to fill the chip, and keys enough to pay for the join (us, split against whole: bf16
+// heads of 64, 8 x 8 heads over 2, 4 queries, 4096 keys 13.0 / 72; 8 heads, 64 queries, 4096 keys 16.5 / 72, 1024 keys 11.8 / 20.6, 300 keys 11.5 / 9.2; 64 x 8 heads, 16 queries,
+// 1024 keys 46.5 / 43.4; 512 x 8 heads of 32, 8 queries, 300 keys 64 / 43; fp32, whose products take longer, 3 x 6 heads of 40, 77 queries, 401 keys 14.8 / 26).
+static bool attn_uses_split(const moy_attention_args* a) {
+  if (a->Lk < (a->dtype == MOY_F32 ? 256 : 512)) return false;
+  return (int64_t)a->Lq * (a->H / a->Hk) <= 16 || (int64_t)a->B * a->H * ((a->Lq + 63) / 64) < 128;
+}
+
+// Splits of at least 256 keys (two 32-key tiles to a wave), as many as give sixteen blocks to a compute unit, of which four fit at a time: sequences differ in
+// length, and what follows fills in (32 caches of up to 16384 keys, 4 key heads of 64: 90.6 us with four blocks, 84.7 with eight, 77.6 with sixteen).  64 at most.
+static void attn_splits(const moy_attention_args* a, int* tiles, int* splits, int* keys) {
+  const int rows = a->Lq * (a->H / a->Hk);
+  *tiles = (rows + 15) / 16;
+  const int64_t blocks = (int64_t)a->B * a->Hk * *tiles;
+  int64_t s = (4096 + blocks - 1) / blocks;
+  const int64_t most = (a->Lk + 255) / 256;
+  if (s > most) s = most;
+  if (s > 64) s = 64;
+  *keys = (int)(((a->Lk + s - 1) / s + 127) / 128 * 128);
+  *splits = (a->Lk + *keys - 1) / *keys;
+}
+
 static int attn_check(const moy_attention_args* a, bool bwd) {
   if (!a || a->dtype < MOY_F32 || a->dtype > MOY_F16) return MOY_EINVAL;
   const int es = a->dtype == MOY_F32 ? 4 : 2;
@@ -1123,6 +1145,15 @@ static int attn_check(const moy_attention_args* a, bool bwd) {
   if (a->mask && (a->m_sb < 0 || a->m_sh < 0 || a->m_sq < 0)) return MOY_EINVAL;
   if (!(a->scale >= 0.f) || !(a->scale - a->scale == 0.f) || (a->o_rest && !aligned16(a->o_rest))) return MOY_EINVAL;
   if ((int64_t)a->B * a->H > (1 << 24) || (int64_t)a->B * a->H * ((a->Lq > a->Lk ? a->Lq : a->Lk) / 64 + 1) > 0x7fffffffLL / 8) return MOY_EINVAL;
+  // every launch has a grid that can be launched
+  const int64_t heads = (int64_t)a->B * a->H, groups = (int64_t)a->B * a->Hk;
+  if (!bwd && attn_uses_split(a)) {
+    int tiles, splits, keys;
+    attn_splits(a, &tiles, &splits, &keys);
+    if (!grid_fits(groups * tiles * splits, 256) || !grid_fits(heads * a->Lq, 256)) return MOY_ENOSYS;
+  } else if (!grid_fits(heads * ((a->Lq + 63) / 64), 256) || (bwd && !grid_fits(groups * ((a->Lk + 63) / 64), 256))) {
+    return MOY_ENOSYS;
+  }
   if (bwd) {
     const int64_t gs[] = {a->g_sb, a->g_sl, a->g_sh};
     for (int64_t s : gs)
@@ -1149,28 +1180,6 @@ static AttnParams attn_params(const moy_attention_args* a) {
   p.dout = a->dout; p.g_sb = a->g_sb; p.g_sl = a->g_sl; p.g_sh = a->g_sh;
   p.dq = a->dq; p.dk = a->dk; p.dv = a->dv;
   return p;
-}
-
-// The keys are split where there are few rows, or too few blocks of 64 queries to fill the chip, and keys enough to pay for the join (us, split against whole: bf16
-// heads of 64, 8 x 8 heads over 2, 4 queries, 4096 keys 13.0 / 72; 8 heads, 64 queries, 4096 keys 16.5 / 72, 1024 keys 11.8 / 20.6, 300 keys 11.5 / 9.2; 64 x 8 heads, 16 queries,
-// 1024 keys 46.5 / 43.4; 512 x 8 heads of 32, 8 queries, 300 keys 64 / 43; fp32, whose products take longer, 3 x 6 heads of 40, 77 queries, 401 keys 14.8 / 26).
-static bool attn_uses_split(const moy_attention_args* a) {
-  if (a->Lk < (a->dtype == MOY_F32 ? 256 : 512)) return false;
-  return (int64_t)a->Lq * (a->H / a->Hk) <= 16 || (int64_t)a->B * a->H * ((a->Lq + 63) / 64) < 128;
-}
-
-// Splits of at least 256 keys (two 32-key tiles to a wave), as many as give sixteen blocks to a compute unit, of which four fit at a time: sequences differ in
-// length, and what follows fills in (32 caches of up to 16384 keys, 4 key heads of 64: 90.6 us with four blocks, 84.7 with eight, 77.6 with sixteen).  64 at most.
-static void attn_splits(const moy_attention_args* a, int* tiles, int* splits, int* keys) {
-  const int rows = a->Lq * (a->H / a->Hk);
-  *tiles = (rows + 15) / 16;
-  const int64_t blocks = (int64_t)a->B * a->Hk * *tiles;
-  int64_t s = (4096 + blocks - 1) / blocks;
-  const int64_t most = (a->Lk + 255) / 256;
-  if (s > most) s = most;
-  if (s > 64) s = 64;
-  *keys = (int)(((a->Lk + s - 1) / s + 127) / 128 * 128);
-  *splits = (a->Lk + *keys - 1) / *keys;
 }
 
 static size_t attn_bias_bytes(const moy_attention_args* a) { return a->table ? (2 * (size_t)a->max_distance + 12) / 4 * 16 : 0; }

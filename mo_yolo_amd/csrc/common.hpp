@@ -215,6 +215,9 @@ inline int launch_status() {
   return e == hipSuccess ? MOY_OK : MOY_ELAUNCH;
 }
 
+// A launch counts its threads in 32 bits: one of 2^32 or more would run the rest of that division, with no error.
+inline bool grid_fits(int64_t blocks, int threads) { return blocks > 0 && blocks <= (int64_t)0xffffffffll / threads; }
+
 // 160 KB of LDS for a kernel that asks for it at its launch.  The attribute is the current device's own: `done` (one for each kernel) has a bit for each device.
 inline int lds_opt_in(const void* kern, std::atomic<uint64_t>& done) {
   int dev = 0;

@@ -211,10 +211,10 @@ struct LinearCall {
     a.x = x.data_ptr(); a.ldx = row_stride(x); a.w = w.data_ptr(); a.ldw = row_stride(w);
     a.r = ptr(r); a.ldr = row_stride(r); a.dy = ptr(dy); a.ldd = row_stride(dy);
   }
-  bool compact() {
+  bool compact() {                         // (what lies further apart than that, if anything)
     bool any = false;
     for (Tensor* t : {&x, &w, &r, &dy})
-      if (t->defined() && !t->is_contiguous()) {
+      if (t->defined() && t->size(0) > 1 && t->stride(0) * t->element_size() > (1 << 22)) {
         *t = t->contiguous();
         any = true;
       }

@@ -587,13 +587,14 @@ __global__ __launch_bounds__(256) void lin_dz_kernel(const T* __restrict__ dy, i
 template <typename T>
 __global__ __launch_bounds__(256) void lin_pad_kernel(const T* __restrict__ src, int64_t ld, int64_t rows, int n, T* __restrict__ dst, int64_t pitch) {
   using K = Chunk<T>;
-  const int64_t chunks = pitch / K::VEC, x = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (x >= rows * chunks) return;
-  const int64_t row = x / chunks;
-  const int c = (int)(x - row * chunks) * K::VEC;
-  float v[K::VEC];
-  K::load(src + row * ld + c, n - c, v);
-  K::store(dst + row * pitch + c, K::VEC, v);
+  const int64_t chunks = pitch / K::VEC;
+  for (int64_t x = (int64_t)blockIdx.x * 256 + threadIdx.x; x < rows * chunks; x += (int64_t)gridDim.x * 256) {
+    const int64_t row = x / chunks;
+    const int c = (int)(x - row * chunks) * K::VEC;
+    float v[K::VEC];
+    K::load(src + row * ld + c, n - c, v);
+    K::store(dst + row * pitch + c, K::VEC, v);
+  }
 }
 
 // -------------------------------------------------------------------------------------------------------------------------------- host
@@ -611,7 +612,7 @@ static LinPick lin_pick(int M, int N, int K, int es) {
   static const struct { int tile; double shared[2], alone[2], block, launch; } kind[3] = {
       {64, {455, 1367}, {624, 2100}, 1500, 8700}, {128, {1214, 5500}, {1170, 5500}, 3000, 13500}, {256, {3825, 0}, {2930, 0}, 8000, 20400}};
   const int nk = (int)(((int64_t)K * es + 127) / 128), wide = es == 4;
-  LinPick best{64, 1, nk};
+  LinPick best{128, 1, nk};
   double least = 0;
   for (const auto& q : kind) {
     if (q.tile == 256 && wide) break;                                          // (fp32: 3 times the 64-row tiles' time)
@@ -619,6 +620,8 @@ static LinPick lin_pick(int M, int N, int K, int es) {
     for (int s = 1; s <= 16 && (s == 1 || (q.tile < 256 && nk / s >= 4)); ++s) {
       const int per = (nk + s - 1) / s;
       if ((nk + per - 1) / per != s) continue;                                 // (the same as a smaller split)
+      // (lin_check has seen to it that one does)
+      if (!grid_fits(tiles * s, q.tile == 256 ? 512 : 256) || (s > 1 && !grid_fits(((int64_t)M * ((N + 3) / 4) + 255) / 256, 256))) continue;
       const double busy = (double)((tiles * s + 255) / 256);
       const double work = per * (busy * q.shared[wide] > q.alone[wide] ? busy * q.shared[wide] : q.alone[wide]);
       const double cost = work + busy * q.block + q.launch + (s > 1 ? 10000 + (double)(s + 1) * M * N * 4 / 2000 : 0);
@@ -688,8 +691,8 @@ static int64_t lin_part_bytes(int M, int N, int K, int es) {
 
 template <typename T>
 static int lin_pad(const void* src, int64_t ld, int64_t rows, int n, void* dst, int64_t pitch, hipStream_t st) {
-  const int64_t chunks = rows * (pitch / Chunk<T>::VEC);
-  hipLaunchKernelGGL((lin_pad_kernel<T>), dim3((unsigned)((chunks + 255) / 256)), dim3(256), 0, st, static_cast<const T*>(src), ld, rows, n, static_cast<T*>(dst), pitch);
+  const int64_t blocks = (rows * (pitch / Chunk<T>::VEC) + 255) / 256, most = 1 << 20;   // (blocks beyond that go round again)
+  hipLaunchKernelGGL((lin_pad_kernel<T>), dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, st, static_cast<const T*>(src), ld, rows, n, static_cast<T*>(dst), pitch);
   return launch_status();
 }
 
@@ -702,8 +705,9 @@ static int lin_check(const moy_linear_args* a, bool bwd) {
   const bool few = !bwd && lin_few(a->M, a->K, lin_es(d));
   auto apart = [&](int64_t ld, int rows) { return !few && rows > 1 && ld > (1 << 22) / lin_es(d); };
   if ((int64_t)a->K * lin_es(d) > (1 << 22) || (int64_t)a->N * lin_es(d) > (1 << 22) || apart(a->ldx, a->M) || apart(a->ldw, a->N)) return MOY_ENOSYS;
-  if ((int64_t)((a->M + 63) / 64) * ((a->N + 63) / 64) * 16 > 0x7fffffffLL || (int64_t)((a->M + 63) / 64) * ((a->K + 63) / 64) * 16 > 0x7fffffffLL) return MOY_ENOSYS;
-  if ((int64_t)a->M * (a->N > a->K ? a->N : a->K) / 4 / 256 > 0x3fffffffLL) return MOY_ENOSYS;
+  // row numbers a tile past the last one are still whole numbers of 32 bits, and each product has a grid that can be launched (in 128-row tiles, if in no others)
+  auto fits = [](int64_t m, int64_t n) { return grid_fits((m + 127) / 128 * ((n + 127) / 128), 256); };
+  if (a->M > 0x7fffffff - 512 || (!bwd && !fits(a->M, a->N)) || (bwd && ((a->dx && !fits(a->M, a->K)) || (a->dw && !fits(a->N, a->K))))) return MOY_ENOSYS;
   if (!bwd) {
     if (apart(a->ldy, a->M) || (a->r && apart(a->ldr, a->M))) return MOY_ENOSYS;
     if (!a->y || !aligned_as(a->y, d) || (a->M > 1 && a->ldy < a->N) || !aligned_as(a->b, a->b_dtype)) return MOY_EINVAL;

@@ -439,3 +439,23 @@ def test_saved_tensors_that_went_through_hooks():
                 y = f(*every)
             with pytest.raises(RuntimeError, match="forward's size"):
                 torch.autograd.grad(y, every, torch.ones_like(y))
+
+
+# -------------------------------------------------------------------------------------------------------------------- largest sizes
+def test_linear_of_more_rows_than_a_launch_of_small_tiles_counts():
+    """2^30 rows and some: 64-row tiles would be 2^32 threads and some, of which a launch runs the rest."""
+    n = (1 << 30) + 64
+    x, w = torch.full((n, 8), 0.5, device="cuda", dtype=torch.bfloat16), torch.ones(8, 8, device="cuda", dtype=torch.bfloat16)
+    x[n // 2], x[-1] = 1.0, 2.0
+    y = ops.linear_forward(x, w)
+    for i, want in ((0, 4.0), (n // 2, 8.0), (n - 1, 16.0), (64, 4.0), (n - 65, 4.0)):
+        assert bool((y[i] == want).all()), i
+    assert float(y.view(-1).narrow(0, 0, 1 << 30).amin()) == 4.0
+    dx = ops.linear_backward(y, x, w, need=(True, False, False))[0]
+    assert bool((dx[-1] == 128.0).all()) and bool((dx[5] == 32.0).all()) and bool((dx[n // 2] == 64.0).all())
+
+
+def test_attention_of_more_heads_than_a_launch_counts_is_refused():
+    q = torch.zeros(1, 1, 8, 8, device="cuda", dtype=torch.bfloat16).expand(1 << 21, 1, 8, 8)
+    with pytest.raises(RuntimeError, match="not implemented"):
+        ops.attention_forward(q, q, q)

@@ -181,3 +181,31 @@ def test_backward_refuses_what_the_forward_did_not_save():
             for bad in (a.to(other), a[..., :-1], *([] if table else [torch.cat((a, a))]), *([] if counted else [a[None]])):
                 with pytest.raises(RuntimeError, match="forward's size"):
                     f(*[bad if j == i else b for j, b in enumerate(args)])
+
+
+# -------------------------------------------------------------------------------------------------------------------- largest sizes
+def test_sizes_whose_launches_would_count_past_32_bits_are_refused():
+    """The workspace queries answer as the calls do."""
+    a = _lib.AttentionArgs()
+    for n in ("q", "k", "v", "o", "dout", "lse", "dq"):
+        setattr(a, n, 0x10000)
+    a.H, a.Hk, a.Lq, a.Lk, a.D, a.scale, a.dtype = 8, 8, 1, 1, 8, 0.125, _lib.BF16
+    forward, backward = (lambda f=f, **kw: [setattr(a, n, x) for n, x in kw.items()] and f(C.byref(a)) for f in (_lib.lib().moy_attention_ws, _lib.lib().moy_attention_bwd_ws))
+    assert forward(B=(1 << 21) - 1) == 0 and backward(B=(1 << 21) - 1) > 0
+    assert forward(B=1 << 21) == backward(B=1 << 21) == _lib.ENOSYS
+    assert forward(B=1 << 20, Lq=65) == _lib.ENOSYS and forward(B=1 << 20, Lq=64) == 0
+    assert forward(B=1 << 20, Lq=1, Lk=65) == 0 and backward(B=1 << 20, Lq=1, Lk=130) == _lib.ENOSYS       # (the gradients of keys walk the keys)
+    assert forward(B=1 << 15, Lq=1, Lk=16384) == 0 and forward(B=1 << 21, Lq=1, Lk=600) == _lib.ENOSYS    # (the kernel for few queries)
+
+    def linear(bwd=False, **kw):
+        b = _lib.LinearArgs()
+        b.x = b.w = b.y = b.dy = b.dx = 0x10000
+        b.N, b.K, b.ldx, b.ldw, b.ldy, b.ldd, b.dtype = 8, 8, 8, 8, 8, 8, _lib.BF16
+        for n, x in kw.items():
+            setattr(b, n, x)
+        return (_lib.lib().moy_linear_bwd_ws if bwd else _lib.lib().moy_linear_ws)(C.byref(b))
+    for bwd in (False, True):
+        assert linear(bwd, M=(1 << 30) + 64) >= 0 and linear(bwd, M=0x7fffffff - 512) >= 0
+        assert linear(bwd, M=0x7fffffff - 511) == _lib.ENOSYS
+    wide = dict(M=1 << 30, N=1 << 20, K=1 << 20, ldw=1 << 20, ldx=1 << 20, ldy=1 << 20, ldd=1 << 20)
+    assert linear(**wide) == linear(True, **wide) == _lib.ENOSYS
